@@ -228,14 +228,14 @@ def plan_of(s):
     if c["op"] == "cache4":
         units = s["units"].tolist()
         m = capi.QuantizedMixer(dense, back, rot, c["heads"], c["kv_heads"], c["dim"], int(c["gated"]), s["scale"], units[0], units[1])
-        need = lib.tbl_quantized_workspace_bytes(C.byref(m), precision, c["seqs"], c["tokens"], c["context"])
+        need = lib.tbl_quantized_workspace_bytes(C.byref(m), precision, 0, c["seqs"], c["tokens"], c["context"])
         space = torch.empty(need, dtype=torch.uint8, device="cuda")
         cache = (p("cache"), c["seqs"], s["capacity"])
         calls = [(lib.tbl_quantized_forward, (C.byref(m), precision, 0, EPS, p("proj"), *cache, *where, c["context"], p("out"), space.data_ptr(), need)),
                  (lib.tbl_quantized_read, (C.byref(m), capi.F32, *cache, *where, p("keys"), p("values")))]
         return calls, (s["out"], s["keys"], s["values"]), (m, space, lib, capi)
     m = capi.DecayMixer(dense, back, rot, p("log_decay"), p("norm"), c["heads"], c["dim"], int(c["gated"]), s["scale"])
-    need = lib.tbl_decay_workspace_bytes(C.byref(m), precision, c["seqs"], c["tokens"])
+    need = lib.tbl_decay_workspace_bytes(C.byref(m), precision, 0, c["seqs"], c["tokens"])
     space = torch.empty(need, dtype=torch.uint8, device="cuda")
     args = (C.byref(m), precision, 0, EPS, p("proj"), p("states"), p("next"), *where, p("out"), space.data_ptr(), need)
     return [(lib.tbl_decay_forward, args)], (s["out"], s["next"]), (m, space, lib, capi)
