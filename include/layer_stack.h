@@ -33,6 +33,8 @@ extern "C" {
 #define TBL_MIXER_GENERAL_DELTA 0
 #define TBL_MIXER_LATENT_ATTENTION 1
 #define TBL_MIXER_ATTENTION 2
+#define TBL_MIXER_QUANTIZED_ATTENTION 3
+#define TBL_MIXER_DECAY_ATTENTION 4
 
 #define TBL_NORM_RMS 0               /* x / sqrt(mean x^2 + eps) * weight                       */
 #define TBL_NORM_DYNAMIC_TANH 1      /* tanh(alpha x) * weight + bias                           */
@@ -44,6 +46,7 @@ extern "C" {
 #define TBL_MAX_DELTA_DIM 256        /* key/value size of a delta-rule head                      */
 #define TBL_MAX_LATENT 1024          /* latent size + rotated part of a latent-attention layer   */
 #define TBL_MAX_ATTENTION_DIM 512    /* query/key size of one map, and value size, of an attention head */
+#define TBL_MAX_ROTATED_DIM 256      /* head size where heads are normed and rotated: quantized and decay attention */
 #define TBL_MAX_STREAMS 8            /* residual streams of a model with hyper-connections       */
 #define TBL_PAIR_BLOCK 32            /* gate / up rows of a feed-forward alternate in blocks of this many rows */
 
@@ -96,6 +99,48 @@ typedef struct tbl_attention_mixer {
     float scale, lambda, out_scale;
 } tbl_attention_mixer;
 
+/* Norm and rotation of query and key heads, every head by itself, in one pass:
+ *   y = x / sqrt(mean x^2 + eps) * norm        (norm [dim], the same for all heads; NULL: y = x)
+ * then the first rot_dim dimensions turn by the angle of the position: a pair (a, b) with entry i of the tables becomes
+ * (a cos - b sin, b cos + a sin).  Pair i is (i, i + rot_dim/2), or with `interleaved` (2i, 2i + 1).  rot_dim even, 0: no rotation
+ * (and no tables).  Tables fp32 [rope_positions, rot_dim/2]. */
+typedef struct tbl_head_rotation {
+    const float *q_norm, *k_norm;
+    const float *rope_cos, *rope_sin;
+    int rot_dim, rope_positions, interleaved;
+} tbl_head_rotation;
+
+/* Softmax attention over a cache that holds keys and values in 4 bits: `heads` query heads share `kv_heads` key/value heads
+ * (query head h uses h / (heads / kv_heads)), causal.  Queries and keys are normed and rotated (tbl_head_rotation) before keys are
+ * rounded.  `in` stacks W_q (heads*dim rows, head by head) | W_k (kv_heads*dim) | W_v (kv_heads*dim) | W_g (heads*dim, only when gated).
+ *   score = scale * (q . k), output: the softmax average of the values [* sigmoid(W_g h)], then `out`.
+ * What the cache holds of a key x (fp32, worked out in 64 bits: no code depends on the order of a sum) or a value x (fp32), with u =
+ * key_scale or value_scale, for every 16 neighbouring dimensions of a head:
+ *   s = e4m3(min(max |x| / (6 u), 448)),   code = e2m1(x / (s u)),   the number is code s u;
+ * all roundings to nearest, ties to even, e2m1 ends at 6; s = 0 makes all codes 0; a group with a number that is not finite is 16 NaNs.
+ * key_scale and value_scale are finite and > 0: chosen so that max |x| / (6 u) of ordinary groups is far from e4m3's ends, 2^-9 and 448.
+ * A cached token of a head is a row of tbl_quantized_row_bytes: with n = dim rounded up to 64, n/2 bytes of key codes (the even
+ * dimension in the low half of a byte), n/2 of value codes, n/16 scales of the key, n/16 of the value, then zeros to a multiple of 16. */
+typedef struct tbl_quantized_mixer {
+    tbl_dense_view in, out;
+    tbl_head_rotation rotation;
+    int heads, kv_heads, dim, gated;
+    float scale, key_scale, value_scale;
+} tbl_quantized_mixer;
+
+/* Linear attention with a constant decay for each head: with q and k normed and rotated (tbl_head_rotation),
+ *   S <- exp(log_decay) S + v k^T,   o = scale S q
+ * ([value][key], fp32).  o is divided by its root mean square per head (eps of the model's norms) and multiplied by norm [heads*dim]
+ * (NULL: neither) and, when gated, by sigmoid(W_g h); then `out`.  `in` stacks W_q | W_k | W_v (heads*dim rows each) | W_g (heads*dim, only
+ * when gated).  log_decay fp32 [heads] <= 0 on the device; -infinity: a token remembers nothing before it. */
+typedef struct tbl_decay_mixer {
+    tbl_dense_view in, out;
+    tbl_head_rotation rotation;
+    const float *log_decay, *norm;
+    int heads, dim, gated;
+    float scale;
+} tbl_decay_mixer;
+
 /* Hyper-connection of one sublayer with `streams` residual streams x_s (fp32 arrays):
  *   input = sum_s in[s] x_s,   x_t <- sum_s mix[s*streams + t] x_s + out[t] * sublayer(norm(input)). */
 typedef struct tbl_hyper {
@@ -123,6 +168,8 @@ typedef struct tbl_stack_layer {
     tbl_tanh_norm tanh1, tanh2;      /* models with TBL_NORM_DYNAMIC_TANH        */
     tbl_hyper hyper1, hyper2;        /* models with streams: of the mixer, of the feed-forward */
     int activation;                  /* TBL_ACT_* of the feed-forward            */
+    tbl_quantized_mixer quantized;
+    tbl_decay_mixer decay;
 } tbl_stack_layer;
 
 typedef struct tbl_stack_model {
@@ -138,8 +185,8 @@ typedef struct tbl_stack_model {
                                         embedding output at first and summed up at the end (no depth average) */
 } tbl_stack_model;
 
-/* Device state of `slots` sequences with room for `capacity` tokens each: positions, delta-rule states (fp32,
- * [head][value][key]), latent caches [token][kv_rank + rot_dim], and attention caches [kv head][token][keys of every map |
+/* Device state of `slots` sequences with room for `capacity` tokens each: positions, delta-rule and decay states (fp32,
+ * [head][value][key]), 4-bit caches [kv head][token][row bytes], latent caches [token][kv_rank + rot_dim], and attention caches [kv head][token][keys of every map |
  * values], each part padded to a multiple of 16 (layers that read another's cache have none).  reset clears one slot (its position and
  * recurrent states), or the whole state when slot < 0: the latter once before the first use, so that cached rows
  * nobody has written hold finite numbers (they are read under a zero weight). */
@@ -206,6 +253,39 @@ int tbl_attention_forward(const tbl_attention_mixer* mixer, int precision, int r
                           void* cache_dev, int slots, int capacity, const int32_t* slots_dev, const int32_t* positions_dev,
                           int n_seq, int n_tok, int context, void* out_dev, void* workspace_dev, size_t workspace_bytes,
                           void* stream);
+/* Norm and rotation of stacked projections proj fp32 [n_seq*n_tok, ld]: q_heads heads of `dim` from column 0 on, then k_heads.  q_dev
+ * [rows, q_heads, dim] and k_dev [rows, k_heads, dim] have the precision's type; either count may be 0 (its pointer is not used then).  Row
+ * sequence*n_tok + t stands at positions_dev[slots_dev[sequence]] + t; a position outside the tables sets TBL_DEV_CACHE_FULL, and its
+ * rows stay as they were.  dim <= TBL_MAX_ROTATED_DIM.  The tables and norms are in place before the call. */
+int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int precision, float eps, const float* proj_dev, int ld, int q_heads,
+                              int k_heads, int dim, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok,
+                              void* q_dev, void* k_dev, void* stream);
+/* Attention over the 4-bit cache on stacked projections proj fp32 [rows, in.outputs]: norm, rotation, rounding and append at
+ * positions_dev[slot] .., attention, output gate -> out (precision's type) [rows, heads*dim].  cache_dev [slots][kv_heads][capacity]
+ * [row bytes], 16-byte aligned; rows behind a sequence's last token are neither used nor written, whatever they hold.  A token past the capacity or the
+ * rotary tables sets TBL_DEV_CACHE_FULL; the rows of its sequence are undefined, the cache holds what has room.  positions_dev is not
+ * advanced, so that a repeated call writes the same rows again.  route: 0 as the step, 1 SIMT over expanded keys and values, 2 the
+ * cache-streaming kernel (warp-level MMAs on the 4-bit rows), 3 the flash kernel (tcgen05) over expanded keys and values, as far as its
+ * tiles have room (dim <= 192); 2 and 3 take bf16 only.  A number that is not finite reaches the rows that see its token, and may reach those of the same call and sequence before it. */
+int tbl_quantized_row_bytes(const tbl_quantized_mixer* mixer);
+size_t tbl_quantized_workspace_bytes(const tbl_quantized_mixer* mixer, int precision, int route, int n_seq, int n_tok, int context);
+int tbl_quantized_forward(const tbl_quantized_mixer* mixer, int precision, int route, float eps, const float* proj_dev, void* cache_dev,
+                          int slots, int capacity, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok, int context,
+                          void* out_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+/* The numbers that cached rows stand for: keys_dev and values_dev (precision's type, either may be NULL) [n_seq*n_tok, kv_heads, dim], of the
+ * tokens at positions_dev[slots_dev[sequence]] + t.  A token outside the capacity sets TBL_DEV_CACHE_FULL, and its rows stay as they were. */
+int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const void* cache_dev, int slots, int capacity,
+                       const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok, void* keys_dev, void* values_dev,
+                       void* stream);
+/* Linear attention with decay on stacked projections proj fp32 [rows, in.outputs]: norm, rotation, recurrence, head norm, output gate -> out
+ * (precision's type) [rows, heads*dim].  states_dev fp32 [slots][heads][dim][dim] are read, next_states_dev (the same array, or another of
+ * its shape) receives those after the last token; slots not named are not touched.  A token past the rotary tables sets TBL_DEV_CACHE_FULL; the rows and
+ * states of its sequence are undefined.  Projections are finite: a prompt is worked out in blocks, in which one that is not spoils other rows.  route: 0 as the step, 1 the scan kernel (any size, fp32
+ * arithmetic), 2 the chunk kernels (tcgen05; bf16, dim <= 128). */
+size_t tbl_decay_workspace_bytes(const tbl_decay_mixer* mixer, int precision, int route, int n_seq, int n_tok);
+int tbl_decay_forward(const tbl_decay_mixer* mixer, int precision, int route, float eps, const float* proj_dev, const float* states_dev,
+                      float* next_states_dev, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok, void* out_dev,
+                      void* workspace_dev, size_t workspace_bytes, void* stream);
 /* One boundary between sublayers with hyper-connections.  streams_dev fp32 [streams] arrays [rows, width] at `stride`
  * floats.  With y_dev (fp32 [rows, width], the last sublayer's result): x_t <- sum_s mix[s, t] x_s + out[t] y, stored in
  * place when `store`; in_weights (NULL: ones) then give u = sum_t in[t] x_t, and h (precision's type) = norm(u), a

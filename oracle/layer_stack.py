@@ -169,6 +169,82 @@ def grouped_attention(h, P, p, cfg, eps, cache):
     return linear(o, P[p + "o"], P.get(p + "o.b"))
 
 
+def rotate_pairs(x, positions, base, dims):
+    """Rotary positions on neighbours: entry 2 i goes with entry 2 i + 1.  x [T, ..., n]."""
+    order = np.concatenate([np.arange(0, dims, 2), np.arange(1, dims, 2), np.arange(dims, np.shape(x)[-1])])
+    y = np.empty(np.shape(x), F)
+    y[..., order] = rotate_half(np.asarray(x, F)[..., order], positions, base, dims)
+    return y
+
+
+def turn_heads(x, norm, rot, positions, eps):
+    """Norm of every head (None: none) and its rotation (None: none): x [T, heads, dim]."""
+    x = np.asarray(x, F) if norm is None else rms_norm(x, norm, eps)
+    if rot is None:
+        return x
+    return (rotate_pairs if rot.get("interleaved") else rotate_half)(x, positions, rot["base"], rot["dims"])
+
+
+def nearest(x, grid):
+    """The value of the ascending grid nearest to each x >= 0; half way: the one of even index; beyond the end: the end."""
+    i = np.clip(np.searchsorted(grid, x, side="right") - 1, 0, len(grid) - 2)
+    low, high = x - grid[i], grid[i + 1] - x
+    return np.where((low > high) | ((low == high) & (i % 2 == 1)), grid[i + 1], grid[i])
+
+
+E2M1 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+E4M3 = np.array([(m / 8 if e == 0 else 1 + m / 8) * 2.0 ** (max(e, 1) - 7) for e in range(16) for m in range(8)][:127])
+
+
+def four_bits(x, scale):
+    """What a 4-bit cache holds of x [..., dim] (taken as fp32): groups of 16 with an e4m3 factor, in units of `scale`."""
+    x, unit = np.asarray(x, np.float32), np.float32(scale)
+    n = x.shape[-1]
+    g = np.pad(x, [(0, 0)] * (x.ndim - 1) + [(0, -n % 16)]).reshape(x.shape[:-1] + (-1, 16))
+    with np.errstate(all="ignore"):
+        s = nearest(np.minimum(np.abs(g).max(-1, keepdims=True) / (unit * np.float32(6)), np.float32(448)).astype(F), E4M3)
+        step = s.astype(np.float32) * unit
+        code = nearest((np.abs(g) / step).astype(F), E2M1)
+        y = np.where(s == 0, 0.0, np.sign(g) * code * s * F(unit))
+    y = np.where(np.isfinite(g).all(-1, keepdims=True), y, np.nan)
+    return y.reshape(x.shape[:-1] + (-1,))[..., :n]
+
+
+def quantized_attention(h, P, p, cfg, eps, cache):
+    """Mixer: h [T, width]; cache is a list of (keys [G, dim], values [G, dim]) as 4 bits hold them."""
+    H, G, d = (cfg[n] for n in ("heads", "kv_heads", "dim"))
+    T, first = len(h), len(cache)
+    pos = np.arange(first, first + T)
+    turn = lambda name, n: turn_heads(linear(h, P[p + name]).reshape(T, n, d), P.get(p + name + ".norm"), cfg.get("rot"), pos, eps)
+    q, k = turn("q", H), turn("k", G)
+    cache.extend(zip(four_bits(k, cfg["key_scale"]), four_bits(linear(h, P[p + "v"]).reshape(T, G, d), cfg["value_scale"])))
+    keys, values = np.array([e[0] for e in cache]), np.array([e[1] for e in cache])
+    o = np.zeros((T, H, d))
+    for t in range(T):
+        n = first + t + 1
+        for i in range(H):
+            o[t, i] = softmax_attention(q[t, i], keys[:n, i // (H // G)], values[:n, i // (H // G)], cfg["scale"])
+    o = o.reshape(T, H * d)
+    return linear(o * sigmoid(linear(h, P[p + "g"])) if p + "g" in P else o, P[p + "o"])
+
+
+def decay_attention(h, P, p, cfg, eps, memory):
+    """Mixer: h [T, width]; memory {"tokens": so far, "states": [heads, value, key]} is updated in place."""
+    H, d = cfg["heads"], cfg["dim"]
+    T, first = len(h), memory["tokens"]
+    pos = np.arange(first, first + T)
+    turn = lambda name: turn_heads(linear(h, P[p + name]).reshape(T, H, d), P.get(p + name + ".norm"), cfg.get("rot"), pos, eps)
+    q, k, v = turn("q"), turn("k"), linear(h, P[p + "v"]).reshape(T, H, d)
+    keep = np.exp(-np.exp(np.asarray(P[p + "decay"], F)))
+    o, S = np.zeros((T, H, d)), memory["states"]
+    for t in range(T):
+        S[:] = keep[:, None, None] * S + v[t][:, :, None] * k[t][:, None, :]
+        o[t] = cfg["scale"] * np.einsum("hvk,hk->hv", S, q[t])
+    memory["tokens"] += T
+    o = rms_norm(o, None, eps).reshape(T, H * d) * np.asarray(P[p + "norm"], F)
+    return linear(o * sigmoid(linear(h, P[p + "g"])) if p + "g" in P else o, P[p + "o"])
+
+
 def streams_in(streams, weights):
     """A sublayer's input: the weighted sum of the residual streams."""
     return sum(F(w) * x for w, x in zip(np.asarray(weights, F), streams))
@@ -202,13 +278,15 @@ class Decoder:
         self.memory: List = []
         for layer in cfg["layers"]:
             m = layer["mixer"]
-            self.memory.append(np.zeros((m["heads"], m["dim"], m["dim"])) if layer["type"] == "general_delta" else [])
+            states = lambda: np.zeros((m["heads"], m["dim"], m["dim"]))
+            self.memory.append(states() if layer["type"] == "general_delta" else {"tokens": 0, "states": states()} if layer["type"] == "decay_attention" else [])
 
     def feed(self, tokens, trace: Optional[list] = None):
         cfg, P, eps = self.cfg, self.P, self.cfg["norm"]["eps"]
         x = embed(P["embed"], tokens, cfg["embedding"]["scale"])
         xs = [x]
-        mixers = {"general_delta": general_delta, "latent_attention": latent_attention}
+        mixers = {"general_delta": general_delta, "latent_attention": latent_attention, "quantized_attention": quantized_attention,
+                  "decay_attention": decay_attention}
         for i, layer in enumerate(cfg["layers"]):
             p = f"l{i}."
             x = x + mixers[layer["type"]](rms_norm(x, P[p + "norm1"], eps), P, p + "mix.", layer["mixer"], eps, self.memory[i])

@@ -113,6 +113,27 @@ class AttentionMixer(C.Structure):
                 ("scale", C.c_float), ("lambda_", C.c_float), ("out_scale", C.c_float)]
 
 
+class HeadRotation(C.Structure):
+    """tbl_head_rotation."""
+
+    _fields_ = [("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rot_dim", C.c_int),
+                ("rope_positions", C.c_int), ("interleaved", C.c_int)]
+
+
+class QuantizedMixer(C.Structure):
+    """tbl_quantized_mixer."""
+
+    _fields_ = [("in_", DenseView), ("out", DenseView), ("rotation", HeadRotation), ("heads", C.c_int), ("kv_heads", C.c_int), ("dim", C.c_int),
+                ("gated", C.c_int), ("scale", C.c_float), ("key_scale", C.c_float), ("value_scale", C.c_float)]
+
+
+class DecayMixer(C.Structure):
+    """tbl_decay_mixer."""
+
+    _fields_ = [("in_", DenseView), ("out", DenseView), ("rotation", HeadRotation), ("log_decay", C.c_void_p), ("norm", C.c_void_p),
+                ("heads", C.c_int), ("dim", C.c_int), ("gated", C.c_int), ("scale", C.c_float)]
+
+
 class Hyper(C.Structure):
     """tbl_hyper."""
 
@@ -131,7 +152,7 @@ class StackLayer(C.Structure):
     _fields_ = [("mixer", C.c_int), ("norm1", C.c_void_p), ("delta", DeltaMixer), ("latent", LatentMixer), ("ff", C.c_int),
                 ("norm2", C.c_void_p), ("gate_up", DenseView), ("down", DenseView), ("depth_weights", C.c_void_p),
                 ("attention", AttentionMixer), ("tanh1", TanhNorm), ("tanh2", TanhNorm), ("hyper1", Hyper), ("hyper2", Hyper),
-                ("activation", C.c_int)]
+                ("activation", C.c_int), ("quantized", QuantizedMixer), ("decay", DecayMixer)]
 
 
 class StackModel(C.Structure):
@@ -143,7 +164,7 @@ class StackModel(C.Structure):
 
 
 F32, BF16 = 0, 1
-MIXER_GENERAL_DELTA, MIXER_LATENT_ATTENTION, MIXER_ATTENTION = 0, 1, 2
+MIXER_GENERAL_DELTA, MIXER_LATENT_ATTENTION, MIXER_ATTENTION, MIXER_QUANTIZED_ATTENTION, MIXER_DECAY_ATTENTION = 0, 1, 2, 3, 4
 NORM_RMS, NORM_DYNAMIC_TANH = 0, 1
 ACT_SILU, ACT_GELU_TANH = 0, 1
 PAIR_BLOCK = 32
@@ -232,6 +253,14 @@ _STACK_SIGNATURES = {
     "tbl_attention_workspace_bytes": (_sz, [C.POINTER(AttentionMixer), _int, _int, _int, _int]),
     "tbl_attention_forward": (_int, [C.POINTER(AttentionMixer), _int, _int, _float, _vp, _vp, _int, _int, _vp, _vp, _int, _int, _int,
                                      _vp, _vp, _sz, _vp]),
+    "tbl_head_rotation_forward": (_int, [C.POINTER(HeadRotation), _int, _float, _vp, _int, _int, _int, _int, _vp, _vp, _int, _int, _vp, _vp, _vp]),
+    "tbl_quantized_row_bytes": (_int, [C.POINTER(QuantizedMixer)]),
+    "tbl_quantized_workspace_bytes": (_sz, [C.POINTER(QuantizedMixer), _int, _int, _int, _int, _int]),
+    "tbl_quantized_forward": (_int, [C.POINTER(QuantizedMixer), _int, _int, _float, _vp, _vp, _int, _int, _vp, _vp, _int, _int, _int, _vp, _vp,
+                                     _sz, _vp]),
+    "tbl_quantized_read": (_int, [C.POINTER(QuantizedMixer), _int, _vp, _int, _int, _vp, _vp, _int, _int, _vp, _vp, _vp]),
+    "tbl_decay_workspace_bytes": (_sz, [C.POINTER(DecayMixer), _int, _int, _int, _int]),
+    "tbl_decay_forward": (_int, [C.POINTER(DecayMixer), _int, _int, _float, _vp, _vp, _vp, _vp, _vp, _int, _int, _vp, _vp, _sz, _vp]),
     "tbl_stream_norm": (_int, [_vp, _sz, _int, _vp, _vp, _vp, _int, _vp, _int, _vp, _int, _int, _int, _float, _float, _vp, _vp, _vp,
                                _vp, _vp]),
     "tbl_depth_norm": (_int, [_vp, _sz, _int, _vp, _int, _vp, _int, _int, _float, _vp, _vp, _vp, _vp]),

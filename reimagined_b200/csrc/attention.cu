@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const Attn
     for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
     const int row = tid >> 4, col = tid & 15;
     const int last = pos0 + min(first + row, total - 1) / p.group;           // last visible token of this thread's row
-    const T* cache = static_cast<const T*>(p.cache) + cache_row(p, slot, g, 0);
+    const T* cache = static_cast<const T*>(p.cache) + cache_row(p, p.by_seq ? seq : slot, g, 0);
     for (int t = t0; t < t1; t += kSimtTokens) {
         __syncthreads();
         for (int i = tid; i < kSimtTokens * p.d; i += kSimtThreads) {
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const Attn
 // ---- merge ----------------------------------------------------------------------------------------------------------------
 // One CTA per (row, head).  128 threads share a map's value columns; of a layer with one map the second half of the CTA
 // takes every other split.
-constexpr int kMergeThreads = 256, kMergeMaxSplits = 1024;
+constexpr int kMergeThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) attention_merge_kernel(const AttnParams p) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kMergeThreads) attention_merge_kernel(const At
             l = fmaf(pl[s], f, l);
         }
         l = warp_sum(l);
-        if (lane == 0) inv_s[warp] = (warp == 0 ? 1.0f : -p.lambda) / l;
+        if (lane == 0) inv_s[warp] = (warp == 0 ? 1.0f : -p.lambda) / l * p.value_scale;
     }
     __syncthreads();
     const int half = tid >> 7, map = p.maps == 2 ? half : 0, s0 = p.maps == 2 ? 0 : half, step = p.maps == 2 ? 1 : 2;
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kMergeThreads) attention_merge_kernel(const At
         for (int w = 0; w < kMergeThreads / 32; ++w) total += red[w];
         f = p.out_scale / sqrtf(total / static_cast<float>(p.vd) + p.eps);
     }
-    const float* gate = p.g_off < 0 ? nullptr : p.proj + static_cast<size_t>(row) * p.ld + p.g_off + head * p.vd;
+    const float* gate = p.gate ? p.gate + static_cast<size_t>(row) * p.ldg + head * p.vd : nullptr;
     T* out = static_cast<T*>(p.out) + (static_cast<size_t>(row) * p.H + head) * p.vd;
     for (int c = tid; c < p.vd; c += kMergeThreads) out[c] = from_f<T>(part[0][c] * f * (gate ? sigmoid_f(gate[c]) : 1.0f));
 }
@@ -241,6 +241,11 @@ int launch_simt(const AttnParams& p, int n_seq, cudaStream_t st) {
     if (p.vd <= 128) return launch_simt_nv<T, 8>(p, n_seq, st);
     if (p.vd <= 256) return launch_simt_nv<T, 16>(p, n_seq, st);
     return launch_simt_nv<T, 32>(p, n_seq, st);
+}
+
+template <typename T>
+int launch_merge(const AttnParams& p, int rows, cudaStream_t st) {
+    return launch_dependent(attention_merge_kernel<T>, dim3(rows, p.H), dim3(kMergeThreads), 0, st, p) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
 
 enum Route { kAuto = 0, kSimt = 1, kStream = 2, kFlash = 3 };
@@ -318,10 +323,17 @@ int run(const tbl_attention_mixer& m, AttnParams p, const Plan& w, int n_seq, cu
         rc = launch_simt<T>(p, n_seq, st);
     }
     if (rc != TBL_OK || !merge) return rc;
-    return launch_dependent(attention_merge_kernel<T>, dim3(rows, p.H), dim3(kMergeThreads), 0, st, p) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+    return launch_merge<T>(p, rows, st);
 }
 
 }  // namespace
+
+int launch_attention_simt(const AttnParams& p, int precision, int n_seq, cudaStream_t st) {
+    return precision == TBL_BF16 ? launch_simt<bf16>(p, n_seq, st) : launch_simt<float>(p, n_seq, st);
+}
+int launch_attention_merge(const AttnParams& p, int precision, int rows, cudaStream_t st) {
+    return precision == TBL_BF16 ? launch_merge<bf16>(p, rows, st) : launch_merge<float>(p, rows, st);
+}
 
 int check_attention(const tbl_attention_mixer& m, int width) {
     if (m.heads <= 0 || m.kv_heads <= 0 || m.heads > 65535 || m.heads % m.kv_heads || m.dim <= 0 || m.vdim <= 0 ||
@@ -365,6 +377,7 @@ int launch_attention(const tbl_attention_mixer& m, int precision, int route, flo
     p.n_slots = n_slots; p.capacity = capacity; p.n_tok = n_tok; p.splits = w.splits;
     p.vec = (p.ld | m.dim | m.vdim) % 4 == 0 && (reinterpret_cast<uintptr_t>(proj) & 15) == 0;
     p.scale_log2 = static_cast<float>(static_cast<double>(m.scale) * 1.4426950408889634); p.lambda = m.lambda; p.out_scale = m.out_scale; p.eps = eps;
+    p.gate = p.g_off < 0 ? nullptr : proj + p.g_off; p.ldg = p.ld; p.value_scale = 1.0f;
     return precision == TBL_BF16 ? run<bf16>(m, p, w, n_seq, st) : run<float>(m, p, w, n_seq, st);
 }
 

@@ -24,6 +24,11 @@ struct AttnParams {
     int H, G, group, maps, d, vd, dp, vp, cw;
     int n_slots, capacity, temperature_positions, n_tok, splits, append, vec;
     float scale_log2, lambda, out_scale, eps;
+    // the merge and flash kernels' gate (null: none), and a factor of one map's output; by_seq: the cache belongs to the step's sequences, not to slots
+    const float* gate;
+    int ldg, by_seq;
+    float value_scale;
+    const float* q_factor;       // flash: not null: q16, keys and values are fp16, and the scores of a query have this factor, [rows][H]
 };
 
 __device__ __forceinline__ float temperature_of(const AttnParams& p, int pos) {
@@ -48,6 +53,11 @@ __device__ __forceinline__ float cache_value(const AttnParams& p, const float* p
 constexpr int kClusterSplits = 8;
 bool attention_stream_supported(const tbl_attention_mixer& m);
 int launch_attention_stream(const AttnParams& p, int n_seq, cudaStream_t st);
+
+// attention.cu: any sizes, split over the context into partial sums, which the merge brings together (p.splits of them)
+constexpr int kMergeMaxSplits = 1024;
+int launch_attention_simt(const AttnParams& p, int precision, int n_seq, cudaStream_t st);
+int launch_attention_merge(const AttnParams& p, int precision, int rows, cudaStream_t st);
 
 // attention_prefill.cu: flash attention on tcgen05
 bool attention_flash_supported(const tbl_attention_mixer& m);

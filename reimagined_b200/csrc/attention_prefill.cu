@@ -28,8 +28,9 @@ struct FlashParams {
     bf16* out;                 // [rows][H * vd]
     float *part_m, *part_l, *part_o;             // heads in chunks: [rows][H][maps] ([vp])
     int* status;
-    int ldg, H, G, group, maps, dp, vd, vp, capacity, n_tok, tiles, chunks, k_stages, v_stages, vec;
-    float scale_log2, lambda, out_scale, eps;
+    int ldg, H, G, group, maps, dp, vd, vp, capacity, n_tok, tiles, chunks, k_stages, v_stages, vec, by_seq;
+    float scale_log2, lambda, out_scale, eps, value_scale;
+    const float* q_factor;
 };
 
 // values as they lie in the cache: 64 columns (128 bytes, swizzled) per token row, groups of 8 tokens 1024 bytes apart (SBO),
@@ -68,6 +69,8 @@ __device__ __forceinline__ void store_row(const FlashParams& p, const float (&v)
     }
 }
 
+// HALF: queries, keys and values in fp16, weights as one term; a factor for every query (p.q_factor), one map.
+template <bool HALF>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_flash_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const FlashParams p) {
@@ -115,7 +118,7 @@ attention_flash_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     };
     const int nblk0 = blocks_of(0), nblk1 = blocks_of(1);
     const int nmax = max(nblk0, nblk1);
-    const int row_q = seq * p.n_tok + q0, row_k = (slot * p.G + head / p.group) * p.capacity;
+    const int row_q = seq * p.n_tok + q0, row_k = ((p.by_seq ? seq : slot) * p.G + head / p.group) * p.capacity;
 
     if (warp == kTmaWarp) {
         // ---------------- TMA ----------------
@@ -150,7 +153,7 @@ attention_flash_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (warp == kMmaWarp) {
         // ---------------- MMA ----------------
         if (elect_one()) {
-            const uint32_t is = idesc_bf16(kBlock), iv = idesc_bf16(vcols) | kTransposeB;
+            const uint32_t is = HALF ? idesc_f16(kBlock) : idesc_bf16(kBlock), iv = (HALF ? idesc_f16(vcols) : idesc_bf16(vcols)) | kTransposeB;
             bool alive = mbar_wait_bounded(q_full, 0, p.status);
             tc_fence_after();
             // ring positions and descriptors are carried along instead of worked out per product
@@ -178,7 +181,7 @@ attention_flash_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {          // 16 tokens each: columns 32 (k / 2) + 8 (k & 1), + 16 for the low term
                                 umma_f16_ta(o, pc + (k >> 1) * 32 + (k & 1) * 8, bd + 128 * k, iv, (h | k) != 0 ? 1u : (j != 0 ? 1u : 0u));
-                                umma_f16_ta(o, pc + (k >> 1) * 32 + (k & 1) * 8 + 16, bd + 128 * k, iv, 1);
+                                if (!HALF) umma_f16_ta(o, pc + (k >> 1) * 32 + (k & 1) * 8 + 16, bd + 128 * k, iv, 1);
                             }
                             // the entry is free once the last tile that uses it has read it
                             if (w == 1 || j >= nblk1) umma_commit(&v_empty[vs]);
@@ -221,12 +224,14 @@ attention_flash_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         float m = -INFINITY, l = 0.0f;
         bool alive = true;
         const int n = w == 0 ? nblk0 : nblk1;
+        float c = p.scale_log2;
+        if (HALF) c *= p.q_factor[(static_cast<size_t>(seq) * p.n_tok + min(q0 + in_cta, p.n_tok - 1)) * p.H + head];
         for (int j = 0; j < n; ++j) {
             alive = mbar_wait_bounded(&s_full[w], j & 1, p.status);
             alive = __all_sync(0xffffffffu, alive);
             if (!alive) break;
             tc_fence_after();
-            softmax_block(s_col, o_col, vcols, pos - j * kBlock, p.scale_log2, j == 0, m, l, p_full + 2 * w, lane);
+            softmax_block<HALF>(s_col, o_col, vcols, pos - j * kBlock, c, j == 0, m, l, p_full + 2 * w, lane);
         }
         const int q = q0 + in_cta;
         const bool ok = q < p.n_tok;
@@ -305,7 +310,7 @@ attention_flash_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     tmem_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(x[e]);
-                    if (ok) store_row(p, v, 1.0f / l, cols - ch * 32, gate ? gate + ch * 32 : nullptr, out + ch * 32);
+                    if (ok) store_row(p, v, p.value_scale / l, cols - ch * 32, gate ? gate + ch * 32 : nullptr, out + ch * 32);
                 }
             }
         }
@@ -355,21 +360,26 @@ int launch_attention_flash(const AttnParams& p, int n_seq, cudaStream_t st) {
     if (n_seq > 65535 || rows > 2147483647LL || cached > 2147483647LL) return TBL_ERR_SHAPE;
     const Rings rings = pick_rings(p.maps, p.dp, p.vp);
     FlashParams f{};
-    f.slots = p.slots; f.positions = p.positions; f.gate = p.g_off < 0 ? nullptr : p.proj + p.g_off; f.out = static_cast<bf16*>(p.out);
+    f.slots = p.slots; f.positions = p.positions; f.gate = p.gate; f.out = static_cast<bf16*>(p.out);
     f.part_m = p.part_m; f.part_l = p.part_l; f.part_o = p.part_o; f.status = p.status;
-    f.ldg = p.ld; f.H = p.H; f.G = p.G; f.group = p.group; f.maps = p.maps; f.dp = p.dp; f.vd = p.vd; f.vp = p.vp; f.capacity = p.capacity;
+    f.ldg = p.ldg; f.H = p.H; f.G = p.G; f.group = p.group; f.maps = p.maps; f.dp = p.dp; f.vd = p.vd; f.vp = p.vp; f.capacity = p.capacity;
     f.n_tok = p.n_tok; f.tiles = ceil_div(p.n_tok, p.maps == 2 ? kBlock : 2 * kBlock); f.chunks = ceil_div(p.vp, kChunk);
     f.k_stages = rings.k; f.v_stages = rings.v; f.vec = p.vec && p.vd % 8 == 0;
     f.scale_log2 = p.scale_log2; f.lambda = p.lambda; f.out_scale = p.out_scale; f.eps = p.eps;
+    f.value_scale = p.value_scale; f.by_seq = p.by_seq;
+    f.q_factor = p.q_factor;
     CUtensorMap mq, mk, mv;
-    const auto t = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const auto t = p.q_factor ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (!make_map(&mq, t, 2, p.q16, rows, static_cast<uint64_t>(p.H) * p.maps * p.dp, 64, kBlock) ||
         !make_map(&mk, t, 2, p.cache, cached, p.cw, 64, kBlock) || !make_map(&mv, t, 2, p.cache, cached, p.cw, 64, 64))
         return TBL_ERR_CUDA;
-    static bool done[64] = {};
-    if (allow_smem(attention_flash_kernel, rings.smem, done) != cudaSuccess) return TBL_ERR_CUDA;
-    return launch_dependent(attention_flash_kernel, dim3(f.tiles, p.H * f.chunks, n_seq), dim3(kThreads), rings.smem, st, mq, mk, mv, f) ==
-                   cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+    const dim3 grid(f.tiles, p.H * f.chunks, n_seq);
+    static bool done[2][64] = {};
+    auto launch = [&](auto kernel, bool (&seen)[64]) {
+        if (allow_smem(kernel, rings.smem, seen) != cudaSuccess) return TBL_ERR_CUDA;
+        return launch_dependent(kernel, grid, dim3(kThreads), rings.smem, st, mq, mk, mv, f) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+    };
+    return p.q_factor ? launch(attention_flash_kernel<true>, done[1]) : launch(attention_flash_kernel<false>, done[0]);
 }
 
 }  // namespace stack

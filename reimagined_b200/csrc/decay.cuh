@@ -1,0 +1,31 @@
+// Shared by the translation units of linear attention with decay (decay_attention.cu, decay_chunk.cu).
+#pragma once
+
+#include "head_rotation.cuh"
+
+namespace tbl {
+namespace stack {
+
+struct DecayParams {
+    const float* proj;           // [rows][ld]: q | k | v | gate
+    const float *q, *k;          // scan: normed and turned, [rows][H][d]
+    float* raw;                  // scan: scale S q, [rows][H][d]
+    const float *log_decay, *norm;
+    const float* states;         // [slots][H][value][key]
+    float* next;                 // the same, after the last token
+    const int32_t *slots, *positions;
+    void* out;                   // [rows][H * d]
+    int* status;
+    Rotation r;
+    const float *q_norm, *k_norm;
+    int ld, H, d, v_off, g_off, n_seq, n_tok, vec;
+    float scale, eps;
+};
+
+// decay_chunk.cu: prompts by chunks on the tensor cores
+bool decay_chunk_supported(const tbl_decay_mixer& m);
+size_t decay_chunk_workspace(const tbl_decay_mixer& m, int n_seq, int n_tok);
+int launch_decay_chunks(const tbl_decay_mixer& m, const DecayParams& p, void* ws, cudaStream_t st);
+
+}  // namespace stack
+}  // namespace tbl

@@ -6,6 +6,8 @@
 // grow by 2^8 (then O and the sum are rescaled).
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "stack.cuh"
 #include "tc05.cuh"
 
@@ -59,7 +61,9 @@ __device__ __forceinline__ void products(uint32_t d_tmem, uint64_t a, uint64_t b
 
 // One block of 128 scores of this thread's row -> weights in place; columns past `last` are not visible.  c = scale log2 e,
 // m the row's maximum (times c), l its sum.  vd: output columns to rescale.  p_full: two barriers, one for each half of the
-// weights, so that the second product starts under the second half's exponentials.
+// weights, so that the second product starts under the second half's exponentials.  HALF: the weights as one fp16 term (12 bits, where operands are
+// fp16 too) in the first 16 of every 32 columns.
+template <bool HALF = false>
 __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, int vd, int last, float c, bool first, float& m, float& l,
                                               uint64_t* p_full, int lane) {
     const bool edge = __any_sync(0xffffffffu, last < kBlock - 1);
@@ -103,7 +107,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, in
     uint64_t sums[2] = {0, 0};
 #pragma unroll
     for (int ch = 0; ch < 4; ++ch) {
-        uint32_t y[32];
+        uint32_t y[HALF ? 16 : 32];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float p0, p1;
@@ -112,14 +116,20 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, in
             p1 = ex2(p1);
             const uint64_t p = pair_of(p0, p1);
             sums[i & 1] = add2(sums[i & 1], p);
+            if constexpr (HALF) {
+                const __half2 h = __floats2half2_rn(p0, p1);
+                y[i] = *reinterpret_cast<const uint32_t*>(&h);
+                continue;
+            }
             // the high term cut off, the low term the (exact) rest rounded
             const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
             y[i] = __byte_perm(b0, b1, 0x7632);
             float r0, r1;
             unpair(add2(p, pair_of(-__uint_as_float(b0 & 0xffff0000u), -__uint_as_float(b1 & 0xffff0000u))), r0, r1);
-            y[16 + i] = pack_bf16(r0, r1);
+            if constexpr (!HALF) y[16 + i] = pack_bf16(r0, r1);
         }
-        tmem_st32(s_col + ch * 32, y);
+        if constexpr (HALF) tmem_st16(s_col + ch * 32, y);
+        else tmem_st32(s_col + ch * 32, y);
         if (ch & 1) {
             tmem_st_wait();
             tc_fence_before();

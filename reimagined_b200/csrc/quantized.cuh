@@ -1,0 +1,82 @@
+// Shared by the translation units of the attention over a 4-bit cache (quantized_attention.cu, quantized_decode.cu).
+//
+// Cache of a layer: [slot][kv head][token][row], a row being, with n = the head size rounded up to 64, n/2 bytes of key codes, n/2 of value codes, n/16
+// scale bytes of the key, n/16 of the value, and zeros to a multiple of 16.  One token of a head is one contiguous row, so that a tile of tokens is one bulk copy.
+#pragma once
+
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include "head_rotation.cuh"
+
+namespace tbl {
+namespace stack {
+
+__host__ __device__ __forceinline__ int quantized_width(int dim) { return (dim + 63) / 64 * 64; }
+__host__ __device__ __forceinline__ int quantized_row(int width) { return (width + width / 8 + 15) / 16 * 16; }
+
+struct QuantizedParams {
+    const float* proj;           // [rows][ld]: q | k | v | gate
+    const float *q_norm, *k_norm;
+    uint8_t* cache;
+    const int32_t *slots, *positions;
+    void* q;                     // queries, normed and turned: [rows][H][ldq]
+    float* q_factor;             // queries in fp16: the power of two they were divided by, [rows][H]
+    void* expanded;              // [sequence][kv head][ctx][key | value]: codes x scales, without the layer's units
+    float *part_m, *part_l, *part_o;
+    void* out;
+    int* status;
+    Rotation r;
+    int ld, g_off;               // of proj; g_off: column of the output gate, < 0: none
+    int H, G, group, d, width, row, ldq, ldo, capacity, n_tok, splits, ctx;
+    float scale_log2, key_unit, value_unit, eps;
+};
+
+__device__ __forceinline__ uint8_t* quantized_at(const QuantizedParams& p, int slot, int g, int token) {
+    return p.cache + (static_cast<size_t>(slot) * p.G + g) * p.capacity * p.row + static_cast<size_t>(token) * p.row;
+}
+// a token has room in the cache and, where heads turn, in the tables
+__device__ __forceinline__ bool quantized_room(const QuantizedParams& p, int pos) {
+    return pos >= 0 && pos < p.capacity && (p.r.half == 0 || pos < p.r.positions);
+}
+
+// two codes of a byte (the low half first) as halves
+__device__ __forceinline__ __half2 codes_of(uint32_t byte) {
+    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1);
+    return *reinterpret_cast<const __half2*>(&h);
+}
+__device__ __forceinline__ float scale_of(uint8_t byte) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(byte, __NV_E4M3);
+    return __half2float(*reinterpret_cast<const __half*>(&h));
+}
+
+// Eight numbers of a group of 16, of which the neighbouring lane (lane ^ 1) holds the others: their codes and the group's scale.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], float unit, uint8_t& scale) {
+    float most = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        most = fmaxf(most, fabsf(x[i]));
+        finite = finite && fabsf(x[i]) < INFINITY;               // false for NaN too
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    finite = (__shfl_xor_sync(0xffffffffu, static_cast<int>(finite), 1) != 0) && finite;
+    scale = finite ? __nv_cvt_float_to_fp8(__fdiv_rn(most, __fmul_rn(unit, 6.0f)), __NV_SATFINITE, __NV_E4M3) : 0x7f;
+    const float step = __fmul_rn(scale_of(scale), unit);
+    uint32_t codes = 0;
+    if (!finite || !(step > 0.0f)) return codes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        codes |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(x[2 * i], step), __fdiv_rn(x[2 * i + 1], step)), __NV_E2M1, cudaRoundNearest))
+                 << (8 * i);
+    return codes;
+}
+
+// quantized_decode.cu: streams the 4-bit rows for a few query rows
+bool quantized_stream_supported(const tbl_quantized_mixer& m);
+int quantized_stream_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
+bool quantized_stream_whole(const tbl_quantized_mixer& m, int splits);     // finishes its rows itself (otherwise it leaves partial sums)
+int launch_quantized_stream(const QuantizedParams& p, int n_seq, cudaStream_t st);
+
+}  // namespace stack
+}  // namespace tbl

@@ -1,0 +1,362 @@
+// Softmax attention over a cache that holds keys and values in 4 bits (e2m1 codes, an e4m3 scale for every 16 numbers).
+//
+//   quantized_prep_kernel    norm and rotation of queries and keys, rounding of keys and values to 4 bits, append
+//   quantized_expand_kernel  the visible cache as numbers: code x scale has six bits, which fp16 and bf16 hold
+//   quantized_read_kernel    the same for single tokens, in the layer's units
+// Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, and weights need one term instead of two), fp32 and other sizes through the SIMT kernel of attention.cu, a few
+// query rows over the 4-bit rows themselves (quantized_decode.cu).  The layer's units enter as factors of the scores and of the output.
+#include <string.h>
+
+#include "attention.cuh"
+#include "quantized.cuh"
+
+namespace tbl {
+namespace stack {
+namespace {
+
+constexpr int kPrepWarps = 8;
+
+// A warp per head of a row: query heads, then key heads, then value heads.  Keys are normed and turned in 64 bits, so that the code of a number does not depend on
+// how a sum of squares is rounded (64-bit arithmetic of 2 x 8 numbers a lane; the row's projections take longer to arrive).
+template <typename T, int V>
+__global__ void __launch_bounds__(32 * kPrepWarps) quantized_prep_kernel(const QuantizedParams p) {
+    __shared__ __align__(16) float head_s[kPrepWarps][TBL_MAX_ROTATED_DIM];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y * kPrepWarps + warp;
+    if (head >= p.H + 2 * p.G) return;
+    const int slot = p.slots[row / p.n_tok], pos = p.positions[slot] + row % p.n_tok;
+    const bool room = quantized_room(p, pos);
+    const int at = p.r.half > 0 ? min(max(pos, 0), p.r.positions - 1) : 0;
+    const float* src = p.proj + static_cast<size_t>(row) * p.ld + head * p.d;
+    HeadUnits<V, 32> x;
+    if (head < p.H) {
+        x.load(p.r, src, p.d, lane);
+        x.template turn<float>(p.r, p.q_norm, p.eps, at, p.d, lane);
+        T* dst = static_cast<T*>(p.q) + (static_cast<size_t>(row) * p.H + head) * p.ldq;
+        float f = 1.0f;
+        if (sizeof(T) == 2 && p.q_factor) {                      // fp16: the largest number of a head lies in [1, 2)
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HeadUnits<V, 32>::kUnits; ++i)
+#pragma unroll
+                for (int e = 0; e < 2 * V; ++e) most = fmaxf(most, fabsf(x.x[i][e]));
+            const uint32_t power = min(__float_as_uint(warp_max(most)) >> 23, 253u);
+            if (power) {
+                f = __uint_as_float((254u - power) << 23);
+                if (lane == 0) p.q_factor[static_cast<size_t>(row) * p.H + head] = __uint_as_float(power << 23);
+            } else if (lane == 0) {
+                p.q_factor[static_cast<size_t>(row) * p.H + head] = 1.0f;
+            }
+        }
+        x.store(p.r, dst, p.d, lane, f);
+        for (int c = p.d + lane; c < p.ldq; c += 32) dst[c] = from_f<T>(0.0f);
+        return;
+    }
+    if (!room) {
+        if (head == p.H && lane == 0) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+        return;
+    }
+    const bool is_k = head < p.H + p.G;
+    float* mine = head_s[warp];
+    for (int c = p.d + lane; c < p.width; c += 32) mine[c] = 0.0f;
+    if (is_k) {
+        x.load(p.r, src, p.d, lane);
+        x.template turn<double>(p.r, p.k_norm, p.eps, at, p.d, lane);
+        x.store(p.r, mine, p.d, lane);
+    } else {
+        for (int c = lane; c < p.d; c += 32) mine[c] = src[c];
+    }
+    __syncwarp();
+    const int g = head - p.H - (is_k ? 0 : p.G);
+    uint8_t* dst = quantized_at(p, slot, g, pos);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = 8 * lane < p.width ? mine[8 * lane + i] : 0.0f;
+    uint8_t scale;
+    const uint32_t codes = quantize8(y, is_k ? p.key_unit : p.value_unit, scale);
+    if (8 * lane < p.width) {
+        reinterpret_cast<uint32_t*>(dst + (is_k ? 0 : p.width / 2))[lane] = codes;
+        if ((lane & 1) == 0) dst[p.width + (is_k ? 0 : p.width / 16) + lane / 2] = scale;
+    }
+    const int used = p.width + p.width / 8;
+    if (!is_k && used + lane < p.row) dst[used + lane] = 0;
+}
+
+// ---- cached numbers ---------------------------------------------------------------------------------------------------------
+// eight codes times their scale
+__device__ __forceinline__ void numbers8(uint32_t codes, float scale, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 c = __half22float2(codes_of((codes >> (8 * i)) & 0xffu));
+        v[2 * i] = c.x * scale;
+        v[2 * i + 1] = c.y * scale;
+    }
+}
+__device__ __forceinline__ void put8(bf16* dst, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+__device__ __forceinline__ void put8(__half* dst, const float (&v)[8]) {
+    __align__(16) __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
+}
+__device__ __forceinline__ void put8(float* dst, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// [sequence][kv head][ctx][key, padded to 16 | value]; a thread per eight numbers, zeros behind the last visible token.
+template <typename T>
+__global__ void __launch_bounds__(256) quantized_expand_kernel(const QuantizedParams p, const int padded) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int per = padded / 4;                                  // eights of a row: key and value
+    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= static_cast<long long>(p.ctx) * per) return;
+    const int token = static_cast<int>(i / per), c = static_cast<int>(i % per), is_v = c >= per / 2, e = c - is_v * (per / 2);
+    const int seq = blockIdx.y / p.G, g = blockIdx.y % p.G, slot = p.slots[seq];
+    const int n = min(p.positions[slot] + p.n_tok, p.capacity);
+    float v[8] = {};
+    if (token < n) {
+        const uint8_t* row = quantized_at(p, slot, g, token);
+        const uint32_t codes = reinterpret_cast<const uint32_t*>(row + is_v * (p.width / 2))[e];
+        numbers8(codes, scale_of(row[p.width + is_v * (p.width / 16) + e / 2]), v);
+    }
+    put8(static_cast<T*>(p.expanded) + ((static_cast<size_t>(blockIdx.y) * p.ctx + token) * per + c) * 8, v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) quantized_read_kernel(const QuantizedParams p, T* keys, T* values) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int row = blockIdx.x, slot = p.slots[row / p.n_tok], pos = p.positions[slot] + row % p.n_tok, per = p.width / 8;
+    if (pos < 0 || pos >= p.capacity) {
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+        return;
+    }
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < p.G * 2 * per; i += gridDim.y * 256) {
+        const int g = i / (2 * per), c = i - g * 2 * per, is_v = c >= per, e = c - is_v * per;
+        T* out = is_v ? values : keys;
+        if (!out) continue;
+        const uint8_t* src = quantized_at(p, slot, g, pos);
+        float v[8];
+        numbers8(reinterpret_cast<const uint32_t*>(src + is_v * (p.width / 2))[e], scale_of(src[p.width + is_v * (p.width / 16) + e / 2]), v);
+        const float unit = is_v ? p.value_unit : p.key_unit;
+        out += (static_cast<size_t>(row) * p.G + g) * p.d + e * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (e * 8 + k < p.d) out[k] = from_f<T>(v[k] * unit);
+    }
+}
+
+// ---- plan -------------------------------------------------------------------------------------------------------------------
+enum Route { kAuto = 0, kSimt = 1, kStream = 2, kFlash = 3 };
+constexpr int kFlashMinTokens = 48;
+
+int padded16(int n) { return static_cast<int>(round_up(n, 16)); }
+
+// the mixer as attention_prefill.cu knows it
+tbl_attention_mixer as_attention(const tbl_quantized_mixer& m) {
+    tbl_attention_mixer a{};
+    a.heads = m.heads; a.kv_heads = m.kv_heads; a.dim = a.vdim = m.dim; a.maps = 1; a.scale = m.scale * m.key_scale; a.kv_from = -1;
+    return a;
+}
+
+int pick_route(const tbl_quantized_mixer& m, int precision, int n_tok) {
+    if (precision != TBL_BF16) return kSimt;
+    if (n_tok >= kFlashMinTokens && attention_flash_supported(as_attention(m))) return kFlash;
+    return quantized_stream_supported(m) ? kStream : kSimt;
+}
+
+struct Plan {
+    int route, splits, ctx;
+    size_t q, factor, expanded, pm, pl, po, bytes;
+};
+
+Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq, int n_tok, int context) {
+    Plan w{};
+    const size_t rows = static_cast<size_t>(n_seq) * n_tok, dp = padded16(m.dim);
+    w.route = route == kAuto ? pick_route(m, precision, n_tok) : route;
+    w.splits = 1;
+    bool parts = w.route == kSimt || (w.route == kFlash && !attention_flash_whole(as_attention(m)));
+    if (w.route == kStream) {
+        w.splits = quantized_stream_splits(m, n_seq, n_tok, context);
+        parts = !quantized_stream_whole(m, w.splits);
+    } else if (w.route == kSimt) {
+        const long long units = static_cast<long long>(ceil_div(static_cast<long long>(n_tok) * (m.heads / m.kv_heads), 16)) * n_seq * m.kv_heads;
+        long long s = 2LL * kNumSm / units;
+        const int tokens = ceil_div(context, 64);                // a split is worth at least 64 tokens
+        if (s > tokens) s = tokens;
+        w.splits = s < 1 ? 1 : static_cast<int>(s < kMergeMaxSplits ? s : kMergeMaxSplits);
+    }
+    w.ctx = static_cast<int>(round_up(context, 128));            // whole blocks of the flash kernel
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };
+    w.q = take(w.route == kStream ? 2 * rows * m.heads * quantized_width(m.dim) : w.route == kFlash ? 2 * rows * m.heads * dp : 4 * rows * m.heads * m.dim);
+    w.factor = take(w.route != kSimt ? sizeof(float) * rows * m.heads : 0);
+    w.expanded = take(w.route == kStream ? 0 : (precision == TBL_BF16 ? 2 : 4) * static_cast<size_t>(n_seq) * m.kv_heads * w.ctx * 2 * dp);
+    const size_t units = rows * m.heads * w.splits;
+    w.pm = take(parts ? sizeof(float) * units : 0);
+    w.pl = take(parts ? sizeof(float) * units : 0);
+    w.po = take(parts ? sizeof(float) * units * dp : 0);
+    w.bytes = off;
+    return w;
+}
+
+template <typename T, int V>
+cudaError_t launch_prep_v(const QuantizedParams& p, int rows, cudaStream_t st) {
+    return launch_dependent(quantized_prep_kernel<T, V>, dim3(rows, ceil_div(p.H + 2 * p.G, kPrepWarps)), dim3(32 * kPrepWarps), 0, st, p);
+}
+template <typename T>
+cudaError_t launch_prep(const QuantizedParams& p, int rows, bool vec, cudaStream_t st) {
+    return vec ? launch_prep_v<T, 4>(p, rows, st) : launch_prep_v<T, 1>(p, rows, st);
+}
+
+// partial sums and outputs as attention.cu's merge takes them
+AttnParams merge_params(const QuantizedParams& p, const tbl_quantized_mixer& m) {
+    AttnParams a{};
+    a.slots = p.slots; a.positions = p.positions; a.part_m = p.part_m; a.part_l = p.part_l; a.part_o = p.part_o; a.out = p.out; a.status = p.status;
+    a.H = p.H; a.G = p.G; a.group = p.group; a.maps = 1; a.d = a.vd = p.d; a.dp = a.vp = padded16(p.d); a.n_tok = p.n_tok; a.splits = p.splits;
+    a.gate = p.g_off < 0 ? nullptr : p.proj + p.g_off; a.ldg = p.ld; a.value_scale = m.value_scale;
+    return a;
+}
+
+int run(const tbl_quantized_mixer& m, int precision, const QuantizedParams& p, const Plan& w, int n_seq, cudaStream_t st) {
+    const int rows = n_seq * p.n_tok;
+    const bool vec = vector_heads(m.rotation, p.d, p.proj, p.ld);
+    const cudaError_t e = w.route == kSimt ? launch_prep<float>(p, rows, vec, st) : launch_prep<__half>(p, rows, vec, st);
+    if (e != cudaSuccess) return TBL_ERR_CUDA;
+    AttnParams a = merge_params(p, m);
+    if (w.route == kStream) {
+        const int rc = launch_quantized_stream(p, n_seq, st);
+        return rc != TBL_OK || quantized_stream_whole(m, w.splits) ? rc : launch_attention_merge(a, precision, rows, st);
+    }
+    const dim3 grid(ceil_div(static_cast<long long>(p.ctx) * (a.dp / 4), 256), n_seq * p.G);
+    const cudaError_t x = w.route == kFlash ? launch_dependent(quantized_expand_kernel<__half>, grid, dim3(256), 0, st, p, a.dp)
+                          : precision == TBL_BF16 ? launch_dependent(quantized_expand_kernel<bf16>, grid, dim3(256), 0, st, p, a.dp)
+                                                  : launch_dependent(quantized_expand_kernel<float>, grid, dim3(256), 0, st, p, a.dp);
+    if (x != cudaSuccess) return TBL_ERR_CUDA;
+    a.cache = p.expanded; a.cw = 2 * a.dp; a.n_slots = n_seq; a.capacity = p.ctx; a.by_seq = 1;
+    a.scale_log2 = p.scale_log2;
+    // the gate's columns decide whether the flash kernel's vector loads are aligned, as the projections' do where it reads them itself
+    a.vec = (p.ld | p.d) % 4 == 0 && aligned16(p.proj);
+    if (w.route == kFlash) {
+        a.q16 = static_cast<bf16*>(p.q);                         // sixteen bits either way
+        a.q_factor = p.q_factor;
+        const int rc = launch_attention_flash(a, n_seq, st);
+        return rc != TBL_OK || attention_flash_whole(as_attention(m)) ? rc : launch_attention_merge(a, precision, rows, st);
+    }
+    a.proj = static_cast<const float*>(p.q); a.ld = p.H * p.d;
+    const int rc = launch_attention_simt(a, precision, n_seq, st);
+    return rc != TBL_OK ? rc : launch_attention_merge(a, precision, rows, st);
+}
+
+QuantizedParams basic_params(const tbl_quantized_mixer& m, int capacity, const int32_t* slots, const int32_t* positions, int n_tok) {
+    QuantizedParams p{};
+    p.slots = slots; p.positions = positions; p.r = rotation_of(m.rotation);
+    p.ld = m.in.outputs; p.g_off = m.gated ? (m.heads + 2 * m.kv_heads) * m.dim : -1;
+    p.H = m.heads; p.G = m.kv_heads; p.group = m.heads / m.kv_heads; p.d = m.dim; p.width = quantized_width(m.dim); p.row = quantized_row(p.width);
+    p.capacity = capacity; p.n_tok = n_tok; p.key_unit = m.key_scale; p.value_unit = m.value_scale;
+    p.status = device_status_ptr();
+    return p;
+}
+
+}  // namespace
+
+int check_quantized(const tbl_quantized_mixer& m, int width) {
+    if (m.heads <= 0 || m.kv_heads <= 0 || m.heads > 65535 || m.heads % m.kv_heads) return TBL_ERR_SHAPE;
+    const int rc = check_rotation(m.rotation, m.dim);
+    if (rc != TBL_OK) return rc;
+    if (!(m.key_scale > 0.0f) || !(m.value_scale > 0.0f) || m.key_scale > 1e30f || m.value_scale > 1e30f || m.key_scale < 1e-30f || m.value_scale < 1e-30f) return TBL_ERR_SCALE;
+    if (m.gated != 0 && m.gated != 1) return TBL_ERR_INVALID_ARG;
+    const long long cols = (static_cast<long long>(m.heads) * (1 + m.gated) + 2LL * m.kv_heads) * m.dim;
+    if (m.in.inputs != width || m.in.outputs != cols || m.out.inputs != m.heads * m.dim || m.out.outputs != width) return TBL_ERR_SHAPE;
+    return m.in.weight && m.out.weight ? TBL_OK : TBL_ERR_INVALID_ARG;
+}
+
+size_t quantized_slot_bytes(const tbl_quantized_mixer& m, int capacity) {
+    return static_cast<size_t>(m.kv_heads) * capacity * quantized_row(quantized_width(m.dim));
+}
+
+size_t quantized_workspace(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context) {
+    return make_plan(m, precision, kAuto, n_seq, n_tok, context).bytes;
+}
+
+int launch_quantized(const tbl_quantized_mixer& m, int precision, int route, float eps, const float* proj, void* cache, int capacity, const int32_t* slots,
+                     const int32_t* positions, int n_seq, int n_tok, int context, void* out, void* ws, cudaStream_t st) {
+    const Plan w = make_plan(m, precision, route, n_seq, n_tok, context);
+    const long long rows = static_cast<long long>(n_seq) * n_tok;
+    if (rows > 2147483647LL || static_cast<long long>(n_seq) * m.kv_heads > 65535 || ceil_div(m.heads + 2 * m.kv_heads, kPrepWarps) > 65535 || w.splits > 65535) return TBL_ERR_SHAPE;
+    QuantizedParams p = basic_params(m, capacity, slots, positions, n_tok);
+    if (!p.status) return TBL_ERR_CUDA;
+    uint8_t* base = static_cast<uint8_t*>(ws);
+    p.proj = proj; p.q_norm = m.rotation.q_norm; p.k_norm = m.rotation.k_norm; p.cache = static_cast<uint8_t*>(cache); p.out = out; p.eps = eps;
+    p.q = base + w.q; p.expanded = base + w.expanded; p.q_factor = w.route != kSimt ? reinterpret_cast<float*>(base + w.factor) : nullptr; p.ldo = padded16(p.d); p.part_m = reinterpret_cast<float*>(base + w.pm); p.part_l = reinterpret_cast<float*>(base + w.pl);
+    p.part_o = reinterpret_cast<float*>(base + w.po); p.splits = w.splits; p.ctx = w.ctx;
+    p.ldq = w.route == kStream ? p.width : w.route == kFlash ? padded16(p.d) : p.d;
+    p.scale_log2 = static_cast<float>(static_cast<double>(m.scale) * m.key_scale * 1.4426950408889634);
+    return run(m, precision, p, w, n_seq, st);
+}
+
+}  // namespace stack
+}  // namespace tbl
+
+using namespace tbl;
+using namespace tbl::stack;
+
+extern "C" {
+
+int tbl_quantized_row_bytes(const tbl_quantized_mixer* mixer) {
+    return mixer && check_quantized(*mixer, mixer->in.inputs) == TBL_OK ? quantized_row(quantized_width(mixer->dim)) : 0;
+}
+
+size_t tbl_quantized_workspace_bytes(const tbl_quantized_mixer* mixer, int precision, int route, int n_seq, int n_tok, int context) {
+    if (!mixer || (precision != TBL_F32 && precision != TBL_BF16) || route < kAuto || route > kFlash || n_seq <= 0 || n_tok <= 0 || context <= 0 ||
+        check_quantized(*mixer, mixer->in.inputs) != TBL_OK)
+        return 0;
+    return make_plan(*mixer, precision, route, n_seq, n_tok, context).bytes;
+}
+
+int tbl_quantized_forward(const tbl_quantized_mixer* mixer, int precision, int route, float eps, const float* proj_dev, void* cache_dev, int slots,
+                          int capacity, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok, int context, void* out_dev,
+                          void* workspace_dev, size_t workspace_bytes, void* stream) {
+    if (!mixer || !proj_dev || !cache_dev || !slots_dev || !positions_dev || !out_dev || n_seq <= 0 || n_tok <= 0 || slots < n_seq || capacity <= 0 ||
+        context < n_tok || context > capacity || (precision != TBL_F32 && precision != TBL_BF16) || route < kAuto || route > kFlash || !(eps >= 0.0f))
+        return TBL_ERR_INVALID_ARG;
+    const int rc = check_quantized(*mixer, mixer->in.inputs);
+    if (rc != TBL_OK) return rc;
+    if ((route == kStream && (precision != TBL_BF16 || !quantized_stream_supported(*mixer))) ||
+        (route == kFlash && (precision != TBL_BF16 || !attention_flash_supported(as_attention(*mixer)))))
+        return TBL_ERR_SHAPE;
+    if (!workspace_dev || workspace_bytes < tbl_quantized_workspace_bytes(mixer, precision, route, n_seq, n_tok, context)) return TBL_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace_dev) & 255) || !aligned16(cache_dev) || !aligned16(out_dev) || (reinterpret_cast<uintptr_t>(proj_dev) & 3))
+        return TBL_ERR_ALIGNMENT;
+    return launch_quantized(*mixer, precision, route, eps, proj_dev, cache_dev, capacity, slots_dev, positions_dev, n_seq, n_tok, context, out_dev,
+                            workspace_dev, static_cast<cudaStream_t>(stream));
+}
+
+int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const void* cache_dev, int slots, int capacity, const int32_t* slots_dev,
+                       const int32_t* positions_dev, int n_seq, int n_tok, void* keys_dev, void* values_dev, void* stream) {
+    if (!mixer || !cache_dev || !slots_dev || !positions_dev || (!keys_dev && !values_dev) || n_seq <= 0 || n_tok <= 0 || slots <= 0 || capacity <= 0 ||
+        (precision != TBL_F32 && precision != TBL_BF16))
+        return TBL_ERR_INVALID_ARG;
+    const int rc = check_quantized(*mixer, mixer->in.inputs);
+    if (rc != TBL_OK) return rc;
+    const long long rows = static_cast<long long>(n_seq) * n_tok;
+    if (rows > 2147483647LL) return TBL_ERR_SHAPE;
+    if (!aligned16(cache_dev)) return TBL_ERR_ALIGNMENT;
+    QuantizedParams p = basic_params(*mixer, capacity, slots_dev, positions_dev, n_tok);
+    if (!p.status) return TBL_ERR_CUDA;
+    p.cache = static_cast<uint8_t*>(const_cast<void*>(cache_dev));
+    const int most = ceil_div(static_cast<long long>(p.G) * p.width / 4, 256);
+    const dim3 grid(static_cast<unsigned>(rows), most < 64 ? most : 64);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = precision == TBL_BF16
+                              ? launch_dependent(quantized_read_kernel<bf16>, grid, dim3(256), 0, st, p, static_cast<bf16*>(keys_dev), static_cast<bf16*>(values_dev))
+                              : launch_dependent(quantized_read_kernel<float>, grid, dim3(256), 0, st, p, static_cast<float*>(keys_dev), static_cast<float*>(values_dev));
+    return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+}
+
+}  // extern "C"

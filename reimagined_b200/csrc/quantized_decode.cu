@@ -1,0 +1,346 @@
+// Attention of a few query rows over a long 4-bit cache (decode, short portions): the rows of 4-bit numbers stream through shared memory once per block of 8 or 16
+// query rows that share a key/value head, and become matrix operands in registers.
+//
+// Code x scale (e2m1 x e4m3: six bits between 2^-10 and 2688) is exact in fp16, so the products are warp-level MMAs (16 x 8 x 16, fp16 operands, fp32
+// sums) of exact keys and values; queries are rounded to fp16 under a power of two per head, softmax weights to fp16 (2^-12 each, where the bf16 result is rounded by
+// 2^-9).  Scores are made as S^T = K Q^T and outputs as O^T = V^T P^T: cached numbers are the A operand, whose 16 x 16 numbers a step cost the fewest MMAs, and the
+// fragments of S^T turn into those of P^T by one transposed 8 x 8 move each.
+//
+// The order of the dimensions inside an MMA is free as long as both operands agree, so a lane takes 16 neighbouring dimensions of a token's key -- one scale -- for four steps, and
+// eight of a value.  For the values two tokens' codes are brought side by side while they are still 4 bits wide (two logic operations for sixteen numbers).
+// A warp works alone on every fourth tile of 32 tokens of the CTA's split: a ring of bulk copies of its own, its own maxima, sums and outputs; the warps meet in
+// shared memory at the end, splits of the context in attention.cu's merge.
+//
+// Bound: the cache's bytes.  A tile of 16 tokens of a head of 128 (2304 bytes, 100 cycles of an SM's share of the memory) costs 64 conversions and some 40 logic
+// operations on one pipe (two warps a cycle) and 64 multiplications on another.
+#include "attention.cuh"
+#include "quantized.cuh"
+#include "tc05.cuh"
+
+namespace tbl {
+namespace stack {
+namespace {
+
+constexpr int kWarps = 4, kTile = 32, kStages = 3;
+constexpr float kRescale = 8.0f;
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// the eight codes of a word as four pairs of halves, times a pair of scales
+__device__ __forceinline__ void widen(uint32_t codes, __half2 scale, uint32_t (&out)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __hmul2(codes_of((codes >> (8 * i)) & 0xffu), scale);
+        out[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// two e4m3 bytes (the low one first) as halves
+__device__ __forceinline__ __half2 scales_of(uint32_t bytes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(bytes), __NV_E4M3);
+    return *reinterpret_cast<const __half2*>(&h);
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
+__device__ __forceinline__ uint32_t lds8(uint32_t a) { uint32_t v; asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
+__device__ __forceinline__ uint2 lds64(uint32_t a) { uint2 v; asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a)); return v; }
+
+// The token (of 16) that stands in row i of an MMA: with rows of 144 bytes the 16 or 32 lanes that a shared-memory access serves together then hit every bank once,
+// for the keys (rows 0 .. 3 and 4 .. 7 of the MMA) as for the values (rows 0, 2, 4, 6 and so on).
+__device__ __forceinline__ int token_of(int i) {
+    const int r = i & 7;
+    return ((r & 1) ? 8 + (((r & 6) + 4) & 7) : r) + (i >> 3);
+}
+
+template <int DP>
+struct Layout {
+    static constexpr int kRow = (DP + DP / 8 + 15) / 16 * 16, kTileBytes = kTile * kRow, kRing = kWarps * kStages * kTileBytes, kLdo = DP + 4;
+};
+template <int DP, int NT>
+constexpr size_t stream_smem() {
+    const size_t ring = Layout<DP>::kRing, merge = sizeof(float) * kWarps * 8 * NT * Layout<DP>::kLdo;
+    return ring > merge ? ring : merge;
+}
+
+// DP: the head size rounded up to 64; NT: blocks of eight query rows.
+template <int DP, int NT>
+__global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const QuantizedParams p) {
+    using L = Layout<DP>;
+    constexpr int kBlocks = DP / 64, kRows = 8 * NT, kThreads = 32 * kWarps;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows], top_s[kRows], sum_s[kRows];
+    __shared__ __align__(8) uint64_t full[kWarps][kStages];
+    float* o_s = reinterpret_cast<float*>(smem);                 // afterwards: [warp][row][kLdo]
+    const int tid = threadIdx.x, warp = tc05::uniform_warp(), lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+    const int seq = blockIdx.x / p.G, g = blockIdx.x % p.G, first = blockIdx.y * kRows, split = blockIdx.z;
+    const int total = p.n_tok * p.group;
+    if (lane == 0)
+        for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
+    fence_mbar_init();
+    fence_proxy_async();
+    __syncthreads();
+    pdl_wait();
+    const int slot = p.slots[seq], pos0 = p.positions[slot];
+    const int n = min(pos0 + min(total - 1, first + kRows - 1) / p.group + 1, p.capacity);       // tokens the last row sees
+    const int per = ((n + p.splits - 1) / p.splits + kTile - 1) / kTile * kTile;
+    const int t0 = min(split * per, max(n, 0)), t1 = min(n, t0 + per);
+    const uint8_t* cache = quantized_at(p, slot, g, 0);
+    uint8_t* ring = smem + warp * kStages * L::kTileBytes;
+    auto load_tile = [&](int stage, int t) {                     // rows past the split's end stay whatever shared memory holds: they are masked
+        if (t < t1 && tc05::elect_one()) {
+            const uint32_t bytes = min(kTile, t1 - t) * L::kRow;
+            mbar_arrive_expect_tx(&full[warp][stage], bytes);
+            bulk_g2s(ring + stage * L::kTileBytes, cache + static_cast<size_t>(t) * L::kRow, bytes, &full[warp][stage]);
+        }
+    };
+    const int begin = t0 + warp * kTile, step = kWarps * kTile;
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) load_tile(s, begin + s * step);
+    // queries: B fragments of every step, two rows (2 t4, 2 t4 + 1) of factors
+    uint32_t q[NT][kBlocks][4][2];
+    float c[NT][2];
+    int last[NT][2];                                             // last token each row of the scores' fragments sees
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+        const int at = first + 8 * u + g8, ok = at < total, r = ok ? at : 0;
+        const __half* src = static_cast<const __half*>(p.q) + ((static_cast<size_t>(seq) * p.n_tok + r / p.group) * p.H + g * p.group + r % p.group) * DP;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const uint2 v = *reinterpret_cast<const uint2*>(src + 64 * b + 16 * t4 + 4 * s);
+                q[u][b][s][0] = ok ? v.x : 0u;
+                q[u][b][s][1] = ok ? v.y : 0u;
+            }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = min(first + 8 * u + 2 * t4 + e, total - 1);
+            c[u][e] = p.scale_log2 * p.q_factor[(static_cast<size_t>(seq) * p.n_tok + row / p.group) * p.H + g * p.group + row % p.group];
+            last[u][e] = min(pos0 + row / p.group, t1 - 1);
+        }
+    }
+    const int all_see = min(pos0 + first / p.group, t1 - 1);     // the last token that every row sees
+    float o[kBlocks * 4][NT][4];
+#pragma unroll
+    for (int i = 0; i < kBlocks * 4; ++i)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][u][e] = 0.0f;
+    float mx[NT][2], sum[NT][2];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) { mx[u][0] = mx[u][1] = -INFINITY; sum[u][0] = sum[u][1] = 0.0f; }
+    const int ka = token_of(g8), va = token_of(2 * t4), vb = token_of(2 * t4 + 1);               // MMA rows 8 .. 15: one token further on
+    bool alive = true;
+    uint32_t phase = 0;
+    int stage = 0;
+    for (int t = begin; t < t1; t += step) {
+        // (after a wait that gave up nothing more is asked for, and what is on its way gets a short time)
+        alive = __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, p.status, alive ? kWaitSpinLimit : 1024)) && alive;
+        const uint32_t tile = smem_u32(ring + stage * L::kTileBytes);
+        float s[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[h][u][e] = 0.0f;
+            const uint32_t row = tile + (16 * h + ka) * L::kRow;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const uint2 x = lds64(row + 32 * b + 8 * t4), y = lds64(row + L::kRow + 32 * b + 8 * t4);
+                const __half2 both = scales_of(lds8(row + DP + 4 * b + t4) | lds8(row + L::kRow + DP + 4 * b + t4) << 8);
+                const __half2 sx = __low2half2(both), sy = __high2half2(both);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    uint32_t a[4], k[4];
+                    widen(w ? x.y : x.x, sx, a);
+                    widen(w ? y.y : y.x, sy, k);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u)
+                            mma_f16(s[h][u], a[2 * e], k[2 * e], a[2 * e + 1], k[2 * e + 1], q[u][b][2 * w + e][0], q[u][b][2 * w + e][1]);
+                }
+            }
+        }
+        const bool whole = t + kTile - 1 <= all_see;             // nothing of the tile is masked
+        uint32_t pt[2][NT][2];
+        float f[NT][2];
+        bool grown = false;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x[4];                                      // tokens ka, ka + 1 of either half
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = s[i >> 1][u][2 * (i & 1) + e] * c[u][e];
+                    if (!whole && t + 16 * (i >> 1) + ka + (i & 1) > last[u][e]) x[i] = -INFINITY;
+                }
+                float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                // the maximum only moves when it grows by 2^8: then output and sum are rescaled
+                const float mn = top > mx[u][e] + kRescale ? top : mx[u][e], base = mn == -INFINITY ? 0.0f : mn;     // nothing seen yet: all weights zero
+                f[u][e] = mn == mx[u][e] ? 1.0f : ex2(mx[u][e] - base);
+                grown = grown || f[u][e] != 1.0f;
+                mx[u][e] = mn;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - base);
+                sum[u][e] = fmaf(sum[u][e], f[u][e], (x[0] + x[1]) + (x[2] + x[3]));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i >> 1][u][2 * (i & 1) + e] = x[i];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const __half2 w = __floats2half2_rn(s[h][u][2 * r], s[h][u][2 * r + 1]);
+                    pt[h][u][r] = transposed(*reinterpret_cast<const uint32_t*>(&w));
+                }
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+            for (int i = 0; i < kBlocks * 4; ++i)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) { o[i][u][0] *= f[u][0]; o[i][u][1] *= f[u][1]; o[i][u][2] *= f[u][0]; o[i][u][3] *= f[u][1]; }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // MMA columns 2 t4, 2 t4 + 1 are tokens va, vb, columns 2 t4 + 8, 2 t4 + 9 the ones behind them
+            const uint32_t ra = tile + (16 * h + va) * L::kRow, rb = tile + (16 * h + vb) * L::kRow;
+            const uint32_t codes = DP / 2 + 4 * g8, scale = DP + DP / 16 + (g8 >> 1);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                uint32_t a[2][8];
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const uint32_t wa = lds32(ra + d * L::kRow + codes + 32 * b), wb = lds32(rb + d * L::kRow + codes + 32 * b);
+                    uint32_t sa = lds8(ra + d * L::kRow + scale + 4 * b), sb = lds8(rb + d * L::kRow + scale + 4 * b);
+                    if (!whole) {                                // rows nobody has written may hold anything: a weight of zero needs a finite value beside it
+                        if (t + 16 * h + va + d >= t1) sa = 0;
+                        if (t + 16 * h + vb + d >= t1) sb = 0;
+                    }
+                    const __half2 sc = scales_of(sa | sb << 8);
+                    uint32_t even[4], odd[4];
+                    widen((wa & 0x0f0f0f0fu) | ((wb << 4) & 0xf0f0f0f0u), sc, even);
+                    widen(((wa >> 4) & 0x0f0f0f0fu) | (wb & 0xf0f0f0f0u), sc, odd);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { a[d][2 * i] = even[i]; a[d][2 * i + 1] = odd[i]; }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) mma_f16(o[4 * b + i][u], a[0][2 * i], a[0][2 * i + 1], a[1][2 * i], a[1][2 * i + 1], pt[h][u][0], pt[h][u][1]);
+            }
+        }
+        __syncwarp();                                            // the tile is no longer read
+        if (alive) load_tile(stage, t + kStages * step);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+    }
+    __syncthreads();                                             // tiles are done with: their room takes the outputs
+    pdl_launch_dependents();
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float l = sum[u][e];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+            if (g8 == 0) { m_s[warp][8 * u + 2 * t4 + e] = mx[u][e]; l_s[warp][8 * u + 2 * t4 + e] = l; }
+            float* dst = o_s + (warp * kRows + 8 * u + 2 * t4 + e) * L::kLdo + 8 * g8;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2)
+                    *reinterpret_cast<float4*>(dst + 64 * b + 2 * i) = make_float4(o[4 * b + i][u][e], o[4 * b + i][u][2 + e], o[4 * b + i + 1][u][e], o[4 * b + i + 1][u][2 + e]);
+        }
+    __syncthreads();
+    // the warps come together: sums of this split, over the first warp's
+    const int rows = min(kRows, total - first);
+    for (int i = tid; i < rows * (DP / 4); i += kThreads) {
+        const int r = i / (DP / 4), col = (i % (DP / 4)) * 4;
+        float top = m_s[0][r];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) top = fmaxf(top, m_s[k][r]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+            const float w = m_s[k][r] == -INFINITY ? 0.0f : ex2(m_s[k][r] - top);
+            const float4 x = *reinterpret_cast<const float4*>(o_s + (k * kRows + r) * L::kLdo + col);
+            v.x = fmaf(x.x, w, v.x); v.y = fmaf(x.y, w, v.y); v.z = fmaf(x.z, w, v.z); v.w = fmaf(x.w, w, v.w);
+            l = fmaf(l_s[k][r], w, l);
+        }
+        *reinterpret_cast<float4*>(o_s + r * L::kLdo + col) = v;
+        if (col == 0) { top_s[r] = top; sum_s[r] = l; }
+    }
+    __syncthreads();
+    if (p.splits > 1) {
+        for (int i = tid; i < rows * p.d; i += kThreads) {
+            const int r = i / p.d, col = i - r * p.d, row = first + r;
+            const size_t u = ((static_cast<size_t>(seq) * p.n_tok + row / p.group) * p.H + g * p.group + row % p.group) * p.splits + split;
+            if (col == 0) { p.part_m[u] = top_s[r]; p.part_l[u] = sum_s[r]; }
+            p.part_o[u * p.ldo + col] = o_s[r * L::kLdo + col];
+        }
+        return;
+    }
+    for (int i = tid; i < rows * p.d; i += kThreads) {
+        const int r = i / p.d, col = i - r * p.d, at = first + r, head = g * p.group + at % p.group;
+        const size_t row = static_cast<size_t>(seq) * p.n_tok + at / p.group;
+        const float gate = p.g_off < 0 ? 1.0f : sigmoid_f(p.proj[row * p.ld + p.g_off + head * p.d + col]);
+        static_cast<bf16*>(p.out)[(row * p.H + head) * p.d + col] = __float2bfloat16_rn(o_s[r * L::kLdo + col] * (p.value_unit / sum_s[r]) * gate);
+    }
+}
+
+// blocks of query rows: 16 at a time halves the trips over the cache, but a head of more than 128 has no registers for it
+int rows_of(int dim, int total) { return total > 8 && dim <= 128 ? 16 : 8; }
+
+template <int DP, int NT>
+cudaError_t launch(const QuantizedParams& p, int n_seq, cudaStream_t st) {
+    static bool done[64] = {};
+    const dim3 grid(n_seq * p.G, ceil_div(static_cast<long long>(p.n_tok) * p.group, 8 * NT), p.splits);
+    if (grid.y > 65535 || grid.z > 65535) return cudaErrorInvalidValue;
+    constexpr size_t smem = stream_smem<DP, NT>();
+    const cudaError_t e = allow_smem(quantized_stream_kernel<DP, NT>, smem, done);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(quantized_stream_kernel<DP, NT>, grid, dim3(32 * kWarps), smem, st, p);
+}
+
+}  // namespace
+
+bool quantized_stream_supported(const tbl_quantized_mixer& m) { return m.dim <= TBL_MAX_ROTATED_DIM; }
+
+int quantized_stream_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
+    const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
+    const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows_of(m.dim, static_cast<int>(total < 64 ? total : 64)));
+    const int tokens = ceil_div(context, kWarps * kTile);        // a split is worth at least a tile of each warp
+    long long s = 4LL * kNumSm / units;                          // four CTAs to an SM
+    if (s > tokens) s = tokens;
+    return s < 1 ? 1 : static_cast<int>(s < kMergeMaxSplits ? s : kMergeMaxSplits);
+}
+
+bool quantized_stream_whole(const tbl_quantized_mixer&, int splits) { return splits == 1; }
+
+int launch_quantized_stream(const QuantizedParams& p, int n_seq, cudaStream_t st) {
+    const long long total = static_cast<long long>(p.n_tok) * p.group;
+    const bool wide = rows_of(p.d, static_cast<int>(total < 64 ? total : 64)) == 16;
+    cudaError_t e;
+    switch (p.width) {
+        case 64: e = wide ? launch<64, 2>(p, n_seq, st) : launch<64, 1>(p, n_seq, st); break;
+        case 128: e = wide ? launch<128, 2>(p, n_seq, st) : launch<128, 1>(p, n_seq, st); break;
+        case 192: e = launch<192, 1>(p, n_seq, st); break;
+        default: e = launch<256, 1>(p, n_seq, st); break;
+    }
+    return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+}
+
+}  // namespace stack
+}  // namespace tbl

@@ -11,7 +11,7 @@ size_t elem(int precision) { return precision == TBL_BF16 ? 2 : 4; }
 
 struct StateLayout {
     int32_t* positions;                        // [slots]
-    uint8_t* layer[TBL_MAX_STACK_LAYERS];      // delta-rule states fp32, the latent cache, or the attention cache (maybe another layer's)
+    uint8_t* layer[TBL_MAX_STACK_LAYERS];      // recurrent states fp32, the latent, 4-bit or attention cache (that maybe another layer's)
     size_t slot_bytes[TBL_MAX_STACK_LAYERS];
     size_t bytes;
 };
@@ -31,6 +31,8 @@ StateLayout carve_state(const tbl_stack_model& m, int precision, int slots, int 
         }
         if (l.mixer == TBL_MIXER_GENERAL_DELTA) L.slot_bytes[i] = sizeof(float) * static_cast<size_t>(l.delta.heads) * l.delta.dim * l.delta.dim;
         else if (l.mixer == TBL_MIXER_LATENT_ATTENTION) L.slot_bytes[i] = elem(precision) * static_cast<size_t>(capacity) * latent_cache_width(l.latent);
+        else if (l.mixer == TBL_MIXER_QUANTIZED_ATTENTION) L.slot_bytes[i] = quantized_slot_bytes(l.quantized, capacity);
+        else if (l.mixer == TBL_MIXER_DECAY_ATTENTION) L.slot_bytes[i] = decay_slot_bytes(l.decay);
         else L.slot_bytes[i] = elem(precision) * static_cast<size_t>(capacity) * l.attention.kv_heads * attention_cache_width(l.attention);
         L.layer[i] = take(L.slot_bytes[i] * slots);
     }
@@ -64,6 +66,14 @@ Scratch carve_scratch(const tbl_stack_model& m, int precision, int n_seq, int n_
             most(proj, l.latent.in.outputs);
             most(mixed, static_cast<size_t>(l.latent.heads) * l.latent.vdim);
             most(mixer, latent_workspace(l.latent, precision, n_seq, n_tok, context));
+        } else if (l.mixer == TBL_MIXER_QUANTIZED_ATTENTION) {
+            most(proj, l.quantized.in.outputs);
+            most(mixed, static_cast<size_t>(l.quantized.heads) * l.quantized.dim);
+            most(mixer, quantized_workspace(l.quantized, precision, n_seq, n_tok, context));
+        } else if (l.mixer == TBL_MIXER_DECAY_ATTENTION) {
+            most(proj, l.decay.in.outputs);
+            most(mixed, static_cast<size_t>(l.decay.heads) * l.decay.dim);
+            most(mixer, decay_workspace(l.decay, precision, n_seq, n_tok));
         } else {
             most(proj, l.attention.in.outputs);
             most(mixed, static_cast<size_t>(l.attention.heads) * l.attention.vdim);
@@ -104,6 +114,8 @@ int check_model(const tbl_stack_model* m, int precision) {
         if (l.mixer == TBL_MIXER_GENERAL_DELTA) rc = check_delta(l.delta, m->width);
         else if (l.mixer == TBL_MIXER_LATENT_ATTENTION) rc = check_latent(l.latent, m->width);
         else if (l.mixer == TBL_MIXER_ATTENTION) rc = check_attention(l.attention, m->width);
+        else if (l.mixer == TBL_MIXER_QUANTIZED_ATTENTION) rc = check_quantized(l.quantized, m->width);
+        else if (l.mixer == TBL_MIXER_DECAY_ATTENTION) rc = check_decay(l.decay, m->width);
         else return TBL_ERR_UNSUPPORTED;
         if (rc != TBL_OK) return rc;
         if (l.mixer == TBL_MIXER_ATTENTION && l.attention.kv_from >= 0) {
@@ -151,7 +163,7 @@ int tbl_stack_state_reset(const tbl_stack_model* model, int precision, int slots
     if (slot < 0) return cudaMemsetAsync(state_dev, 0, L.bytes, st) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
     if (cudaMemsetAsync(L.positions + slot, 0, sizeof(int32_t), st) != cudaSuccess) return TBL_ERR_CUDA;
     for (int i = 0; i < model->n_layers; ++i) {
-        if (model->layers[i].mixer != TBL_MIXER_GENERAL_DELTA) continue;
+        if (model->layers[i].mixer != TBL_MIXER_GENERAL_DELTA && model->layers[i].mixer != TBL_MIXER_DECAY_ATTENTION) continue;
         if (cudaMemsetAsync(L.layer[i] + slot * L.slot_bytes[i], 0, L.slot_bytes[i], st) != cudaSuccess) return TBL_ERR_CUDA;
     }
     return TBL_OK;
@@ -200,6 +212,20 @@ int tbl_stack_step(const tbl_stack_model* model, int precision, int slots, int c
                 e = launch_latent(l.latent, precision, 0, m.norm_eps, S.proj, state.layer[i], capacity, slots_dev, state.positions, n_seq, n_tok,
                                   context, S.mixed, S.mixer, 0, st);
             return e == TBL_OK ? linear(l.latent.out, S.mixed, l.latent.heads * l.latent.vdim, out, residual) : e;
+        }
+        if (l.mixer == TBL_MIXER_QUANTIZED_ATTENTION) {
+            int e = linear(l.quantized.in, S.h, W, S.proj, nullptr);
+            if (e == TBL_OK)
+                e = launch_quantized(l.quantized, precision, 0, m.norm_eps, S.proj, state.layer[i], capacity, slots_dev, state.positions, n_seq, n_tok,
+                                     context, S.mixed, S.mixer, st);
+            return e == TBL_OK ? linear(l.quantized.out, S.mixed, l.quantized.heads * l.quantized.dim, out, residual) : e;
+        }
+        if (l.mixer == TBL_MIXER_DECAY_ATTENTION) {
+            int e = linear(l.decay.in, S.h, W, S.proj, nullptr);
+            float* states = reinterpret_cast<float*>(state.layer[i]);
+            if (e == TBL_OK)
+                e = launch_decay(l.decay, precision, 0, m.norm_eps, S.proj, states, states, slots_dev, state.positions, n_seq, n_tok, S.mixed, S.mixer, st);
+            return e == TBL_OK ? linear(l.decay.out, S.mixed, l.decay.heads * l.decay.dim, out, residual) : e;
         }
         int e = linear(l.attention.in, S.h, W, S.proj, nullptr);
         if (e == TBL_OK)

@@ -186,6 +186,20 @@ int launch_attention(const tbl_attention_mixer& m, int precision, int route, flo
 int attention_cache_width(const tbl_attention_mixer& m);      // cached numbers per token and key/value head
 int check_attention(const tbl_attention_mixer& m, int width);
 
+// ---- quantized_attention.cu ------------------------------------------------------------------------------------------
+size_t quantized_workspace(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context);
+size_t quantized_slot_bytes(const tbl_quantized_mixer& m, int capacity);
+int launch_quantized(const tbl_quantized_mixer& m, int precision, int route, float eps, const float* proj, void* cache, int capacity, const int32_t* slots,
+                     const int32_t* positions, int n_seq, int n_tok, int context, void* out, void* ws, cudaStream_t st);
+int check_quantized(const tbl_quantized_mixer& m, int width);
+
+// ---- decay_attention.cu ------------------------------------------------------------------------------------------------
+size_t decay_workspace(const tbl_decay_mixer& m, int precision, int n_seq, int n_tok);
+size_t decay_slot_bytes(const tbl_decay_mixer& m);
+int launch_decay(const tbl_decay_mixer& m, int precision, int route, float eps, const float* proj, const float* states, float* next, const int32_t* slots,
+                 const int32_t* positions, int n_seq, int n_tok, void* out, void* ws, cudaStream_t st);
+int check_decay(const tbl_decay_mixer& m, int width);
+
 int check_delta(const tbl_delta_mixer& m, int width);
 int check_latent(const tbl_latent_mixer& m, int width);
 

@@ -14,7 +14,11 @@ owns device memory and streams only.
 Guselix is this family with the mixers `general_delta` (delta rule with per-channel decay and removal rate) and
 `latent_attention`, RMS norms and a learned average over the depth after every layer.  Goguvik has the mixer `attention`
 (differential, grouped key/value heads, query temperature, layers that read an earlier layer's cache), Dynamic Tanh norms
-and several residual streams ("streams") joined by hyper-connections.
+and several residual streams ("streams") joined by hyper-connections.  Either design's layers may also be `quantized_attention` (grouped attention
+over a 4-bit cache) and `decay_attention` (linear attention with a decay for each head), both with normed and rotated queries and keys:
+
+    {"heads", "kv_heads", "dim", "scale", "key_scale", "value_scale", "qk_norm": true, "rot": {"base", "dims", "interleaved": false} or null, "gated": true}
+    {"heads", "dim", "scale", "qk_norm": true, "rot": ..., "gated": true}
 """
 from __future__ import annotations
 
@@ -109,10 +113,63 @@ def _fill_attention(e: "StackEngine", layer: capi.StackLayer, p: str, m: dict) -
         a.temperature, a.temperature_positions = e.query_temperature(float(m["q_temp"]["coef"]), m["q_temp"]["every"]), e.capacity
 
 
+def _head_norms(m: dict) -> Shapes:
+    return {"q.norm": (m["dim"],), "k.norm": (m["dim"],)} if m.get("qk_norm", True) else {}
+
+
+def _head_rotation(e: "StackEngine", p: str, m: dict) -> capi.HeadRotation:
+    """Norm weights of query and key heads, and the rotation {"base", "dims", "interleaved"} (null: none)."""
+    r, rot = capi.HeadRotation(), m.get("rot")
+    if m.get("qk_norm", True):
+        r.q_norm, r.k_norm = e.f32(e.weights[p + "q.norm"]), e.f32(e.weights[p + "k.norm"])
+    if rot is not None:
+        r.rot_dim, r.rope_positions, r.interleaved = rot["dims"], e.capacity, int(bool(rot.get("interleaved", False)))
+        r.rope_cos, r.rope_sin = e.rotation(float(rot["base"]), rot["dims"])
+    return r
+
+
+def _gate(m: dict) -> Tuple[str, ...]:
+    return ("g",) if m.get("gated", True) else ()
+
+
+def _quantized_shapes(m: dict, width: int, rank: int) -> Shapes:
+    h, g, d = (m[n] for n in ("heads", "kv_heads", "dim"))
+    rows = {"q": h * d, "k": g * d, "v": g * d, **{n: h * d for n in _gate(m)}}
+    return {**{name: (n, width) for name, n in rows.items()}, **_head_norms(m), "o": (width, h * d)}
+
+
+def _fill_quantized(e: "StackEngine", layer: capi.StackLayer, p: str, m: dict) -> None:
+    a = layer.quantized
+    layer.mixer = capi.MIXER_QUANTIZED_ATTENTION
+    a.heads, a.kv_heads, a.dim, a.gated = m["heads"], m["kv_heads"], m["dim"], len(_gate(m))
+    a.scale, a.key_scale, a.value_scale = float(m["scale"]), float(m["key_scale"]), float(m["value_scale"])
+    a.in_ = e.dense([p + n for n in ("q", "k", "v") + _gate(m)])
+    a.out = e.dense([p + "o"])
+    a.rotation = _head_rotation(e, p, m)
+
+
+def _decay_shapes(m: dict, width: int, rank: int) -> Shapes:
+    hd = m["heads"] * m["dim"]
+    return {**{n: (hd, width) for n in ("q", "k", "v") + _gate(m)}, **_head_norms(m), "decay": (m["heads"],), "norm": (hd,), "o": (width, hd)}
+
+
+def _fill_decay(e: "StackEngine", layer: capi.StackLayer, p: str, m: dict) -> None:
+    a = layer.decay
+    layer.mixer = capi.MIXER_DECAY_ATTENTION
+    a.heads, a.dim, a.gated, a.scale = m["heads"], m["dim"], len(_gate(m)), float(m["scale"])
+    a.in_ = e.dense([p + n for n in ("q", "k", "v") + _gate(m)])
+    a.out = e.dense([p + "o"])
+    a.rotation = _head_rotation(e, p, m)
+    a.log_decay = e.f32(-torch.exp(e.weights[p + "decay"].double()))        # S <- exp(-exp(decay)) S
+    a.norm = e.f32(e.weights[p + "norm"])
+
+
 MIXERS: Dict[str, Mixer] = {
     "general_delta": Mixer(_delta_shapes, _fill_delta),
     "latent_attention": Mixer(_latent_shapes, _fill_latent),
     "attention": Mixer(_attention_shapes, _fill_attention),
+    "quantized_attention": Mixer(_quantized_shapes, _fill_quantized),
+    "decay_attention": Mixer(_decay_shapes, _fill_decay),
 }
 
 
@@ -207,6 +264,8 @@ def synthetic_weights(cfg: dict, seed: int = 1, rank: int = 16, device: str = "c
             w[-1] += 1.0
         elif ".hc" in name:
             w = 0.2 * w + (torch.eye(shape[0], device=device) if name.endswith(".mix") else 1.0 / shape[0] if name.endswith(".in") else 1.0)
+        elif name.endswith(".mix.decay"):
+            w = w - 3.0
         elif name.endswith(".alpha"):
             w = 0.5 + 0.1 * w.clamp(-3.0, 3.0)
         elif name.endswith(".b"):
