@@ -258,7 +258,7 @@ DECAY = {
     "wide": cfgd(2, 256, 64, 0.1),
     "dim200": cfgd(1, 200, 0, 0.1, gated=False),
 }
-C_SIZES = []
+C_SIZES = [s for s in DECAY if s not in ("wide", "dim200")]
 
 
 @pytest.mark.parametrize("precision,route,size", [(0, SCAN, s) for s in DECAY] + [(1, SCAN, "plain"), (1, SCAN, "odd"), (1, SCAN, "wide")] +
@@ -268,6 +268,10 @@ def test_decay_attention(cuda, stack_lib, precision, route, size):
     a = Decay(cuda, stack_lib, DECAY[size], precision)
     rng = np.random.default_rng(5)
     tol = 2.0 ** -7 if precision else 2e-5
+    if size == "one" and route == CHUNK:
+        # A head of one number may come out near zero, where its norm has the slope 1 / sqrt(eps): that times the rounding of the terms (three operands of
+        # about one, 2^-12 each at most) of as many tokens as the decay keeps, which add up at random: four standard deviations.
+        tol += 4 * 2.0 ** -12 * np.sqrt(3 / (1 - np.exp(2.0 * a.rates.max()))) / np.sqrt(a.eps)
     for slots, n in [([1], 130), ([1], 2), ([2], 61), ([1, 2], 3), ([1, 2], 1), ([2, 1], 1), ([1, 2], 270), ([2], 1), ([1, 2], 128), ([2], 129)]:
         proj = rng.standard_normal((len(slots) * n, a.cols)).astype(np.float32)
         rows_close(a.forward(route, slots, proj), a.oracle(slots, proj), tol, f"slots {slots} n {n}")
@@ -276,7 +280,7 @@ def test_decay_attention(cuda, stack_lib, precision, route, size):
     assert stack_lib.tbl_device_status(stream(cuda)) == 0
 
 
-@pytest.mark.parametrize("precision,route", [(0, SCAN), (1, SCAN)])
+@pytest.mark.parametrize("precision,route", [(0, SCAN), (1, SCAN), (1, CHUNK)])
 def test_decay_forgets_and_remembers(cuda, stack_lib, precision, route):
     """No memory at all, a token's, no decay, a decay that fp32 can hardly tell from none; no head norm; states into another array."""
     rates = [-np.inf, -200.0, -1.0, -1e-3, -1e-6, 0.0]
