@@ -1,167 +1,397 @@
 // Linear attention with a constant decay for each head: S <- exp(log_decay) S + v k^T, o = scale S q.
 //
-//   (head_rotation.cu)       queries and keys, normed and turned
-//   decay_scan_kernel        the recurrence token by token, fp32: any size, single tokens and short portions
+//   decay_step_kernel        up to eight tokens, everything in one launch (heads of a multiple of four)
+//   decay_scan_kernel        the recurrence token by token, any size, between (head_rotation.cu), which norms and turns queries and keys, and
 //   decay_finish_kernel      head norm and output gate
 // Prompts in bf16 go by chunks (decay_chunk.cu).
 //
 // The decay enters as S + (exp(log_decay) - 1) S: 1 - exp(log_decay) has 24 bits however slow the decay is, whereas a decay rounded to fp32 would be off by 2^-25
 // every token, all in one direction.
 #include "decay.cuh"
+#include "flash.cuh"
 
 namespace tbl {
 namespace stack {
 namespace {
 
-constexpr int kScanThreads = 256, kScanTile = 8;
+using flash::fma2;
+using flash::pair_of;
+using flash::unpair;
+
+constexpr int kThreads = 256, kTile = 8;
+
+// LK lanes share a value row's keys: lane a holds 4 a + 4 LK j + e for j < C, in pairs of fp32.  A lane holds R rows, a warp 32 / LK times as many.  Lanes along
+// the keys, so that what all rows multiply with comes out of shared memory in whole lines (eight lanes a row: 328 lines a token for 32 rows of 90, and
+// they were the bound).
+template <int LK, int C, int R>
+struct State {
+    static constexpr int kKeys = 4 * LK * C, kRows = 32 / LK * R;
+    uint64_t s[R][2 * C];
+
+    static __device__ __forceinline__ bool wide(const DecayParams& p) {
+        return p.d % 4 == 0 && (reinterpret_cast<uintptr_t>(p.states) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.next) & 15) == 0;
+    }
+    // rows from `row` on of a head's state in global memory
+    __device__ __forceinline__ void load(const DecayParams& p, const float* head, int row, int share) {
+        const bool w = wide(p);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float* src = head + static_cast<size_t>(row + r) * p.d;
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const int c = 4 * share + 4 * LK * j;
+                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (row + r < p.d) {
+                    if (w) {
+                        if (c < p.d) f = *reinterpret_cast<const float4*>(src + c);
+                    } else {
+                        if (c < p.d) f.x = src[c];
+                        if (c + 1 < p.d) f.y = src[c + 1];
+                        if (c + 2 < p.d) f.z = src[c + 2];
+                        if (c + 3 < p.d) f.w = src[c + 3];
+                    }
+                }
+                s[r][2 * j] = pair_of(f.x, f.y);
+                s[r][2 * j + 1] = pair_of(f.z, f.w);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(const DecayParams& p, float* head, int row, int share) const {
+        const bool w = wide(p);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (row + r >= p.d) continue;
+            float* dst = head + static_cast<size_t>(row + r) * p.d;
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const int c = 4 * share + 4 * LK * j;
+                float4 f;
+                unpair(s[r][2 * j], f.x, f.y);
+                unpair(s[r][2 * j + 1], f.z, f.w);
+                if (w) {
+                    if (c < p.d) *reinterpret_cast<float4*>(dst + c) = f;
+                } else {
+                    if (c < p.d) dst[c] = f.x;
+                    if (c + 1 < p.d) dst[c + 1] = f.y;
+                    if (c + 2 < p.d) dst[c + 2] = f.z;
+                    if (c + 3 < p.d) dst[c + 3] = f.w;
+                }
+            }
+        }
+    }
+    // one token: the state, and this lane's share of its rows' outputs; v: the rows' values (R floats, R a multiple of 4 on 16 bytes)
+    __device__ __forceinline__ void step(uint64_t less, const float* q, const float* k, const float* v, int share, float (&a)[R]) {
+        ulonglong2 qq[C], kk[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            qq[j] = *reinterpret_cast<const ulonglong2*>(q + 4 * share + 4 * LK * j);
+            kk[j] = *reinterpret_cast<const ulonglong2*>(k + 4 * share + 4 * LK * j);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(v + r);
+            const float vr[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint64_t vv = pair_of(vr[e], vr[e]);
+                uint64_t acc = 0;
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    uint64_t &x = s[r + e][2 * j], &y = s[r + e][2 * j + 1];
+                    x = fma2(kk[j].x, vv, fma2(less, x, x));
+                    y = fma2(kk[j].y, vv, fma2(less, y, y));
+                    acc = fma2(qq[j].x, x, acc);
+                    acc = fma2(qq[j].y, y, acc);
+                }
+                float lo, hi;
+                unpair(acc, lo, hi);
+                a[r + e] = lo + hi;
+            }
+        }
+    }
+    // sums over the lanes of R rows at once: halves of the rows change sides until a lane has one row, rows_at(share)
+    static __device__ __forceinline__ float sums(float (&a)[R], int share) {
+        int n = R;
+#pragma unroll
+        for (int o = LK / 2; o; o >>= 1) {
+            if (n > 1) {
+                n >>= 1;
+                const bool upper = (share & o) != 0;
+#pragma unroll
+                for (int i = 0; i < R / 2; ++i)
+                    if (i < n) {
+                        const float keep = upper ? a[i + n] : a[i], give = upper ? a[i] : a[i + n];
+                        a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+            } else {
+                a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+            }
+        }
+        return a[0];
+    }
+    static_assert(R <= LK, "a lane keeps one row");
+    static __device__ __forceinline__ int row_at(int share) { return share / (LK / R); }
+    static __device__ __forceinline__ bool writes(int share) { return share % (LK / R) == 0; }
+};
+
+// norm and gate of a head's output, a warp; x: number lane + 32 i
+template <typename T>
+__device__ __forceinline__ void finish_head(const DecayParams& p, const float* src, const float* gate, size_t row, int head, int lane) {
+    constexpr int kPer = TBL_MAX_ROTATED_DIM / 32;
+    float x[kPer], g[kPer], ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const bool in = lane + 32 * i < p.d;
+        x[i] = in ? src[lane + 32 * i] : 0.0f;
+        g[i] = in && gate ? gate[lane + 32 * i] : 0.0f;
+        ss = fmaf(x[i], x[i], ss);
+    }
+    const float f = p.norm ? 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(p.d) + p.eps) : 1.0f;
+    T* out = static_cast<T*>(p.out) + (row * p.H + head) * p.d;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c = lane + 32 * i;
+        if (c < p.d) out[c] = from_f<T>(x[i] * f * (p.norm ? __ldg(p.norm + head * p.d + c) : 1.0f) * (gate ? sigmoid_f(g[i]) : 1.0f));
+    }
+}
+
+// Up to eight tokens of a head in one launch.  A CTA has the whole head: its state comes into shared memory by one bulk copy and goes back by another, so that registers
+// hold a few rows at a time and three CTAs of heads of 128 share an SM; while it comes, a warp each norms and turns the tokens' queries and keys.  Bound by the
+// state's bytes: the projections are asked for first, or they would queue behind the states of the whole batch.
+constexpr size_t kStepRoom = 200 * 1024;
+size_t step_smem(int keys, int d, int n_tok) { return sizeof(float) * (static_cast<size_t>(d) * d + static_cast<size_t>(n_tok) * (2 * keys + 3 * d)); }
+
+template <typename T, int V, int LK, int C>
+__global__ void __launch_bounds__(kThreads) decay_step_kernel(const DecayParams p) {
+    using S = State<LK, C, 4>;
+    extern __shared__ __align__(128) float room[];
+    __shared__ __align__(8) uint64_t full;
+    float *state_s = room, *q_s = state_s + p.d * p.d, *k_s = q_s + p.n_tok * S::kKeys, *v_s = k_s + p.n_tok * S::kKeys, *g_s = v_s + p.n_tok * p.d,
+          *o_s = g_s + p.n_tok * p.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = lane % LK;
+    const int head = blockIdx.x % p.H, seq = blockIdx.x / p.H;
+    const uint32_t bytes = p.d * p.d * 4;
+    pdl_launch_dependents();
+    if (tid == 0) {
+        mbar_init(&full, 1);
+        fence_mbar_init();
+    }
+    if (p.d != S::kKeys)
+        for (int i = tid; i < 2 * p.n_tok * S::kKeys; i += kThreads) q_s[i] = 0.0f;
+    pdl_wait();
+    const int slot = p.slots[seq];
+    const size_t row0 = static_cast<size_t>(seq) * p.n_tok;
+    const float* proj = p.proj + row0 * p.ld + head * p.d;
+    HeadUnits<V, 32> x;                                          // of this warp's first vector
+    if (warp < 2 * p.n_tok) x.load(p.r, proj + static_cast<size_t>(warp >> 1) * p.ld + (warp & 1) * p.H * p.d, p.d, lane);
+    for (int i = tid; i < 2 * p.n_tok * p.d; i += kThreads) {
+        const int is_g = i >= p.n_tok * p.d, e = i - is_g * p.n_tok * p.d;
+        if (!is_g || p.g_off >= 0) v_s[i] = proj[static_cast<size_t>(e / p.d) * p.ld + (is_g ? p.g_off : p.v_off) + e % p.d];
+    }
+    const size_t at = (static_cast<size_t>(slot) * p.H + head) * p.d * p.d;
+    const int pos = p.positions[slot];
+    if (tid == 0) {
+        mbar_arrive_expect_tx(&full, bytes);
+        bulk_g2s(state_s, p.states + at, bytes, &full);
+        if (p.r.half > 0 && head == 0 && (pos < 0 || pos + p.n_tok > p.r.positions)) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+    }
+    __syncthreads();
+    for (int i = warp; i < 2 * p.n_tok; i += kThreads / 32) {
+        const int t = i >> 1, is_k = i & 1;
+        if (i != warp) x.load(p.r, proj + static_cast<size_t>(t) * p.ld + is_k * p.H * p.d, p.d, lane);
+        x.template turn<float>(p.r, is_k ? p.k_norm : p.q_norm, p.eps, p.r.half > 0 ? min(max(pos + t, 0), p.r.positions - 1) : 0, p.d, lane);
+        x.store(p.r, (is_k ? k_s : q_s) + t * S::kKeys, p.d, lane);
+    }
+    const float l = expm1f(p.log_decay[head]);
+    const uint64_t less = pair_of(l, l);
+    const bool alive = mbar_wait_bounded(&full, 0, p.status);
+    __syncthreads();
+    // four rows a lane at a time (d is a multiple of four: all there or none)
+    for (int r0 = warp * S::kRows; r0 < p.d; r0 += kThreads / 32 * S::kRows) {
+        const int r = r0 + lane / LK * 4;
+        const bool in = r < p.d;
+        S s;
+        float* mine = state_s + (in ? r : 0) * p.d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const int c = 4 * share + 4 * LK * j;
+                const ulonglong2 f = c < p.d ? *reinterpret_cast<const ulonglong2*>(mine + i * p.d + c) : make_ulonglong2(0, 0);
+                s.s[i][2 * j] = f.x;
+                s.s[i][2 * j + 1] = f.y;
+            }
+        for (int n = 0; n < p.n_tok; ++n) {
+            float a[4];
+            s.step(less, q_s + n * S::kKeys, k_s + n * S::kKeys, v_s + n * p.d + (in ? r : 0), share, a);
+            const float o = S::sums(a, share);
+            if (in && S::writes(share)) o_s[n * p.d + r + S::row_at(share)] = o * p.scale;
+        }
+        __syncwarp();                                            // (lanes without rows have read others')
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const int c = 4 * share + 4 * LK * j;
+                if (in && c < p.d) *reinterpret_cast<ulonglong2*>(mine + i * p.d + c) = make_ulonglong2(s.s[i][2 * j], s.s[i][2 * j + 1]);
+            }
+    }
+    fence_proxy_async();
+    __syncthreads();
+    if (tid == 0 && alive) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.next + at), "r"(smem_u32(state_s)), "r"(bytes) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    for (int t = warp; t < p.n_tok; t += kThreads / 32) finish_head<T>(p, o_s + t * p.d, p.g_off < 0 ? nullptr : g_s + t * p.d, row0 + t, head, lane);
+    if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");       // shared memory has been read
+}
 
 __device__ __forceinline__ void copy4(float* dst, const float* src, bool ok) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
 
-// Eight lanes share a value row's keys, KP keys each (lane a holds 4 a + 32 j + e); a lane holds R rows, a CTA 32 R.  The tokens' vectors come by tiles of
-// kScanTile ahead of their use.
-template <int KP, int R>
+// Any number of tokens: a CTA of four warps has 4 State::kRows rows of a head.  The tokens' vectors come by tiles of kTile ahead of their use, a thread the same columns of every
+// token; two tokens' instructions mix.
+constexpr int kScanThreads = 128;
+template <int LK, int C, int R>
 __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayParams p) {
-    constexpr int kKeys = 8 * KP, kRows = 32 * R;
-    __shared__ __align__(16) float q_s[2][kScanTile][kKeys], k_s[2][kScanTile][kKeys];
-    __shared__ float v_s[2][kScanTile][kRows];
-    pdl_launch_dependents();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = lane & 7;
+    using S = State<LK, C, R>;
+    constexpr int kRows = kScanThreads / 32 * S::kRows, kCols = 2 * S::kKeys + kRows, kPer = (kCols + kScanThreads - 1) / kScanThreads;
+    __shared__ __align__(16) float vec_s[2][kTile][kCols];       // queries, keys, values
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = lane % LK, first = warp * S::kRows + lane / LK * R;
     const int head = blockIdx.x % p.H, seq = blockIdx.x / p.H, row0 = blockIdx.y * kRows;
     pdl_wait();
-    const int slot = p.slots[seq], first = warp * 4 * R + (lane >> 3) * R;       // first of this lane's rows within the CTA's
-    const size_t state = (static_cast<size_t>(slot) * p.H + head) * p.d * p.d;
+    const int slot = p.slots[seq];
+    const size_t state = (static_cast<size_t>(slot) * p.H + head) * p.d * p.d, token0 = static_cast<size_t>(seq) * p.n_tok;
+    const float* src[kPer];
+    size_t stride[kPer];
+    bool in[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c = tid + i * kScanThreads, e = c < S::kKeys ? c : c < 2 * S::kKeys ? c - S::kKeys : row0 + c - 2 * S::kKeys;
+        in[i] = c < kCols && e < p.d;
+        const size_t at = (token0 * p.H + head) * p.d + (in[i] ? e : 0);
+        src[i] = c < S::kKeys ? p.q + at : c < 2 * S::kKeys ? p.k + at : p.proj + token0 * p.ld + p.v_off + head * p.d + (in[i] ? e : 0);
+        stride[i] = c < 2 * S::kKeys ? static_cast<size_t>(p.H) * p.d : p.ld;
+    }
     auto fetch = [&](int t0, int buf) {
-        const int n = min(kScanTile, p.n_tok - t0);
-        for (int i = tid; i < n * (2 * kKeys + kRows); i += kScanThreads) {
-            const int t = i / (2 * kKeys + kRows), c = i - t * (2 * kKeys + kRows);
-            const size_t row = static_cast<size_t>(seq) * p.n_tok + t0 + t, at = (row * p.H + head) * p.d;
-            if (c < kKeys) copy4(&q_s[buf][t][c], p.q + at + (c < p.d ? c : 0), c < p.d);
-            else if (c < 2 * kKeys) copy4(&k_s[buf][t][c - kKeys], p.k + at + (c - kKeys < p.d ? c - kKeys : 0), c - kKeys < p.d);
-            else {
-                const int r = row0 + c - 2 * kKeys;
-                copy4(&v_s[buf][t][c - 2 * kKeys], p.proj + row * p.ld + p.v_off + head * p.d + (r < p.d ? r : 0), r < p.d);
+        const int n = min(kTile, p.n_tok - t0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int c = tid + i * kScanThreads;
+            if (c >= kCols) break;
+#pragma unroll
+            for (int t = 0; t < kTile; ++t) {
+                if (t >= n) break;
+                copy4(&vec_s[buf][t][c], src[i], in[i]);
+                src[i] += stride[i];
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     fetch(0, 0);
-    float s[R][KP];
-    const bool wide = p.d % 4 == 0 && (reinterpret_cast<uintptr_t>(p.states) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.next) & 15) == 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int row = row0 + first + r;
-        const float* src = p.states + state + static_cast<size_t>(row) * p.d;
-#pragma unroll
-        for (int j = 0; j < KP / 4; ++j) {
-            const int c = 4 * share + 32 * j;
-            if (wide) {
-                const float4 f = row < p.d && c < p.d ? *reinterpret_cast<const float4*>(src + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                s[r][4 * j] = f.x; s[r][4 * j + 1] = f.y; s[r][4 * j + 2] = f.z; s[r][4 * j + 3] = f.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[r][4 * j + e] = row < p.d && c + e < p.d ? src[c + e] : 0.0f;
-            }
-        }
-    }
-    const float less = expm1f(p.log_decay[head]);
-    for (int t0 = 0, buf = 0; t0 < p.n_tok; t0 += kScanTile, buf ^= 1) {
+    S s;
+    s.load(p, p.states + state, row0 + first, share);
+    const float l = expm1f(p.log_decay[head]);
+    const uint64_t less = pair_of(l, l);
+    const int row = row0 + first + S::row_at(share);
+    const bool writes = S::writes(share) && row < p.d;
+    float* raw = p.raw + (token0 * p.H + head) * p.d + row;
+    for (int t0 = 0, buf = 0; t0 < p.n_tok; t0 += kTile, buf ^= 1) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();                                         // this tile is there, the one before it is no longer read
-        if (t0 + kScanTile < p.n_tok) fetch(t0 + kScanTile, buf ^ 1);
-        const int n = min(kScanTile, p.n_tok - t0);
-        for (int t = 0; t < n; ++t) {
-            float v[R], a[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) { v[r] = v_s[buf][t][first + r]; a[r] = 0.0f; }
-#pragma unroll
-            for (int j = 0; j < KP / 4; ++j) {
-                const float4 q = *reinterpret_cast<const float4*>(&q_s[buf][t][4 * share + 32 * j]);
-                const float4 k = *reinterpret_cast<const float4*>(&k_s[buf][t][4 * share + 32 * j]);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float* x = &s[r][4 * j];
-                    x[0] = fmaf(k.x, v[r], fmaf(less, x[0], x[0])); a[r] = fmaf(q.x, x[0], a[r]);
-                    x[1] = fmaf(k.y, v[r], fmaf(less, x[1], x[1])); a[r] = fmaf(q.y, x[1], a[r]);
-                    x[2] = fmaf(k.z, v[r], fmaf(less, x[2], x[2])); a[r] = fmaf(q.z, x[2], a[r]);
-                    x[3] = fmaf(k.w, v[r], fmaf(less, x[3], x[3])); a[r] = fmaf(q.w, x[3], a[r]);
-                }
+        if (t0 + kTile < p.n_tok) fetch(t0 + kTile, buf ^ 1);
+        const int n = min(kTile, p.n_tok - t0);
+        auto token = [&](int t, float (&a)[R]) {
+            const float* v = vec_s[buf][t];
+            s.step(less, v, v + S::kKeys, v + 2 * S::kKeys + first, share, a);
+        };
+        int t = 0;
+        for (; t + 2 <= n; t += 2) {
+            float a[R], b[R];
+            token(t, a);
+            token(t + 1, b);
+            const float x = S::sums(a, share), y = S::sums(b, share);
+            if (writes) {
+                raw[0] = x * p.scale;
+                raw[static_cast<size_t>(p.H) * p.d] = y * p.scale;
             }
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-#pragma unroll
-                for (int o = 4; o; o >>= 1) a[r] += __shfl_xor_sync(0xffffffffu, a[r], o);
-                const int row = row0 + first + r;
-                if (share == 0 && row < p.d) p.raw[((static_cast<size_t>(seq) * p.n_tok + t0 + t) * p.H + head) * p.d + row] = a[r] * p.scale;
-            }
+            raw += 2 * static_cast<size_t>(p.H) * p.d;
+        }
+        if (t < n) {
+            float a[R];
+            token(t, a);
+            const float x = S::sums(a, share);
+            if (writes) raw[0] = x * p.scale;
+            raw += static_cast<size_t>(p.H) * p.d;
         }
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int row = row0 + first + r;
-        if (row >= p.d) continue;
-        float* dst = p.next + state + static_cast<size_t>(row) * p.d;
-#pragma unroll
-        for (int j = 0; j < KP / 4; ++j) {
-            const int c = 4 * share + 32 * j;
-            if (wide) {
-                if (c < p.d) *reinterpret_cast<float4*>(dst + c) = make_float4(s[r][4 * j], s[r][4 * j + 1], s[r][4 * j + 2], s[r][4 * j + 3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < p.d) dst[c + e] = s[r][4 * j + e];
-            }
-        }
-    }
+    pdl_launch_dependents();
+    s.store(p, p.next + state, row0 + first, share);
 }
 
 // A warp per head of a row.
 template <typename T>
 __global__ void __launch_bounds__(256) decay_finish_kernel(const DecayParams p) {
-    constexpr int kPer = TBL_MAX_ROTATED_DIM / 32;
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int row = blockIdx.x, head = blockIdx.y * 8 + (threadIdx.x >> 5);
     if (head >= p.H) return;
-    const float* src = p.raw + (static_cast<size_t>(row) * p.H + head) * p.d;
     const float* gate = p.g_off < 0 ? nullptr : p.proj + static_cast<size_t>(row) * p.ld + p.g_off + head * p.d;
-    float x[kPer], ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) { x[i] = lane + 32 * i < p.d ? src[lane + 32 * i] : 0.0f; ss = fmaf(x[i], x[i], ss); }
-    const float f = p.norm ? 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(p.d) + p.eps) : 1.0f;
-    T* out = static_cast<T*>(p.out) + (static_cast<size_t>(row) * p.H + head) * p.d;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int c = lane + 32 * i;
-        if (c < p.d) out[c] = from_f<T>(x[i] * f * (p.norm ? __ldg(p.norm + head * p.d + c) : 1.0f) * (gate ? sigmoid_f(gate[c]) : 1.0f));
-    }
+    finish_head<T>(p, p.raw + (static_cast<size_t>(row) * p.H + head) * p.d, gate, row, head, threadIdx.x & 31);
 }
 
-template <int KP, int R>
-cudaError_t launch_scan_r(const DecayParams& p, cudaStream_t st) {
-    return launch_dependent(decay_scan_kernel<KP, R>, dim3(p.n_seq * p.H, ceil_div(p.d, 32 * R)), dim3(kScanThreads), 0, st, p);
+int keys_of(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+bool step_supported(const tbl_decay_mixer& m, int n_tok) { return n_tok <= kTile && m.dim % 4 == 0 && step_smem(keys_of(m.dim), m.dim, n_tok) <= kStepRoom; }
+template <typename T, int V, int LK, int C>
+cudaError_t launch_step_lk(const DecayParams& p, cudaStream_t st) {
+    static bool done[64] = {};
+    const size_t smem = step_smem(4 * LK * C, p.d, p.n_tok);
+    const cudaError_t e = allow_smem(decay_step_kernel<T, V, LK, C>, smem, done);
+    return e != cudaSuccess ? e : launch_dependent(decay_step_kernel<T, V, LK, C>, dim3(p.n_seq * p.H), dim3(kThreads), smem, st, p);
 }
-template <int KP, int MOST>
-cudaError_t launch_scan_kp(const DecayParams& p, cudaStream_t st) {
-    // as many rows to a lane as still leave two CTAs to an SM
-    const long long units = static_cast<long long>(p.n_seq) * p.H;
-    if (MOST >= 4 && units * ceil_div(p.d, 128) >= 2 * kNumSm) return launch_scan_r<KP, MOST>(p, st);
-    if (MOST >= 2 && units * ceil_div(p.d, 64) >= 2 * kNumSm) return launch_scan_r<KP, MOST < 2 ? MOST : 2>(p, st);
-    return launch_scan_r<KP, 1>(p, st);
+template <typename T, int V>
+cudaError_t launch_step_v(const DecayParams& p, cudaStream_t st) {
+    switch (keys_of(p.d)) {
+        case 32: return launch_step_lk<T, V, 8, 1>(p, st);
+        case 64: return launch_step_lk<T, V, 16, 1>(p, st);
+        case 128: return launch_step_lk<T, V, 32, 1>(p, st);
+        default: return launch_step_lk<T, V, 32, 2>(p, st);
+    }
+}
+template <typename T>
+cudaError_t launch_step(const DecayParams& p, cudaStream_t st) {
+    return p.vec ? launch_step_v<T, 4>(p, st) : launch_step_v<T, 1>(p, st);
+}
+
+template <int LK, int C, int R>
+cudaError_t launch_scan_r(const DecayParams& p, cudaStream_t st) {
+    // Behind a kernel of many rows an early launch finds room on few SMs and stays there, several blocks to one (three prompts of 301 tokens, 10 heads of 90: 288
+    // and 150 us).
+    const dim3 grid(p.n_seq * p.H, ceil_div(p.d, kScanThreads / 32 * State<LK, C, R>::kRows));
+    if (p.n_tok > kTile) {
+        decay_scan_kernel<LK, C, R><<<grid, kScanThreads, 0, st>>>(p);
+        note_launch();
+        return cudaGetLastError();
+    }
+    return launch_dependent(decay_scan_kernel<LK, C, R>, grid, dim3(kScanThreads), 0, st, p);
 }
 cudaError_t launch_scan(const DecayParams& p, cudaStream_t st) {
-    if (p.d <= 32) return launch_scan_kp<4, 1>(p, st);
-    if (p.d <= 64) return launch_scan_kp<8, 2>(p, st);
-    if (p.d <= 128) return launch_scan_kp<16, 4>(p, st);
-    return launch_scan_kp<32, 2>(p, st);
+    // twice the rows to a lane once that leaves every SM two blocks
+    const long long units = static_cast<long long>(p.n_seq) * p.H;
+    switch (keys_of(p.d)) {
+        case 32: return launch_scan_r<8, 1, 4>(p, st);
+        case 64: return launch_scan_r<16, 1, 4>(p, st);
+        case 128: return units >= 2 * kNumSm ? launch_scan_r<32, 1, 16>(p, st) : launch_scan_r<32, 1, 8>(p, st);
+        default: return launch_scan_r<32, 2, 8>(p, st);
+    }
 }
 
 enum Route { kAuto = 0, kScan = 1, kChunk = 2 };
 constexpr int kChunkMinTokens = 48;
 
 struct Plan {
-    int route;
+    int route, whole;            // whole: the scan of a few tokens in one launch
     size_t q, k, raw, chunk, bytes;
 };
 
@@ -170,12 +400,13 @@ Plan make_plan(const tbl_decay_mixer& m, int precision, int route, int n_seq, in
     w.route = route != kAuto ? route : precision == TBL_BF16 && n_tok >= kChunkMinTokens && decay_chunk_supported(m) ? kChunk : kScan;
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };
-    const size_t numbers = w.route == kScan ? static_cast<size_t>(n_seq) * n_tok * m.heads * m.dim : 0;
+    w.whole = w.route == kScan && step_supported(m, n_tok);
+    const size_t numbers = w.route == kScan && !w.whole ? static_cast<size_t>(n_seq) * n_tok * m.heads * m.dim : 0;
     w.q = take(4 * numbers);
     w.k = take(4 * numbers);
     w.raw = take(4 * numbers);
     w.chunk = take(w.route == kChunk ? decay_chunk_workspace(m, n_seq, n_tok) : 0);
-    w.bytes = off;
+    w.bytes = off > 0 ? off : 256;
     return w;
 }
 
@@ -209,6 +440,7 @@ int launch_decay(const tbl_decay_mixer& m, int precision, int route, float eps, 
     p.ld = m.in.outputs; p.H = m.heads; p.d = m.dim; p.v_off = 2 * m.heads * m.dim; p.g_off = m.gated ? 3 * m.heads * m.dim : -1;
     p.n_seq = n_seq; p.n_tok = n_tok; p.scale = m.scale; p.eps = eps; p.vec = vector_heads(m.rotation, m.dim, proj, p.ld);
     if (w.route == kChunk) return launch_decay_chunks(m, p, base + w.chunk, st);
+    if (w.whole) return (precision == TBL_BF16 ? launch_step<bf16>(p, st) : launch_step<float>(p, st)) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
     float *q = reinterpret_cast<float*>(base + w.q), *k = reinterpret_cast<float*>(base + w.k);
     p.q = q; p.k = k; p.raw = reinterpret_cast<float*>(base + w.raw);
     const RotationCall c{proj, p.ld, m.heads, m.heads, m.dim, slots, positions, n_seq, n_tok, eps, q, k};

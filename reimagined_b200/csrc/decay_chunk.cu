@@ -3,16 +3,16 @@
 // With y = exp(log_decay) and S the state before a chunk, the token i of the chunk (from 0 on) has
 //   o_i = scale (sum_{j <= i} y^(i-j) (q_i . k_j) v_j + y^(i+1) S q_i),      S' = y^n S + sum_j y^(n-1-j) v_j k_j^T.
 //
-//   decay_sums_kernel    the last sum of every chunk: no chunk waits for another
+//   decay_sums_kernel    the last sum of every chunk: no chunk waits for another; keys and values as the operands of the products below
 //   decay_join_kernel    the states before the chunks one after the other, element by element in fp32
 //   decay_chunk_kernel   the outputs of every chunk: two products for the tokens inside, one for the state
-// Queries and keys are normed and turned where they are read, from the fp32 projections: what has to pass through memory is the projections, twice for keys and
-// values.  A long prompt goes by pieces whose projections and sums stay in the second-level cache between the three kernels.
+// Queries and keys are normed and turned where they are read, from the fp32 projections, which pass through memory once.  A long prompt goes by pieces whose
+// operands and sums stay in the second-level cache between the three kernels.
 //
-// Precision.  The states are sums over the whole sequence and stay fp32: their products take both operands as three bf16 terms each (24 bits; six products, the
-// five small ones in an accumulator of their own, so that what the tensor core's sums cut off is of their size).  Outputs are rounded to bf16, so their operands are
-// fp16 under a power of two for every token, and for every row of a state (errors of 2^-12; keys, values and weights y^(i-j) share the smallest of their
-// factors of a chunk, which only costs numbers 2^-14 below the chunk's largest their last bits).
+// Precision.  The states are sums over the whole sequence and stay fp32: their products take both operands as two fp16 terms each (22 bits, three products; numbers
+// 2^-14 below a tile's largest keep fewer).  Outputs are rounded to bf16, so their operands are single fp16 terms under a power of two for every token, and for every
+// row of a state (errors of 2^-12; a weight carries the factors of its key and value beside the largest of the chunk, which only costs numbers 2^-14
+// below that their last bits).
 #include <cuda_fp16.h>
 
 #include "decay.cuh"
@@ -32,10 +32,13 @@ constexpr uint32_t kTransposeA = 1u << 15, kTransposeB = 1u << 16;
 struct ChunkParams {
     DecayParams d;
     float* sums;                 // [unit][chunk of the piece][key / 4][value][4]
+    uint8_t* tokens;             // [unit][chunk]: keys, then values in fp16, as they lie in shared memory (128 rows, swizzled tiles of 64 columns)
+    float* powers;               // [unit][chunk][2][128]: the power of two a token's key, value was divided by
     uint8_t* images;             // [unit][chunk]: the state before it as the B operand [value][key] of fp16, as it lies in shared memory
     float* scales;               // [unit][chunk][value]: the power of two its rows were divided by
     const float* states;         // before the piece
     int first, chunks;           // first token of the piece, its chunks for each sequence
+    float per_dim;               // 1 / d
 };
 
 // sixteen-bit operands that lie with neighbours of the M or N side together: rows of 64 (128 bytes, swizzled), a row per token, groups of 8 tokens 1024 bytes
@@ -46,90 +49,160 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t addr, int box) {
 // place of column c of row r in tiles of 64 columns, `tile` bytes each
 __device__ __forceinline__ uint32_t swizzled(int r, int c, int tile) { return (c >> 6) * tile + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2; }
 
-template <int V>
-__device__ __forceinline__ void put_halves(uint8_t* base, int r, int c, int tile, const float* v, float f) {
-    uint8_t* dst = base + swizzled(r, c, tile);
-    if (V == 4) {
-        const __half2 a = __floats2half2_rn(v[0] * f, v[V > 1 ? 1 : 0] * f), b = __floats2half2_rn(v[V > 2 ? 2 : 0] * f, v[V > 3 ? 3 : 0] * f);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    } else {
-        *reinterpret_cast<__half*>(dst) = __float2half_rn(v[0] * f);
+// A head's numbers over the lanes of a warp: LPH lanes for a token, 32 / LPH tokens side by side, eight numbers a lane in units of 2 V (head_rotation.cuh).  What
+// does not change from token to token stays in registers: a run's columns, and its place in a row of operands.  EXACT: the head is DP wide.
+template <int DP, int V, bool EXACT>
+struct HeadLane {
+    static constexpr int kLph = V == 4 ? DP / 8 : 32, kSide = 32 / kLph, kUnits = 4 / V, kRuns = 2 * kUnits;
+    using Units = HeadUnits<V, kLph>;
+    int at[kRuns];               // column of a run
+    uint32_t mix[kRuns];         // its 16-byte piece of a row of 64, mixed with the lane's own token of those side by side
+    __device__ __forceinline__ HeadLane(const Rotation& r, int gl, int group) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) Units::runs(r, gl + kLph * u, at[2 * u], at[2 * u + 1]);
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u) mix[u] = (((at[u] >> 3) & 7) ^ group) << 4;
     }
-}
-// three bf16 terms of each number, in three tiles `piece` bytes apart
-template <int V>
-__device__ __forceinline__ void put_terms(uint8_t* base, int r, int c, int tile, int piece, const float* v, float f) {
-    uint8_t* dst = base + swizzled(r, c, tile);
-    float x[4];
+    // byte of run u in row 8 k + i kSide + group of tiles of 64 columns, `tile` bytes each
+    __device__ __forceinline__ uint32_t place(int u, int k8, int i, int group, int tile) const {
+        return static_cast<uint32_t>((at[u] >> 6) * tile + (at[u] & 7) * 2 + (k8 + group) * 128) + (mix[u] ^ (((i * kSide) & 7) << 4)) + i * kSide * 128;
+    }
+    __device__ __forceinline__ void load(const float* src, int dim, float (&x)[8]) const {
 #pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = v[e] * f;
+        for (int u = 0; u < kRuns; ++u) Units::load_run(src, at[u], EXACT ? 1 << 30 : dim, x + V * u);
+    }
+    // the angles of a table row for this lane's pairs (units that do not turn: cos 1, sin 0)
+    __device__ __forceinline__ void angles(const Rotation& r, int gl, int row, float (&c)[4], float (&s)[4]) const {
 #pragma unroll
-    for (int t = 0; t < 3; ++t) {
-        if (V == 4) {
-            const uint32_t a = pack_bf16(x[0], x[V > 1 ? 1 : 0]), b = pack_bf16(x[V > 2 ? 2 : 0], x[V > 3 ? 3 : 0]);
-            *reinterpret_cast<uint2*>(dst + t * piece) = make_uint2(a, b);
-            x[0] -= bf_lo(a); x[V > 1 ? 1 : 0] -= bf_hi(a); x[V > 2 ? 2 : 0] -= bf_lo(b); x[V > 3 ? 3 : 0] -= bf_hi(b);
-        } else {
-            const bf16 a = __float2bfloat16_rn(x[0]);
-            *reinterpret_cast<bf16*>(dst + t * piece) = a;
-            x[0] -= __bfloat162float(a);
+        for (int u = 0; u < kUnits; ++u) {
+            const int n = V * (gl + kLph * u);
+            if (n < r.half) {
+                Units::load_run(r.cos + static_cast<size_t>(row) * r.half, n, 1 << 30, c + V * u);
+                Units::load_run(r.sin + static_cast<size_t>(row) * r.half, n, 1 << 30, s + V * u);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) { c[V * u + e] = 1.0f; s[V * u + e] = 0.0f; }
+            }
         }
     }
-}
-
-// How a token's head lies over the lanes of a warp: LPH lanes for a token, 32 / LPH tokens side by side.
-template <int DP, int V>
-struct Lanes {
-    static constexpr int kLph = V == 4 ? DP / 8 : 32, kSide = 32 / kLph;
-    using Units = HeadUnits<V, kLph>;
+    __device__ __forceinline__ void turn(bool pairs, const float (&c)[4], const float (&s)[4], float (&x)[8]) const {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float *y = x + 2 * V * u, cj = c[V * u + j], sj = s[V * u + j];
+                if (pairs) {
+                    const float a = y[2 * j], b = y[2 * j + 1];
+                    y[2 * j] = a * cj - b * sj;
+                    y[2 * j + 1] = b * cj + a * sj;
+                } else {
+                    const float a = y[j], b = y[V + j];
+                    y[j] = a * cj - b * sj;
+                    y[V + j] = b * cj + a * sj;
+                }
+            }
+    }
 };
 
-__device__ __forceinline__ Rotation unturned() { return Rotation{nullptr, nullptr, 0, 0, 0}; }
-
-// largest number of a head over its lanes, as a power of two (1 for a head of zeros)
-template <int LPH, typename U>
-__device__ __forceinline__ float power_of(const U& x) {
-    float most = 0.0f;
+template <int LPH>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < U::kUnits; ++i)
+    for (int o = LPH / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <int LPH>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-        for (int e = 0; e < static_cast<int>(sizeof(x.x[0]) / 4); ++e) most = fmaxf(most, fabsf(x.x[i][e]));
-#pragma unroll
-    for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const uint32_t power = min(__float_as_uint(most) >> 23, 253u);
+    for (int o = LPH / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// the power of two at or below v (1 for 0), and one over it
+__device__ __forceinline__ float power_of(float v) {
+    const uint32_t power = min(__float_as_uint(v) >> 23, 253u);
     return power ? __uint_as_float(power << 23) : 1.0f;
 }
 __device__ __forceinline__ float inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
+__device__ __forceinline__ float largest(const float (&x)[8]) {
+    float m = fabsf(x[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+    return m;
+}
+__device__ __forceinline__ float squares(const float (&x)[8]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e], x[e], s);
+    return s;
+}
+
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+// V numbers as fp16
+template <int V>
+__device__ __forceinline__ void put_halves(uint8_t* dst, const float* y) {
+    if (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(bits_of(__floats2half2_rn(y[0], y[V > 1 ? 1 : 0])), bits_of(__floats2half2_rn(y[V > 2 ? 2 : 0], y[V > 3 ? 3 : 0])));
+    else *reinterpret_cast<__half*>(dst) = __float2half_rn(y[0]);
+}
+// V numbers as two fp16 terms (22 bits) in tiles `piece` bytes apart, and the first term once more where `also` is
+template <int V>
+__device__ __forceinline__ void put_terms(uint8_t* dst, int piece, const float* y, uint8_t* also) {
+    if (V == 4) {
+        const __half2 a = __floats2half2_rn(y[0], y[V > 1 ? 1 : 0]), b = __floats2half2_rn(y[V > 2 ? 2 : 0], y[V > 3 ? 3 : 0]);
+        const float2 fa = __half22float2(a), fb = __half22float2(b);
+        const uint2 w = make_uint2(bits_of(a), bits_of(b));
+        *reinterpret_cast<uint2*>(dst) = w;
+        if (also) *reinterpret_cast<uint2*>(also) = w;
+        *reinterpret_cast<uint2*>(dst + piece) =
+            make_uint2(bits_of(__floats2half2_rn(y[0] - fa.x, y[V > 1 ? 1 : 0] - fa.y)), bits_of(__floats2half2_rn(y[V > 2 ? 2 : 0] - fb.x, y[V > 3 ? 3 : 0] - fb.y)));
+    } else {
+        const __half a = __float2half_rn(y[0]);
+        *reinterpret_cast<__half*>(dst) = a;
+        if (also) *reinterpret_cast<__half*>(also) = a;
+        *reinterpret_cast<__half*>(dst + piece) = __float2half_rn(y[0] - __half2float(a));
+    }
+}
 
 struct Place {
-    int unit, seq, head, chunk, first, n, slot, pos0;    // first: token of the sequence's portion; n: tokens of the chunk
+    int unit, seq, head, chunk, n, slot, pos0;           // n: tokens of the chunk
+    size_t at, row0;                                     // index of (unit, chunk), first row of the projections
 };
 __device__ __forceinline__ Place place_of(const ChunkParams& c, int unit, int chunk) {
     Place a;
     a.unit = unit; a.seq = unit / c.d.H; a.head = unit % c.d.H; a.chunk = chunk;
-    a.first = c.first + chunk * kTokens;
-    a.n = min(kTokens, c.d.n_tok - a.first);
+    const int first = c.first + chunk * kTokens;
+    a.n = min(kTokens, c.d.n_tok - first);
     a.slot = c.d.slots[a.seq];
-    a.pos0 = c.d.positions[a.slot] + a.first;
+    a.pos0 = c.d.positions[a.slot] + first;
+    a.at = static_cast<size_t>(unit) * c.chunks + chunk;
+    a.row0 = static_cast<size_t>(a.seq) * c.d.n_tok + first;
     return a;
 }
 __device__ __forceinline__ int table_row(const DecayParams& p, int pos) { return p.r.half > 0 ? min(max(pos, 0), p.r.positions - 1) : 0; }
 
+// the power of two that a normed head's numbers are divided by: sqrt(d) times the largest weight bounds them
+template <int LPH>
+__device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
+    return power_of(sqrtf(static_cast<float>(dim)) * lanes_max<LPH>(largest(w)));
+}
+
 // ---- sums of the chunks -----------------------------------------------------------------------------------------------------------------
-// One CTA per (unit, chunk): D[value][key] = sum over tokens, M = 128 values (of which DP count), N = DP keys, two tiles of 64 tokens; both operands lie as they come, a row
-// per token.  Bound by memory and by the cutting of numbers into terms; two CTAs to an SM.
-template <int DP, int V>
+// One CTA per (unit, chunk), two tiles of 64 tokens: D[value][key] = sum over a tile's tokens, M = 128 values (of which DP count), N = DP keys; both operands lie as they
+// come, a row per token.  Keys are divided by their power of two, values (times the decay to the chunk's end) by the tile's largest, both then brought up to 2^14, where
+// fp16 has room below: two terms hold 22 bits, three products 22 bits of the sums, which a tile has in columns of its own.  The keys' first terms and the values
+// go to decay_chunk_kernel on the way, as the tiles that it multiplies.  Bound by instructions, ten for a number; two CTAs to an SM.
+constexpr float kUp = 8192.0f;                           // 2^13: numbers below 2 end below 2^14
+template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkParams c) {
-    using Ln = Lanes<DP, V>;
-    constexpr int kPiece = DP / 64 * kBox, kPerWarp = 64 / kWarps, kRounds = kPerWarp / Ln::kSide;
+    using Lane = HeadLane<DP, V, EXACT>;
+    constexpr int kPiece = DP / 64 * kBox, kTile = DP / 64 * kSub, kPerWarp = 64 / kWarps, kRounds = kPerWarp / Lane::kSide, kRuns = Lane::kRuns;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(8) uint64_t done;
     __shared__ uint32_t tmem_slot;
-    uint8_t *k_s = smem, *v_s = smem + 3 * kPiece;       // three terms each (the values' last tile may be read past its end: room for that is behind)
-    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    __shared__ float weight_s[kTokens], most_s[2][kWarps];       // weight_s: decay from a token to the end of its chunk, 0 behind it
+    uint8_t *k_s = smem, *v_s = smem + 2 * kPiece;       // two terms each (the values' last tile may be read past its end: room for that is behind)
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const DecayParams& p = c.d;
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         mbar_init(&done, 1);
         fence_mbar_init();
     }
@@ -137,8 +210,6 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (p.d != DP)                                       // columns nobody writes
-        for (int i = threadIdx.x; i < 6 * kPiece / 16; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -147,69 +218,106 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
     pdl_wait();
     const Place a = place_of(c, blockIdx.y, blockIdx.x);
     const float rate = p.log_decay[a.head];
-    const int group = lane / Ln::kLph, gl = lane % Ln::kLph;
-    const float* base = p.proj + (static_cast<size_t>(a.seq) * p.n_tok + a.first) * p.ld + a.head * p.d;
-    if (p.r.half > 0 && threadIdx.x == 0 && (a.pos0 < 0 || a.pos0 + a.n > p.r.positions)) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+    if (tid < kTokens) weight_s[tid] = tid < a.n - 1 ? expf(rate * static_cast<float>(a.n - 1 - tid)) : tid < a.n ? 1.0f : 0.0f;
+    const int group = lane / Lane::kLph, gl = lane % Lane::kLph;
+    const Lane kl(p.r, gl, group), vl(Rotation{nullptr, nullptr, 0, 0, 0}, gl, group);
+    const float* base = p.proj + a.row0 * p.ld + a.head * p.d;
+    if (p.r.half > 0 && tid == 0 && (a.pos0 < 0 || a.pos0 + a.n > p.r.positions)) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+    float w[8], bound = 1.0f;
+    const bool normed = p.k_norm != nullptr;
+    if (normed) {
+        kl.load(p.k_norm, p.d, w);
+        bound = bound_of<Lane::kLph>(w, p.d);
+    }
+    uint8_t* keys = c.tokens + a.at * 2 * kTile;
+    float* powers = c.powers + a.at * 2 * kTokens;
+    __syncthreads();
     bool alive = true;
-    const int tiles = (a.n + 63) / 64;
-    for (int tile = 0; tile < tiles; ++tile) {
-        typename Ln::Units k[kRounds], v[kRounds];
+    float back[2];                                       // from a tile's sums to theirs
 #pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-            const int j = tile * 64 + warp * kPerWarp + i * Ln::kSide + group, n = j < a.n ? p.d : 0;
-            const float* src = base + static_cast<size_t>(min(j, a.n - 1)) * p.ld;
-            k[i].load(p.r, src + p.H * p.d, n, gl);
-            v[i].load(unturned(), src + p.v_off, n, gl);
+    for (int tile = 0; tile < 2; ++tile) {
+        float k[kRounds][8], v[kRounds][8], inv[kRounds], up[kRounds], most = 0.0f;
+        const int j0 = tile * 64 + warp * kPerWarp + group;
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {              // (rows behind the last token: that one again, times 0)
+            const float* src = base + static_cast<size_t>(min(j0 + i * Lane::kSide, a.n - 1)) * p.ld;
+            kl.load(src + p.H * p.d, p.d, k[i]);
+            vl.load(src + p.v_off, p.d, v[i]);
         }
-        if (tile) alive = mbar_wait_bounded(&done, 0, p.status);          // the first tile's products have read their operands
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
-            const int r = warp * kPerWarp + i * Ln::kSide + group, j = tile * 64 + r;
-            k[i].template turn<float>(p.r, p.k_norm, p.eps, table_row(p, a.pos0 + min(j, a.n - 1)), p.d, gl);
-            if (j >= a.n) {                              // (the norm of nothing may be 0 / 0)
+            const int j = j0 + i * Lane::kSide;
+            float cs[4], sn[4], power = bound;
+            kl.angles(p.r, gl, table_row(p, a.pos0 + min(j, a.n - 1)), cs, sn);
+            inv[i] = 1.0f;
+            if (normed) {
+                inv[i] = rsqrtf(lanes_sum<Lane::kLph>(squares(k[i])) * c.per_dim + p.eps);
 #pragma unroll
-                for (int u = 0; u < Ln::Units::kUnits; ++u)
-#pragma unroll
-                    for (int e = 0; e < 2 * V; ++e) k[i].x[u][e] = 0.0f;
+                for (int e = 0; e < 8; ++e) k[i][e] *= w[e];
             }
-            const float f = j < a.n - 1 ? expf(rate * static_cast<float>(a.n - 1 - j)) : 1.0f;
+            kl.turn(p.r.interleaved != 0, cs, sn, k[i]);
+            if (!normed) power = power_of(lanes_max<Lane::kLph>(largest(k[i])));
+            const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_of(v_most);
+            inv[i] = j < a.n ? inv[i] * inverse_power(power) * kUp : 0.0f;
+            up[i] = weight_s[j] * power;
+            most = fmaxf(most, v_most * up[i]);
+            // the values as they are, for the products inside the chunk
+            const float f = j < a.n ? inverse_power(v_power) : 0.0f;
 #pragma unroll
-            for (int u = 0; u < Ln::Units::kUnits; ++u) {
-                int x, y;
-                Ln::Units::runs(p.r, gl + Ln::kLph * u, x, y);
-                if (x < p.d) put_terms<V>(k_s, r, x, kBox, kPiece, k[i].x[u], 1.0f);
-                if (y < p.d) put_terms<V>(k_s, r, y, kBox, kPiece, k[i].x[u] + V, 1.0f);
-                Ln::Units::runs(unturned(), gl + Ln::kLph * u, x, y);
-                if (x < p.d) put_terms<V>(v_s, r, x, kBox, kPiece, v[i].x[u], f);
-                if (y < p.d) put_terms<V>(v_s, r, y, kBox, kPiece, v[i].x[u] + V, f);
+            for (int u = 0; u < kRuns; ++u) {
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = v[i][V * u + e] * f;
+                if (vl.at[u] < DP) put_halves<V>(keys + kTile + vl.place(u, tile * 64 + warp * kPerWarp, i, group, kSub), y);
+            }
+            if (gl == 0) { powers[j] = power; powers[kTokens + j] = v_power; }
+        }
+        most = warp_max(most);
+        if (lane == 0) most_s[tile][warp] = most;
+        if (tile) alive = mbar_wait_bounded(&done, 0, p.status);          // the first tile's products have read their operands
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) most = fmaxf(most, most_s[tile][i]);
+        const float top = fmaxf(power_of(most), 7.8886091e-31f), down = inverse_power(top) * kUp;
+        back[tile] = top * (1.0f / (kUp * kUp));
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            const float f = up[i] * down;
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u) {
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = k[i][V * u + e] * inv[i];
+                if (kl.at[u] < DP)
+                    put_terms<V>(k_s + kl.place(u, warp * kPerWarp, i, group, kBox), kPiece, y, keys + kl.place(u, tile * 64 + warp * kPerWarp, i, group, kSub));
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = v[i][V * u + e] * f;
+                if (vl.at[u] < DP) put_terms<V>(v_s + vl.place(u, warp * kPerWarp, i, group, kBox), kPiece, y, nullptr);
             }
         }
         fence_proxy_async();
         __syncthreads();
         if (warp == 0 && elect_one() && alive) {
             tc_fence_after();
-            const uint32_t id = idesc_bf16(DP) | kTransposeA | kTransposeB;
+            const uint32_t id = idesc_f16(DP) | kTransposeA | kTransposeB, d = tmem + tile * DP;
             const uint64_t vd = desc_rows(smem_u32(v_s), kBox), kd = desc_rows(smem_u32(k_s), kBox);
             constexpr int kStep = kPiece / 16;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {                // 16 tokens each; terms whose orders add up to 2 and 1 first
-                const uint32_t more = tile | s;
-                umma_f16(tmem + DP, vd + 2 * kStep + 128 * s, kd + 128 * s, id, more);
-                umma_f16(tmem + DP, vd + 128 * s, kd + 2 * kStep + 128 * s, id, 1);
-                umma_f16(tmem + DP, vd + kStep + 128 * s, kd + kStep + 128 * s, id, 1);
-                umma_f16(tmem + DP, vd + kStep + 128 * s, kd + 128 * s, id, 1);
-                umma_f16(tmem + DP, vd + 128 * s, kd + kStep + 128 * s, id, 1);
-                umma_f16(tmem, vd + 128 * s, kd + 128 * s, id, more);
+            for (int s = 0; s < 4; ++s) {                // the small products first, 16 tokens each
+                umma_f16(d, vd + kStep + 128 * s, kd + 128 * s, id, s != 0);
+                umma_f16(d, vd + 128 * s, kd + kStep + 128 * s, id, 1);
             }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) umma_f16(d, vd + 128 * s, kd + 128 * s, id, 1);
             umma_commit(&done);
         }
     }
-    alive = mbar_wait_bounded(&done, (tiles - 1) & 1, p.status) && alive;
+    alive = mbar_wait_bounded(&done, 1, p.status) && alive;
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;              // value
     if (alive && (warp & 3) * 32 < DP) {
-        float* dst = c.sums + (static_cast<size_t>(a.unit) * c.chunks + a.chunk) * DP * DP;
+        float* dst = c.sums + a.at * DP * DP;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
 #pragma unroll
         for (int q = 0; q < DP / 64; ++q) {
@@ -221,10 +329,10 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
                 float4 f;
-                f.x = __uint_as_float(x[e]) + __uint_as_float(y[e]);
-                f.y = __uint_as_float(x[e + 1]) + __uint_as_float(y[e + 1]);
-                f.z = __uint_as_float(x[e + 2]) + __uint_as_float(y[e + 2]);
-                f.w = __uint_as_float(x[e + 3]) + __uint_as_float(y[e + 3]);
+                f.x = fmaf(__uint_as_float(x[e]), back[0], __uint_as_float(y[e]) * back[1]);
+                f.y = fmaf(__uint_as_float(x[e + 1]), back[0], __uint_as_float(y[e + 1]) * back[1]);
+                f.z = fmaf(__uint_as_float(x[e + 2]), back[0], __uint_as_float(y[e + 2]) * back[1]);
+                f.w = fmaf(__uint_as_float(x[e + 3]), back[0], __uint_as_float(y[e + 3]) * back[1]);
                 reinterpret_cast<float4*>(dst)[(col + e) / 4 * DP + row] = f;
             }
         }
@@ -267,10 +375,8 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
             float most = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[e]));
-#pragma unroll
-            for (int o = kLph / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const uint32_t bits = min(__float_as_uint(most) >> 23, 253u);
-            const float power = bits ? __uint_as_float(bits << 23) : 1.0f, inv = inverse_power(power);
+            most = lanes_max<kLph>(most);
+            const float power = power_of(most), inv = inverse_power(power);
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -298,34 +404,32 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 
 // ---- outputs of the chunks ----------------------------------------------------------------------------------------------------------------
 // One CTA per (unit, chunk).  Scores Q K^T in the first 128 columns of its tensor memory, weights in their place (fp16, the A operand of the second product), the
-// tokens' part of the outputs behind them, then the state's part over the weights.  The state's operand comes by one bulk copy into the keys' room.  Outputs are
-// collected in shared memory, so that gates are read and rows are written whole.
-template <int DP, int V>
+// tokens' part of the outputs behind them, then the state's part over the weights.  Keys and values come by bulk copies while the queries are normed, the state's operand
+// by another into the keys' room.  Outputs are collected in shared memory, so that gates are read and rows are written whole.
+template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkParams c) {
-    using Ln = Lanes<DP, V>;
+    using Lane = HeadLane<DP, V, EXACT>;
     constexpr int kTile = DP / 64 * kSub, kPerWarp = kTokens / kWarps, kLdo = DP + 4, kImage = DP * DP * 2;
-    // rounds of loads in flight at once
-    constexpr int kRounds = kPerWarp / Ln::kSide, kFlight = V == 4 ? (kRounds < 4 ? kRounds : 4) : 2;
+    constexpr int kRounds = kPerWarp / Lane::kSide, kFlight = kRounds < 4 ? kRounds : 4;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ float power_s[kTokens + 1];               // y^n
-    __shared__ float q_f[kTokens], kv_f[kTokens], v_f[kTokens], scale_s[DP], ss_s[2][kTokens], most_s;
-    __shared__ __align__(8) uint64_t bars[3];            // scores, state's image, outputs
+    __shared__ __align__(16) float kv_f[kTokens], scale_s[DP];
+    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[2][kTokens], most_s;       // power_s: y^n
+    __shared__ __align__(8) uint64_t bars[4];            // keys and values, scores, state's image, outputs
     __shared__ uint32_t tmem_slot;
     uint8_t *q_s = smem, *k_s = smem + kTile, *v_s = smem + 2 * kTile;
     float* o_s = reinterpret_cast<float*>(smem);         // afterwards: [token][kLdo]
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const DecayParams& p = c.d;
     if (tid == 0) {
-        for (int i = 0; i < 3; ++i) mbar_init(&bars[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&bars[i], 1);
         fence_mbar_init();
+        fence_proxy_async();
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (p.d != DP)
-        for (int i = tid; i < 3 * kTile / 16; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -333,39 +437,54 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
     pdl_launch_dependents();
     pdl_wait();
     const Place a = place_of(c, blockIdx.y, blockIdx.x);
-    const size_t at = static_cast<size_t>(a.unit) * c.chunks + a.chunk;
+    if (warp == 0 && elect_one()) {
+        mbar_arrive_expect_tx(&bars[0], 2 * kTile);
+        bulk_g2s(k_s, c.tokens + a.at * 2 * kTile, 2 * kTile, &bars[0]);
+    }
+    __syncwarp();
     const float rate = p.log_decay[a.head];
     if (tid <= kTokens) power_s[tid] = tid ? expf(rate * static_cast<float>(tid)) : 1.0f;
-    if (tid < DP) scale_s[tid] = c.scales[at * DP + tid];
-    const int group = lane / Ln::kLph, gl = lane % Ln::kLph;
-    const float* base = p.proj + (static_cast<size_t>(a.seq) * p.n_tok + a.first) * p.ld + a.head * p.d;
-#pragma unroll 1
-    for (int what = 0; what < 3; ++what) {               // queries, keys, values
-        const Rotation r = what < 2 ? p.r : unturned();
-        const float* src = base + (what == 0 ? 0 : what == 1 ? p.H * p.d : p.v_off);
-        const float* norm = what == 0 ? p.q_norm : p.k_norm;
-        uint8_t* dst = smem + what * kTile;
+    if (tid < DP) scale_s[tid] = c.scales[a.at * DP + tid];
+    const int group = lane / Lane::kLph, gl = lane % Lane::kLph;
+    const float* base = p.proj + a.row0 * p.ld + a.head * p.d;
+    {
+        const Lane ql(p.r, gl, group);
+        float w[8], bound = 1.0f;
+        const bool normed = p.q_norm != nullptr;
+        if (normed) {
+            ql.load(p.q_norm, p.d, w);
+            bound = bound_of<Lane::kLph>(w, p.d);
+        }
 #pragma unroll 1
         for (int i0 = 0; i0 < kRounds; i0 += kFlight) {
-            typename Ln::Units x[kFlight];
+            float x[kFlight][8];
 #pragma unroll
             for (int i = 0; i < kFlight; ++i) {
-                const int j = warp * kPerWarp + (i0 + i) * Ln::kSide + group;
-                x[i].load(r, src + static_cast<size_t>(min(j, a.n - 1)) * p.ld, j < a.n ? p.d : 0, gl);
+                const int j = warp * kPerWarp + (i0 + i) * Lane::kSide + group;
+                ql.load(base + static_cast<size_t>(min(j, a.n - 1)) * p.ld, p.d, x[i]);
             }
 #pragma unroll
             for (int i = 0; i < kFlight; ++i) {
-                const int j = warp * kPerWarp + (i0 + i) * Ln::kSide + group;
-                if (what < 2) x[i].template turn<float>(r, norm, p.eps, table_row(p, a.pos0 + min(j, a.n - 1)), p.d, gl);
-                const float power = power_of<Ln::kLph>(x[i]), inv = inverse_power(power);
-                if (gl == 0) (what == 0 ? q_f : what == 1 ? kv_f : v_f)[j] = power;
+                const int j = warp * kPerWarp + (i0 + i) * Lane::kSide + group;
+                float cs[4], sn[4];
+                ql.angles(p.r, gl, table_row(p, a.pos0 + min(j, a.n - 1)), cs, sn);
+                float inv = 1.0f, power = bound;
+                if (normed) {
+                    inv = rsqrtf(lanes_sum<Lane::kLph>(squares(x[i])) * c.per_dim + p.eps);
 #pragma unroll
-                for (int u = 0; u < Ln::Units::kUnits; ++u) {
-                    int y, z;
-                    Ln::Units::runs(r, gl + Ln::kLph * u, y, z);
-                    if (y < p.d) put_halves<V>(dst, j, y, kSub, x[i].x[u], inv);
-                    if (z < p.d) put_halves<V>(dst, j, z, kSub, x[i].x[u] + V, inv);
+                    for (int e = 0; e < 8; ++e) x[i][e] *= w[e];
                 }
+                ql.turn(p.r.interleaved != 0, cs, sn, x[i]);
+                if (!normed) power = power_of(lanes_max<Lane::kLph>(largest(x[i])));
+                const float f = inv * inverse_power(power);
+#pragma unroll
+                for (int u = 0; u < Lane::kRuns; ++u) {
+                    float y[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[e] = x[i][V * u + e] * f;
+                    if (ql.at[u] < DP) put_halves<V>(q_s + ql.place(u, warp * kPerWarp, i0 + i, group, kSub), y);
+                }
+                if (gl == 0) q_f[j] = power;
             }
         }
     }
@@ -374,33 +493,35 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
     bool alive = true;
     if (warp == 0) {
         if (elect_one()) {
+            const bool there = mbar_wait_bounded(&bars[0], 0, p.status);
             tc_fence_after();
-            flash::products(tmem, smem_desc_sw128(smem_u32(q_s)), smem_desc_sw128(smem_u32(k_s)), DP / 16, idesc_f16(kTokens), 0);
-            umma_commit(&bars[0]);
+            if (there) flash::products(tmem, smem_desc_sw128(smem_u32(q_s)), smem_desc_sw128(smem_u32(k_s)), DP / 16, idesc_f16(kTokens), 0);
+            umma_commit(&bars[1]);
         }
         __syncwarp();
     } else if (warp == 1) {                              // the largest factor of a token's key and value together
+        const float* powers = c.powers + a.at * 2 * kTokens;
         float f[kTokens / 32], most = 0.0f;
 #pragma unroll
         for (int i = 0; i < kTokens / 32; ++i) {
             const int j = lane + 32 * i;
             // (as exponents: the product of two powers of two may pass the ends of fp32)
-            f[i] = static_cast<float>(static_cast<int>(__float_as_uint(kv_f[j]) >> 23) + static_cast<int>(__float_as_uint(v_f[j]) >> 23));
+            f[i] = static_cast<float>(static_cast<int>(__float_as_uint(powers[j]) >> 23) + static_cast<int>(__float_as_uint(powers[kTokens + j]) >> 23));
             if (j >= a.n) f[i] = 0.0f;
             most = fmaxf(most, f[i]);
         }
         most = warp_max(most);
 #pragma unroll
-        for (int i = 0; i < kTokens / 32; ++i) kv_f[lane + 32 * i] = exp2f(f[i] - most);
+        for (int i = 0; i < kTokens / 32; ++i) kv_f[lane + 32 * i] = exp2f(f[i] - most) * (1.0f / kUp);     // (keys come brought up by kUp)
         if (lane == 0) most_s = most - 254.0f;
     }
     __syncthreads();
-    alive = mbar_wait_bounded(&bars[0], 0, p.status);
+    alive = mbar_wait_bounded(&bars[1], 0, p.status);
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     if (alive && warp == 0 && elect_one()) {             // the keys are done with
-        mbar_arrive_expect_tx(&bars[1], kImage);
-        bulk_g2s(k_s, c.images + at * kImage, kImage, &bars[1]);
+        mbar_arrive_expect_tx(&bars[2], kImage);
+        bulk_g2s(k_s, c.images + a.at * kImage, kImage, &bars[2]);
     }
     __syncwarp();
     const int row = (warp & 3) * 32 + lane, half = warp >> 2;
@@ -408,22 +529,27 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
 #pragma unroll 1
     for (int ch = 2 * half; ch < 2 * half + 2; ++ch) {
         uint32_t x[32], y[16];
-        if (ch * 32 > (warp & 3) * 32 + 31) {            // nothing of it is visible to these rows
+        if (ch > (warp & 3)) {                           // nothing of it is visible to these rows
 #pragma unroll
             for (int e = 0; e < 16; ++e) y[e] = 0;
         } else {
             tmem_ld32(tmem + lanes + ch * 32, x);
             tmem_ld_wait();
+            const float* power = power_s + (row - ch * 32);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float w[2];
+            for (int e = 0; e < 32; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(kv_f + ch * 32 + e);
+                float w[4];
+                if (ch == (warp & 3)) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int j = ch * 32 + 2 * e + k;
-                    w[k] = j <= row ? __uint_as_float(x[2 * e + k]) * power_s[max(row - j, 0)] * kv_f[j] : 0.0f;
+                    for (int k = 0; k < 4; ++k) w[k] = e + k <= lane ? __uint_as_float(x[e + k]) * power[-(e + k <= lane ? e + k : 0)] : 0.0f;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = __uint_as_float(x[e + k]) * power[-(e + k)];
                 }
-                const __half2 h = __floats2half2_rn(w[0], w[1]);
-                y[e] = *reinterpret_cast<const uint32_t*>(&h);
+                const __half2 h0 = __floats2half2_rn(w[0] * f.x, w[1] * f.y), h1 = __floats2half2_rn(w[2] * f.z, w[3] * f.w);
+                y[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+                y[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
             }
         }
         tmem_st16(tmem + lanes + ch * 32, y);
@@ -437,12 +563,12 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
         const uint32_t id = idesc_f16(DP) | kTransposeB;
 #pragma unroll
         for (int k = 0; k < kTokens / 16; ++k) umma_f16_ta(tmem + kTokens, tmem + (k >> 1) * 32 + (k & 1) * 8, vd + 128 * k, id, k != 0);
-        const bool image = mbar_wait_bounded(&bars[1], 0, p.status);
+        const bool image = mbar_wait_bounded(&bars[2], 0, p.status);
         if (image) flash::products(tmem, smem_desc_sw128(smem_u32(q_s)), smem_desc_sw128(smem_u32(k_s)), DP / 16, idesc_f16(DP), 0);
-        umma_commit(&bars[2]);
+        umma_commit(&bars[3]);
     }
     __syncwarp();
-    if (alive) alive = mbar_wait_bounded(&bars[2], 0, p.status);
+    if (alive) alive = mbar_wait_bounded(&bars[3], 0, p.status);
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     // a row's halves are two threads'; the sums of squares meet in shared memory
@@ -457,13 +583,14 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-            float o[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[k] = fmaf(__uint_as_float(x[e + k]), inside, __uint_as_float(y[e + k]) * (before * scale_s[col + e + k]));
-                if (col + e + k < p.d) ss = fmaf(o[k], o[k], ss);
-            }
-            *reinterpret_cast<float4*>(o_s + row * kLdo + col + e) = make_float4(o[0], o[1], o[2], o[3]);
+            const float4 g = *reinterpret_cast<const float4*>(scale_s + col + e);
+            float4 o;                                    // (columns from d on are zeros)
+            o.x = fmaf(__uint_as_float(x[e]), inside, __uint_as_float(y[e]) * (before * g.x));
+            o.y = fmaf(__uint_as_float(x[e + 1]), inside, __uint_as_float(y[e + 1]) * (before * g.y));
+            o.z = fmaf(__uint_as_float(x[e + 2]), inside, __uint_as_float(y[e + 2]) * (before * g.z));
+            o.w = fmaf(__uint_as_float(x[e + 3]), inside, __uint_as_float(y[e + 3]) * (before * g.w));
+            ss = fmaf(o.x, o.x, ss); ss = fmaf(o.y, o.y, ss); ss = fmaf(o.z, o.z, ss); ss = fmaf(o.w, o.w, ss);
+            *reinterpret_cast<float4*>(o_s + row * kLdo + col + e) = o;
         }
     }
     ss_s[half][row] = ss;
@@ -474,35 +601,43 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
     }
     if (!alive) return;
-    bf16* out = static_cast<bf16*>(p.out) + ((static_cast<size_t>(a.seq) * p.n_tok + a.first) * p.H + a.head) * p.d;
+    bf16* out = static_cast<bf16*>(p.out) + (a.row0 * p.H + a.head) * p.d;
     const float* gate = p.g_off < 0 ? nullptr : base + p.g_off;
     const float* norm = p.norm ? p.norm + a.head * p.d : nullptr;
     const bool vec = p.vec && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && (reinterpret_cast<uintptr_t>(p.norm) & 15) == 0;
+    // (the gate's sigmoid by the fast exponential and reciprocal, 2^-21 each, before a rounding of 2^-9)
+    auto open = [](float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); };
+    auto row_factor = [&](int j) { return norm ? rsqrtf((ss_s[0][j] + ss_s[1][j]) * c.per_dim + p.eps) : 1.0f; };
     if (vec) {
-        constexpr int kLanes = DP / 4;                   // lanes to a row
-        const int col = (tid % kLanes) * 4;
+        constexpr int kLanes = DP / 4, kRows = kThreads / kLanes, kBatch = 8;            // lanes to a row, rows at a time
+        const int col = (tid % kLanes) * 4, j0 = tid / kLanes;
+        if (col >= p.d) return;
         float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-        if (norm && col < p.d) w = *reinterpret_cast<const float4*>(norm + col);
-        if (col < p.d) {
-#pragma unroll 4
-            for (int j = tid / kLanes; j < a.n; j += kThreads / kLanes) {
-                const float4 o = *reinterpret_cast<const float4*>(o_s + j * kLdo + col);
-                float4 g = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                if (gate) {
-                    g = *reinterpret_cast<const float4*>(gate + static_cast<size_t>(j) * p.ld + col);
-                    g = make_float4(sigmoid_f(g.x), sigmoid_f(g.y), sigmoid_f(g.z), sigmoid_f(g.w));
-                }
-                const float n = norm ? 1.0f / sqrtf((ss_s[0][j] + ss_s[1][j]) / static_cast<float>(p.d) + p.eps) : 1.0f;
-                *reinterpret_cast<uint2*>(out + static_cast<size_t>(j) * p.H * p.d + col) =
-                    make_uint2(pack_bf16(o.x * n * w.x * g.x, o.y * n * w.y * g.y), pack_bf16(o.z * n * w.z * g.z, o.w * n * w.w * g.w));
+        if (norm) w = *reinterpret_cast<const float4*>(norm + col);
+#pragma unroll 1
+        for (int b = 0; b < kTokens / kRows; b += kBatch) {
+            float4 g[kBatch];
+            if (gate) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    g[i] = *reinterpret_cast<const float4*>(gate + static_cast<size_t>(min(j0 + (b + i) * kRows, a.n - 1)) * p.ld + col);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int j = j0 + (b + i) * kRows;
+                if (j >= a.n) continue;
+                float4 o = *reinterpret_cast<const float4*>(o_s + j * kLdo + col);
+                const float n = row_factor(j);
+                o = make_float4(o.x * n * w.x, o.y * n * w.y, o.z * n * w.z, o.w * n * w.w);
+                if (gate) o = make_float4(o.x * open(g[i].x), o.y * open(g[i].y), o.z * open(g[i].z), o.w * open(g[i].w));
+                *reinterpret_cast<uint2*>(out + static_cast<size_t>(j) * p.H * p.d + col) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
             }
         }
     } else {
         for (int i = tid; i < a.n * p.d; i += kThreads) {
             const int j = i / p.d, col = i - j * p.d;
-            const float n = norm ? norm[col] / sqrtf((ss_s[0][j] + ss_s[1][j]) / static_cast<float>(p.d) + p.eps) : 1.0f;
-            out[static_cast<size_t>(j) * p.H * p.d + col] =
-                __float2bfloat16_rn(o_s[j * kLdo + col] * n * (gate ? sigmoid_f(gate[static_cast<size_t>(j) * p.ld + col]) : 1.0f));
+            out[static_cast<size_t>(j) * p.H * p.d + col] = __float2bfloat16_rn(o_s[j * kLdo + col] * row_factor(j) * (norm ? norm[col] : 1.0f) *
+                                                                                (gate ? open(gate[static_cast<size_t>(j) * p.ld + col]) : 1.0f));
         }
     }
 }
@@ -510,44 +645,53 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
 int width_of(int dim) { return dim <= 64 ? 64 : 128; }
 
-// Chunks of a piece for each sequence: keys, values, sums and images of a piece stay within this many bytes.
-constexpr size_t kPieceBytes = 96u << 20;
+// Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes.
+constexpr size_t kPieceBytes = 352u << 20;
 int chunks_of(const tbl_decay_mixer& m, int n_seq, int n_tok) {
     const size_t units = static_cast<size_t>(n_seq) * m.heads, w = width_of(m.dim);
-    const size_t chunk = units * (kTokens * m.dim * 8 + w * w * 6);
+    const size_t chunk = units * (kTokens * (m.dim * 8 + w * 4) + w * w * 6);
     const int all = ceil_div(n_tok, kTokens), most = static_cast<int>(kPieceBytes / chunk);
     return most < 1 ? 1 : (most < all ? most : all);
 }
 
-struct Rooms { size_t sums, images, scales, bytes; };
+struct Rooms { size_t sums, tokens, powers, images, scales, bytes; };
 Rooms rooms_of(const tbl_decay_mixer& m, int n_seq, int n_tok) {
     const size_t w = width_of(m.dim), blocks = static_cast<size_t>(n_seq) * m.heads * chunks_of(m, n_seq, n_tok);
     Rooms r{};
-    r.sums = 0;
-    r.images = round_up(blocks * w * w * 4, 256);
-    r.scales = r.images + round_up(blocks * w * w * 2, 256);
-    r.bytes = r.scales + round_up(blocks * w * 4, 256);
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };
+    r.sums = take(blocks * w * w * 4);
+    r.tokens = take(blocks * kTokens * w * 4);
+    r.powers = take(blocks * kTokens * 8);
+    r.images = take(blocks * w * w * 2);
+    r.scales = take(blocks * w * 4);
+    r.bytes = off;
     return r;
 }
 
-template <int DP, int V>
+template <int DP, int V, bool EXACT>
 cudaError_t run(ChunkParams c, int per, cudaStream_t st) {
     static bool sums_done[64] = {}, chunk_done[64] = {};
-    constexpr size_t sums_smem = 1024 + 6 * (DP / 64) * kBox + (DP == 64 ? kBox : 0);
+    constexpr size_t sums_smem = 1024 + 4 * (DP / 64) * kBox + (DP == 64 ? kBox : 0);
     constexpr size_t tiles = 3 * (DP / 64) * kSub, collect = sizeof(float) * kTokens * (DP + 4);
     constexpr size_t chunk_smem = 1024 + (tiles > collect ? tiles : collect);
-    cudaError_t e = allow_smem(decay_sums_kernel<DP, V>, sums_smem, sums_done);
-    if (e == cudaSuccess) e = allow_smem(decay_chunk_kernel<DP, V>, chunk_smem, chunk_done);
+    cudaError_t e = allow_smem(decay_sums_kernel<DP, V, EXACT>, sums_smem, sums_done);
+    if (e == cudaSuccess) e = allow_smem(decay_chunk_kernel<DP, V, EXACT>, chunk_smem, chunk_done);
     const int units = c.d.n_seq * c.d.H, all = ceil_div(c.d.n_tok, kTokens);
     for (int at = 0; e == cudaSuccess && at < all; at += per) {
         c.first = at * kTokens;
         c.chunks = all - at < per ? all - at : per;
         c.states = at == 0 ? c.d.states : c.d.next;
-        e = launch_dependent(decay_sums_kernel<DP, V>, dim3(c.chunks, units), dim3(kThreads), sums_smem, st, c);
+        e = launch_dependent(decay_sums_kernel<DP, V, EXACT>, dim3(c.chunks, units), dim3(kThreads), sums_smem, st, c);
         if (e == cudaSuccess) e = launch_dependent(decay_join_kernel<DP>, dim3(DP * DP / 8 / 128, units), dim3(128), 0, st, c);
-        if (e == cudaSuccess) e = launch_dependent(decay_chunk_kernel<DP, V>, dim3(c.chunks, units), dim3(kThreads), chunk_smem, st, c);
+        if (e == cudaSuccess) e = launch_dependent(decay_chunk_kernel<DP, V, EXACT>, dim3(c.chunks, units), dim3(kThreads), chunk_smem, st, c);
     }
     return e;
+}
+template <int DP>
+cudaError_t run_width(const ChunkParams& c, int per, cudaStream_t st) {
+    if (!c.d.vec) return run<DP, 1, false>(c, per, st);
+    return c.d.d == DP ? run<DP, 4, true>(c, per, st) : run<DP, 4, false>(c, per, st);
 }
 
 }  // namespace
@@ -562,11 +706,10 @@ int launch_decay_chunks(const tbl_decay_mixer& m, const DecayParams& p, void* ws
     uint8_t* base = static_cast<uint8_t*>(ws);
     ChunkParams c{};
     c.d = p;
-    c.sums = reinterpret_cast<float*>(base + r.sums); c.images = base + r.images; c.scales = reinterpret_cast<float*>(base + r.scales);
+    c.per_dim = 1.0f / static_cast<float>(p.d);
+    c.sums = reinterpret_cast<float*>(base + r.sums); c.tokens = base + r.tokens; c.powers = reinterpret_cast<float*>(base + r.powers); c.images = base + r.images; c.scales = reinterpret_cast<float*>(base + r.scales);
     const int per = chunks_of(m, p.n_seq, p.n_tok);
-    cudaError_t e;
-    if (width_of(m.dim) == 64) e = p.vec ? run<64, 4>(c, per, st) : run<64, 1>(c, per, st);
-    else e = p.vec ? run<128, 4>(c, per, st) : run<128, 1>(c, per, st);
+    const cudaError_t e = width_of(m.dim) == 64 ? run_width<64>(c, per, st) : run_width<128>(c, per, st);
     return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
 

@@ -17,6 +17,9 @@ struct Rotation {
 };
 inline Rotation rotation_of(const tbl_head_rotation& r) { return Rotation{r.rope_cos, r.rope_sin, r.rot_dim / 2, r.rope_positions, r.interleaved}; }
 
+__device__ __forceinline__ float reciprocal_root(float v) { return rsqrtf(v); }          // 2 units in the last place
+__device__ __forceinline__ double reciprocal_root(double v) { return 1.0 / sqrt(v); }
+
 // A head spread over LPH lanes, in units of 2 V numbers: V pairs (a, b) that turn together, or numbers that do not turn.  Without `interleaved` a unit that
 // turns is two runs of V neighbours half a rotated part apart, otherwise it is 2 V neighbours.  V = 4: 16-byte accesses (vector_heads below), V = 1: any size.
 template <int V, int LPH>
@@ -59,7 +62,7 @@ struct HeadUnits {
                 for (int e = 0; e < 2 * V; ++e) ss += A(x[i][e]) * A(x[i][e]);
 #pragma unroll
             for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            inv = A(1) / sqrt(ss / A(dim) + A(eps));
+            inv = reciprocal_root(ss / A(dim) + A(eps));
         }
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {

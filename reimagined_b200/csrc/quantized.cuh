@@ -72,11 +72,56 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], float unit, u
     return codes;
 }
 
+// A head of a row: for a key (turned = its rotation) normed and turned in 64 bits, so that the code of a number does not depend on how a sum of squares is rounded;
+// then rounded to 4 bits.  A warp; `mine`: its room for the head's numbers; lane i has the codes of numbers 8 i .. 8 i + 7, even lanes the scale of 16.
+template <int V>
+__device__ __forceinline__ uint32_t quantize_head(const QuantizedParams& p, const float* src, bool is_k, int at, float* mine, int lane, uint8_t& scale) {
+    for (int c = p.d + lane; c < p.width; c += 32) mine[c] = 0.0f;
+    if (is_k) {
+        HeadUnits<V, 32> x;
+        x.load(p.r, src, p.d, lane);
+        x.template turn<double>(p.r, p.k_norm, p.eps, at, p.d, lane);
+        x.store(p.r, mine, p.d, lane);
+    } else {
+        for (int c = lane; c < p.d; c += 32) mine[c] = src[c];
+    }
+    __syncwarp();
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = 8 * lane < p.width ? mine[8 * lane + i] : 0.0f;
+    const uint32_t codes = quantize8(y, is_k ? p.key_unit : p.value_unit, scale);
+    __syncwarp();
+    return codes;
+}
+// its place in a row (in global or shared memory); a value's warp writes the row's padding too
+__device__ __forceinline__ void put_row(const QuantizedParams& p, uint8_t* dst, bool is_k, uint32_t codes, uint8_t scale, int lane) {
+    if (8 * lane < p.width) {
+        reinterpret_cast<uint32_t*>(dst + (is_k ? 0 : p.width / 2))[lane] = codes;
+        if ((lane & 1) == 0) dst[p.width + (is_k ? 0 : p.width / 16) + lane / 2] = scale;
+    }
+    const int used = p.width + p.width / 8;
+    if (!is_k && used + lane < p.row) dst[used + lane] = 0;
+}
+// fp16 queries: the power of two a head is divided by, so that its largest number lies in [1, 2), and the factor that does it
+template <int V>
+__device__ __forceinline__ float query_power(const HeadUnits<V, 32>& x, float& factor) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HeadUnits<V, 32>::kUnits; ++i)
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) most = fmaxf(most, fabsf(x.x[i][e]));
+    const uint32_t power = min(__float_as_uint(warp_max(most)) >> 23, 253u);
+    factor = power ? __uint_as_float((254u - power) << 23) : 1.0f;
+    return power ? __uint_as_float(power << 23) : 1.0f;
+}
+
 // quantized_decode.cu: streams the 4-bit rows for a few query rows
-bool quantized_stream_supported(const tbl_quantized_mixer& m);
-int quantized_stream_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
-bool quantized_stream_whole(const tbl_quantized_mixer& m, int splits);     // finishes its rows itself (otherwise it leaves partial sums)
-int launch_quantized_stream(const QuantizedParams& p, int n_seq, cudaStream_t st);
+struct StreamPlan {
+    int warps, splits;           // of a CTA; of the context
+    int whole;                   // one token of a sequence, no splits: the kernel norms, rounds, appends and finishes by itself
+};
+StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
+int launch_quantized_stream(const QuantizedParams& p, const StreamPlan& plan, int vec, int n_seq, cudaStream_t st);
 
 }  // namespace stack
 }  // namespace tbl

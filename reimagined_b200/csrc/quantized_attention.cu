@@ -16,8 +16,7 @@ namespace {
 
 constexpr int kPrepWarps = 8;
 
-// A warp per head of a row: query heads, then key heads, then value heads.  Keys are normed and turned in 64 bits, so that the code of a number does not depend on
-// how a sum of squares is rounded (64-bit arithmetic of 2 x 8 numbers a lane; the row's projections take longer to arrive).
+// A warp per head of a row: query heads, then key heads, then value heads.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kPrepWarps) quantized_prep_kernel(const QuantizedParams p) {
     __shared__ __align__(16) float head_s[kPrepWarps][TBL_MAX_ROTATED_DIM];
@@ -35,19 +34,9 @@ __global__ void __launch_bounds__(32 * kPrepWarps) quantized_prep_kernel(const Q
         x.template turn<float>(p.r, p.q_norm, p.eps, at, p.d, lane);
         T* dst = static_cast<T*>(p.q) + (static_cast<size_t>(row) * p.H + head) * p.ldq;
         float f = 1.0f;
-        if (sizeof(T) == 2 && p.q_factor) {                      // fp16: the largest number of a head lies in [1, 2)
-            float most = 0.0f;
-#pragma unroll
-            for (int i = 0; i < HeadUnits<V, 32>::kUnits; ++i)
-#pragma unroll
-                for (int e = 0; e < 2 * V; ++e) most = fmaxf(most, fabsf(x.x[i][e]));
-            const uint32_t power = min(__float_as_uint(warp_max(most)) >> 23, 253u);
-            if (power) {
-                f = __uint_as_float((254u - power) << 23);
-                if (lane == 0) p.q_factor[static_cast<size_t>(row) * p.H + head] = __uint_as_float(power << 23);
-            } else if (lane == 0) {
-                p.q_factor[static_cast<size_t>(row) * p.H + head] = 1.0f;
-            }
+        if (sizeof(T) == 2 && p.q_factor) {
+            const float power = query_power(x, f);
+            if (lane == 0) p.q_factor[static_cast<size_t>(row) * p.H + head] = power;
         }
         x.store(p.r, dst, p.d, lane, f);
         for (int c = p.d + lane; c < p.ldq; c += 32) dst[c] = from_f<T>(0.0f);
@@ -58,29 +47,9 @@ __global__ void __launch_bounds__(32 * kPrepWarps) quantized_prep_kernel(const Q
         return;
     }
     const bool is_k = head < p.H + p.G;
-    float* mine = head_s[warp];
-    for (int c = p.d + lane; c < p.width; c += 32) mine[c] = 0.0f;
-    if (is_k) {
-        x.load(p.r, src, p.d, lane);
-        x.template turn<double>(p.r, p.k_norm, p.eps, at, p.d, lane);
-        x.store(p.r, mine, p.d, lane);
-    } else {
-        for (int c = lane; c < p.d; c += 32) mine[c] = src[c];
-    }
-    __syncwarp();
-    const int g = head - p.H - (is_k ? 0 : p.G);
-    uint8_t* dst = quantized_at(p, slot, g, pos);
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = 8 * lane < p.width ? mine[8 * lane + i] : 0.0f;
     uint8_t scale;
-    const uint32_t codes = quantize8(y, is_k ? p.key_unit : p.value_unit, scale);
-    if (8 * lane < p.width) {
-        reinterpret_cast<uint32_t*>(dst + (is_k ? 0 : p.width / 2))[lane] = codes;
-        if ((lane & 1) == 0) dst[p.width + (is_k ? 0 : p.width / 16) + lane / 2] = scale;
-    }
-    const int used = p.width + p.width / 8;
-    if (!is_k && used + lane < p.row) dst[used + lane] = 0;
+    const uint32_t codes = quantize_head<V>(p, src, is_k, at, head_s[warp], lane, scale);
+    put_row(p, quantized_at(p, slot, head - p.H - (is_k ? 0 : p.G), pos), is_k, codes, scale, lane);
 }
 
 // ---- cached numbers ---------------------------------------------------------------------------------------------------------
@@ -151,6 +120,52 @@ __global__ void __launch_bounds__(256) quantized_read_kernel(const QuantizedPara
     }
 }
 
+// ---- splits of the context come together --------------------------------------------------------------------------------------
+// A CTA per (row, head); a warp takes every eighth split, a lane four neighbouring numbers, so that all partial sums are on their way at once.
+constexpr int kMergeWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(32 * kMergeWarps) quantized_merge_kernel(const QuantizedParams p) {
+    __shared__ __align__(16) float part_s[kMergeWarps][TBL_MAX_ROTATED_DIM];
+    pdl_launch_dependents();
+    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const size_t unit = (static_cast<size_t>(row) * p.H + head) * p.splits;
+    pdl_wait();
+    const float gate = p.g_off >= 0 && tid < p.d ? p.proj[static_cast<size_t>(row) * p.ld + p.g_off + head * p.d + tid] : 0.0f;
+    float most = -INFINITY, sum = 0.0f;
+    for (int s = lane; s < p.splits; s += 32) most = fmaxf(most, p.part_m[unit + s]);
+    most = warp_max(most);
+    for (int s = lane; s < p.splits; s += 32) {
+        const float m = p.part_m[unit + s];
+        sum = fmaf(p.part_l[unit + s], m == -INFINITY ? 0.0f : ex2(m - most), sum);
+    }
+    sum = warp_sum(sum);
+    float4 acc[TBL_MAX_ROTATED_DIM / 128];
+#pragma unroll
+    for (int b = 0; b < TBL_MAX_ROTATED_DIM / 128; ++b) acc[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int s = warp; s < p.splits; s += kMergeWarps) {
+        const float m = p.part_m[unit + s], f = m == -INFINITY ? 0.0f : ex2(m - most);
+        const float* src = p.part_o + (unit + s) * p.ldo;
+#pragma unroll
+        for (int b = 0; b < TBL_MAX_ROTATED_DIM / 128; ++b)
+            if (128 * b + 4 * lane < p.ldo) {
+                const float4 x = *reinterpret_cast<const float4*>(src + 128 * b + 4 * lane);
+                acc[b].x = fmaf(x.x, f, acc[b].x); acc[b].y = fmaf(x.y, f, acc[b].y); acc[b].z = fmaf(x.z, f, acc[b].z); acc[b].w = fmaf(x.w, f, acc[b].w);
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < TBL_MAX_ROTATED_DIM / 128; ++b) *reinterpret_cast<float4*>(&part_s[warp][128 * b + 4 * lane]) = acc[b];
+    __syncthreads();
+    if (tid < p.d) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; ++w) v += part_s[w][tid];
+        v *= p.value_unit / sum;
+        static_cast<T*>(p.out)[(static_cast<size_t>(row) * p.H + head) * p.d + tid] = from_f<T>(p.g_off >= 0 ? v * sigmoid_f(gate) : v);
+    }
+}
+static_assert(32 * kMergeWarps >= TBL_MAX_ROTATED_DIM, "a thread per number");
+
 // ---- plan -------------------------------------------------------------------------------------------------------------------
 enum Route { kAuto = 0, kSimt = 1, kStream = 2, kFlash = 3 };
 constexpr int kFlashMinTokens = 48;
@@ -166,12 +181,12 @@ tbl_attention_mixer as_attention(const tbl_quantized_mixer& m) {
 
 int pick_route(const tbl_quantized_mixer& m, int precision, int n_tok) {
     if (precision != TBL_BF16) return kSimt;
-    if (n_tok >= kFlashMinTokens && attention_flash_supported(as_attention(m))) return kFlash;
-    return quantized_stream_supported(m) ? kStream : kSimt;
+    return n_tok >= kFlashMinTokens && attention_flash_supported(as_attention(m)) ? kFlash : kStream;
 }
 
 struct Plan {
     int route, splits, ctx;
+    StreamPlan stream;
     size_t q, factor, expanded, pm, pl, po, bytes;
 };
 
@@ -182,8 +197,9 @@ Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq
     w.splits = 1;
     bool parts = w.route == kSimt || (w.route == kFlash && !attention_flash_whole(as_attention(m)));
     if (w.route == kStream) {
-        w.splits = quantized_stream_splits(m, n_seq, n_tok, context);
-        parts = !quantized_stream_whole(m, w.splits);
+        w.stream = quantized_stream_plan(m, n_seq, n_tok, context);
+        w.splits = w.stream.splits;
+        parts = w.splits > 1;
     } else if (w.route == kSimt) {
         const long long units = static_cast<long long>(ceil_div(static_cast<long long>(n_tok) * (m.heads / m.kv_heads), 16)) * n_seq * m.kv_heads;
         long long s = 2LL * kNumSm / units;
@@ -214,6 +230,12 @@ cudaError_t launch_prep(const QuantizedParams& p, int rows, bool vec, cudaStream
     return vec ? launch_prep_v<T, 4>(p, rows, st) : launch_prep_v<T, 1>(p, rows, st);
 }
 
+int launch_merge(const QuantizedParams& p, int precision, int rows, cudaStream_t st) {
+    const dim3 grid(rows, p.H), block(32 * kMergeWarps);
+    return (precision == TBL_BF16 ? launch_dependent(quantized_merge_kernel<bf16>, grid, block, 0, st, p)
+                                  : launch_dependent(quantized_merge_kernel<float>, grid, block, 0, st, p)) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+}
+
 // partial sums and outputs as attention.cu's merge takes them
 AttnParams merge_params(const QuantizedParams& p, const tbl_quantized_mixer& m) {
     AttnParams a{};
@@ -226,12 +248,13 @@ AttnParams merge_params(const QuantizedParams& p, const tbl_quantized_mixer& m) 
 int run(const tbl_quantized_mixer& m, int precision, const QuantizedParams& p, const Plan& w, int n_seq, cudaStream_t st) {
     const int rows = n_seq * p.n_tok;
     const bool vec = vector_heads(m.rotation, p.d, p.proj, p.ld);
-    const cudaError_t e = w.route == kSimt ? launch_prep<float>(p, rows, vec, st) : launch_prep<__half>(p, rows, vec, st);
+    const bool whole = w.route == kStream && w.stream.whole;
+    const cudaError_t e = whole ? cudaSuccess : w.route == kSimt ? launch_prep<float>(p, rows, vec, st) : launch_prep<__half>(p, rows, vec, st);
     if (e != cudaSuccess) return TBL_ERR_CUDA;
     AttnParams a = merge_params(p, m);
     if (w.route == kStream) {
-        const int rc = launch_quantized_stream(p, n_seq, st);
-        return rc != TBL_OK || quantized_stream_whole(m, w.splits) ? rc : launch_attention_merge(a, precision, rows, st);
+        const int rc = launch_quantized_stream(p, w.stream, vec, n_seq, st);
+        return rc != TBL_OK || w.splits == 1 ? rc : launch_merge(p, precision, rows, st);
     }
     const dim3 grid(ceil_div(static_cast<long long>(p.ctx) * (a.dp / 4), 256), n_seq * p.G);
     const cudaError_t x = w.route == kFlash ? launch_dependent(quantized_expand_kernel<__half>, grid, dim3(256), 0, st, p, a.dp)
@@ -250,7 +273,7 @@ int run(const tbl_quantized_mixer& m, int precision, const QuantizedParams& p, c
     }
     a.proj = static_cast<const float*>(p.q); a.ld = p.H * p.d;
     const int rc = launch_attention_simt(a, precision, n_seq, st);
-    return rc != TBL_OK ? rc : launch_attention_merge(a, precision, rows, st);
+    return rc != TBL_OK ? rc : launch_merge(p, precision, rows, st);
 }
 
 QuantizedParams basic_params(const tbl_quantized_mixer& m, int capacity, const int32_t* slots, const int32_t* positions, int n_tok) {
@@ -327,8 +350,7 @@ int tbl_quantized_forward(const tbl_quantized_mixer* mixer, int precision, int r
         return TBL_ERR_INVALID_ARG;
     const int rc = check_quantized(*mixer, mixer->in.inputs);
     if (rc != TBL_OK) return rc;
-    if ((route == kStream && (precision != TBL_BF16 || !quantized_stream_supported(*mixer))) ||
-        (route == kFlash && (precision != TBL_BF16 || !attention_flash_supported(as_attention(*mixer)))))
+    if ((route == kStream && precision != TBL_BF16) || (route == kFlash && (precision != TBL_BF16 || !attention_flash_supported(as_attention(*mixer)))))
         return TBL_ERR_SHAPE;
     if (!workspace_dev || workspace_bytes < tbl_quantized_workspace_bytes(mixer, precision, route, n_seq, n_tok, context)) return TBL_ERR_WORKSPACE;
     if ((reinterpret_cast<uintptr_t>(workspace_dev) & 255) || !aligned16(cache_dev) || !aligned16(out_dev) || (reinterpret_cast<uintptr_t>(proj_dev) & 3))

@@ -21,7 +21,7 @@ namespace tbl {
 namespace stack {
 namespace {
 
-constexpr int kWarps = 4, kTile = 32, kStages = 3;
+constexpr int kTile = 32;
 constexpr float kRescale = 8.0f;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -33,11 +33,13 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// the eight codes of a word as four pairs of halves, times a pair of scales
+// the eight codes of a word as four pairs of halves, times a pair of scales (as one piece of assembly the conversions take their byte of the word by themselves)
 __device__ __forceinline__ void widen(uint32_t codes, __half2 scale, uint32_t (&out)[4]) {
+    asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %4;\ncvt.rn.f16x2.e2m1x2 %0, a;\ncvt.rn.f16x2.e2m1x2 %1, b;\ncvt.rn.f16x2.e2m1x2 %2, c;\ncvt.rn.f16x2.e2m1x2 %3, d;\n}"
+        : "=r"(out[0]), "=r"(out[1]), "=r"(out[2]), "=r"(out[3]) : "r"(codes));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __half2 h = __hmul2(codes_of((codes >> (8 * i)) & 0xffu), scale);
+        const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&out[i]), scale);
         out[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
 }
@@ -57,24 +59,24 @@ __device__ __forceinline__ int token_of(int i) {
     return ((r & 1) ? 8 + (((r & 6) + 4) & 7) : r) + (i >> 3);
 }
 
-template <int DP>
+template <int DP, int NT, int W>
 struct Layout {
-    static constexpr int kRow = (DP + DP / 8 + 15) / 16 * 16, kTileBytes = kTile * kRow, kRing = kWarps * kStages * kTileBytes, kLdo = DP + 4;
+    static constexpr int kStages = W == 4 ? 3 : 2, kRow = (DP + DP / 8 + 15) / 16 * 16, kTileBytes = kTile * kRow, kRing = W * kStages * kTileBytes, kLdo = DP + 4;
+    static constexpr size_t kMerge = sizeof(float) * W * 8 * NT * kLdo, kBytes = kRing > kMerge ? kRing : kMerge;
 };
-template <int DP, int NT>
-constexpr size_t stream_smem() {
-    const size_t ring = Layout<DP>::kRing, merge = sizeof(float) * kWarps * 8 * NT * Layout<DP>::kLdo;
-    return ring > merge ? ring : merge;
-}
 
-// DP: the head size rounded up to 64; NT: blocks of eight query rows.
-template <int DP, int NT>
-__global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const QuantizedParams p) {
-    using L = Layout<DP>;
-    constexpr int kBlocks = DP / 64, kRows = 8 * NT, kThreads = 32 * kWarps;
+// DP: the head size rounded up to 64; NT: blocks of eight query rows; W: warps; V: 0, or how the vectors of a whole call (StreamPlan) are read (HeadUnits).
+template <int DP, int NT, int W, int V>
+__global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const QuantizedParams p) {
+    using L = Layout<DP, NT, W>;
+    constexpr int kBlocks = DP / 64, kRows = 8 * NT, kThreads = 32 * W, kStages = L::kStages;
+    constexpr bool kWhole = V > 0;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows], top_s[kRows], sum_s[kRows];
-    __shared__ __align__(8) uint64_t full[kWarps][kStages];
+    __shared__ float m_s[W][kRows], l_s[W][kRows], top_s[kRows], sum_s[kRows];
+    __shared__ __align__(8) uint64_t full[W][kStages];
+    __shared__ __align__(16) __half q_s[kWhole ? kRows : 1][kWhole ? DP : 8];
+    __shared__ __align__(16) float head_s[kWhole ? (W < 8 ? W : 8) : 1][kWhole ? DP : 4], factor_s[kRows];
+    __shared__ __align__(16) uint8_t fresh_s[kWhole ? L::kRow : 16];
     float* o_s = reinterpret_cast<float*>(smem);                 // afterwards: [warp][row][kLdo]
     const int tid = threadIdx.x, warp = tc05::uniform_warp(), lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
     const int seq = blockIdx.x / p.G, g = blockIdx.x % p.G, first = blockIdx.y * kRows, split = blockIdx.z;
@@ -89,18 +91,51 @@ __global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const Qua
     const int n = min(pos0 + min(total - 1, first + kRows - 1) / p.group + 1, p.capacity);       // tokens the last row sees
     const int per = ((n + p.splits - 1) / p.splits + kTile - 1) / kTile * kTile;
     const int t0 = min(split * per, max(n, 0)), t1 = min(n, t0 + per);
+    // the token of a whole call (at pos0, the last one) comes from the projections, not from the cache
+    const int fresh = kWhole && quantized_room(p, pos0) ? pos0 : -1, cached = fresh >= 0 ? min(t1, fresh) : t1;
     const uint8_t* cache = quantized_at(p, slot, g, 0);
     uint8_t* ring = smem + warp * kStages * L::kTileBytes;
     auto load_tile = [&](int stage, int t) {                     // rows past the split's end stay whatever shared memory holds: they are masked
         if (t < t1 && tc05::elect_one()) {
-            const uint32_t bytes = min(kTile, t1 - t) * L::kRow;
-            mbar_arrive_expect_tx(&full[warp][stage], bytes);
-            bulk_g2s(ring + stage * L::kTileBytes, cache + static_cast<size_t>(t) * L::kRow, bytes, &full[warp][stage]);
+            const int rows = min(kTile, cached - t);
+            if (!kWhole || rows > 0) {
+                mbar_arrive_expect_tx(&full[warp][stage], rows * L::kRow);
+                bulk_g2s(ring + stage * L::kTileBytes, cache + static_cast<size_t>(t) * L::kRow, rows * L::kRow, &full[warp][stage]);
+            } else {
+                mbar_arrive(&full[warp][stage]);
+            }
         }
     };
-    const int begin = t0 + warp * kTile, step = kWarps * kTile;
+    const int begin = t0 + warp * kTile, step = W * kTile;
 #pragma unroll
     for (int s = 0; s < kStages; ++s) load_tile(s, begin + s * step);
+    if constexpr (kWhole) {                                      // a warp per head: queries, the key, the value
+        constexpr int kHeads = W < 8 ? W : 8;
+        const float* src = p.proj + static_cast<size_t>(seq) * p.ld;
+        const int at = p.r.half > 0 ? min(max(pos0, 0), p.r.positions - 1) : 0;
+        for (int i = tid; i < kRows * DP / 8; i += kThreads) reinterpret_cast<uint4*>(&q_s[0][0])[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        if (warp < kHeads)
+            for (int i = warp; i < p.group + 2; i += kHeads) {
+                if (i < 2) {                                     // (these first: they take longer)
+                    const bool is_k = i == 0;
+                    uint8_t scale;
+                    const uint32_t codes = quantize_head<V>(p, src + ((is_k ? p.H : p.H + p.G) + g) * p.d, is_k, at, head_s[warp], lane, scale);
+                    put_row(p, fresh_s, is_k, codes, scale, lane);
+                    if (fresh >= 0) put_row(p, quantized_at(p, slot, g, fresh), is_k, codes, scale, lane);
+                } else {
+                    HeadUnits<V, 32> x;
+                    float f;
+                    x.load(p.r, src + (g * p.group + i - 2) * p.d, p.d, lane);
+                    x.template turn<float>(p.r, p.q_norm, p.eps, at, p.d, lane);
+                    const float power = query_power(x, f);
+                    if (lane == 0) factor_s[i - 2] = power;
+                    x.store(p.r, q_s[i - 2], p.d, lane, f);
+                }
+            }
+        if (fresh < 0 && tid == 0 && g == 0) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+        __syncthreads();
+    }
     // queries: B fragments of every step, two rows (2 t4, 2 t4 + 1) of factors
     uint32_t q[NT][kBlocks][4][2];
     float c[NT][2];
@@ -108,7 +143,8 @@ __global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const Qua
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
         const int at = first + 8 * u + g8, ok = at < total, r = ok ? at : 0;
-        const __half* src = static_cast<const __half*>(p.q) + ((static_cast<size_t>(seq) * p.n_tok + r / p.group) * p.H + g * p.group + r % p.group) * DP;
+        const __half* src = kWhole ? q_s[kWhole ? 8 * u + g8 : 0]
+                                   : static_cast<const __half*>(p.q) + ((static_cast<size_t>(seq) * p.n_tok + r / p.group) * p.H + g * p.group + r % p.group) * DP;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
@@ -120,7 +156,7 @@ __global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const Qua
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int row = min(first + 8 * u + 2 * t4 + e, total - 1);
-            c[u][e] = p.scale_log2 * p.q_factor[(static_cast<size_t>(seq) * p.n_tok + row / p.group) * p.H + g * p.group + row % p.group];
+            c[u][e] = p.scale_log2 * (kWhole ? factor_s[row] : p.q_factor[(static_cast<size_t>(seq) * p.n_tok + row / p.group) * p.H + g * p.group + row % p.group]);
             last[u][e] = min(pos0 + row / p.group, t1 - 1);
         }
     }
@@ -143,6 +179,11 @@ __global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const Qua
         // (after a wait that gave up nothing more is asked for, and what is on its way gets a short time)
         alive = __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, p.status, alive ? kWaitSpinLimit : 1024)) && alive;
         const uint32_t tile = smem_u32(ring + stage * L::kTileBytes);
+        if (kWhole && fresh >= t && fresh < t + kTile) {
+            uint32_t* dst = reinterpret_cast<uint32_t*>(ring + stage * L::kTileBytes + (fresh - t) * L::kRow);
+            for (int i = lane; i < L::kRow / 4; i += 32) dst[i] = reinterpret_cast<const uint32_t*>(fresh_s)[i];
+            __syncwarp();
+        }
         float s[2][NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -269,11 +310,11 @@ __global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const Qua
         const int r = i / (DP / 4), col = (i % (DP / 4)) * 4;
         float top = m_s[0][r];
 #pragma unroll
-        for (int k = 1; k < kWarps; ++k) top = fmaxf(top, m_s[k][r]);
+        for (int k = 1; k < W; ++k) top = fmaxf(top, m_s[k][r]);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
+        for (int k = 0; k < W; ++k) {
             const float w = m_s[k][r] == -INFINITY ? 0.0f : ex2(m_s[k][r] - top);
             const float4 x = *reinterpret_cast<const float4*>(o_s + (k * kRows + r) * L::kLdo + col);
             v.x = fmaf(x.x, w, v.x); v.y = fmaf(x.y, w, v.y); v.z = fmaf(x.z, w, v.z); v.w = fmaf(x.w, w, v.w);
@@ -303,41 +344,56 @@ __global__ void __launch_bounds__(32 * kWarps) quantized_stream_kernel(const Qua
 // blocks of query rows: 16 at a time halves the trips over the cache, but a head of more than 128 has no registers for it
 int rows_of(int dim, int total) { return total > 8 && dim <= 128 ? 16 : 8; }
 
-template <int DP, int NT>
+template <int DP, int NT, int W, int V>
 cudaError_t launch(const QuantizedParams& p, int n_seq, cudaStream_t st) {
     static bool done[64] = {};
     const dim3 grid(n_seq * p.G, ceil_div(static_cast<long long>(p.n_tok) * p.group, 8 * NT), p.splits);
     if (grid.y > 65535 || grid.z > 65535) return cudaErrorInvalidValue;
-    constexpr size_t smem = stream_smem<DP, NT>();
-    const cudaError_t e = allow_smem(quantized_stream_kernel<DP, NT>, smem, done);
+    constexpr size_t smem = Layout<DP, NT, W>::kBytes;
+    const cudaError_t e = allow_smem(quantized_stream_kernel<DP, NT, W, V>, smem, done);
     if (e != cudaSuccess) return e;
-    return launch_dependent(quantized_stream_kernel<DP, NT>, grid, dim3(32 * kWarps), smem, st, p);
+    return launch_dependent(quantized_stream_kernel<DP, NT, W, V>, grid, dim3(32 * W), smem, st, p);
+}
+template <int DP, int NT>
+cudaError_t launch_plan(const QuantizedParams& p, const StreamPlan& plan, int vec, int n_seq, cudaStream_t st) {
+    if constexpr (DP <= 128) {
+        if (plan.warps == 16) return !plan.whole ? launch<DP, NT, 16, 0>(p, n_seq, st) : vec ? launch<DP, NT, 16, 4>(p, n_seq, st) : launch<DP, NT, 16, 1>(p, n_seq, st);
+    }
+    return !plan.whole ? launch<DP, NT, 4, 0>(p, n_seq, st) : vec ? launch<DP, NT, 4, 4>(p, n_seq, st) : launch<DP, NT, 4, 1>(p, n_seq, st);
 }
 
 }  // namespace
 
-bool quantized_stream_supported(const tbl_quantized_mixer& m) { return m.dim <= TBL_MAX_ROTATED_DIM; }
-
-int quantized_stream_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
+StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
-    const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows_of(m.dim, static_cast<int>(total < 64 ? total : 64)));
-    const int tokens = ceil_div(context, kWarps * kTile);        // a split is worth at least a tile of each warp
-    long long s = 4LL * kNumSm / units;                          // four CTAs to an SM
+    const int rows = rows_of(m.dim, static_cast<int>(total < 64 ? total : 64));
+    const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows);
+    StreamPlan w{4, 1, 0};
+    const int tokens = ceil_div(context, 4 * kTile);             // a split is worth at least a tile of each warp
+    long long s = 4LL * kNumSm / units;                          // four CTAs of four warps to an SM
     if (s > tokens) s = tokens;
-    return s < 1 ? 1 : static_cast<int>(s < kMergeMaxSplits ? s : kMergeMaxSplits);
+    if (s > kMergeMaxSplits) s = kMergeMaxSplits;
+    w.splits = s < 1 ? 1 : static_cast<int>(s);
+    // Instead of splits, which another kernel has to join (some three tiles' time): one CTA of sixteen warps an SM.  Tiles that a warp takes one after the other:
+    if (w.splits > 1 && m.dim <= 128) {
+        const double wide = ceil_div(context, 16 * kTile) * static_cast<double>(ceil_div(units, kNumSm)), split = ceil_div(context, 4LL * kTile * w.splits) + 3.0;
+        if (wide <= split) { w.warps = 16; w.splits = 1; }
+    }
+    // As a whole one launch less, but fewer CTAs to an SM, whose own chains before the first tile show once they take turns (64 sequences of 8 heads over 4096 tokens
+    // 95 and 83 us)
+    w.whole = n_tok == 1 && w.splits == 1 && total <= rows && units <= (w.warps == 16 ? 1 : 2) * kNumSm;
+    return w;
 }
 
-bool quantized_stream_whole(const tbl_quantized_mixer&, int splits) { return splits == 1; }
-
-int launch_quantized_stream(const QuantizedParams& p, int n_seq, cudaStream_t st) {
+int launch_quantized_stream(const QuantizedParams& p, const StreamPlan& plan, int vec, int n_seq, cudaStream_t st) {
     const long long total = static_cast<long long>(p.n_tok) * p.group;
-    const bool wide = rows_of(p.d, static_cast<int>(total < 64 ? total : 64)) == 16;
+    const bool two = rows_of(p.d, static_cast<int>(total < 64 ? total : 64)) == 16;
     cudaError_t e;
     switch (p.width) {
-        case 64: e = wide ? launch<64, 2>(p, n_seq, st) : launch<64, 1>(p, n_seq, st); break;
-        case 128: e = wide ? launch<128, 2>(p, n_seq, st) : launch<128, 1>(p, n_seq, st); break;
-        case 192: e = launch<192, 1>(p, n_seq, st); break;
-        default: e = launch<256, 1>(p, n_seq, st); break;
+        case 64: e = two ? launch_plan<64, 2>(p, plan, vec, n_seq, st) : launch_plan<64, 1>(p, plan, vec, n_seq, st); break;
+        case 128: e = two ? launch_plan<128, 2>(p, plan, vec, n_seq, st) : launch_plan<128, 1>(p, plan, vec, n_seq, st); break;
+        case 192: e = launch_plan<192, 1>(p, plan, vec, n_seq, st); break;
+        default: e = launch_plan<256, 1>(p, plan, vec, n_seq, st); break;
     }
     return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
