@@ -264,7 +264,7 @@ int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int precision, 
  * positions_dev[slot] .., attention, output gate -> out (precision's type) [rows, heads*dim].  cache_dev [slots][kv_heads][capacity]
  * [row bytes], 16-byte aligned; rows behind a sequence's last token are neither used nor written, whatever they hold.  A token past the capacity or the
  * rotary tables sets TBL_DEV_CACHE_FULL; the rows of its sequence are undefined, the cache holds what has room.  positions_dev is not
- * advanced, so that a repeated call writes the same rows again.  route: 0 as the step, 1 SIMT over expanded keys and values, 2 the
+ * advanced, so that a repeated call writes the same rows again.  route: 0 as the step, 1 fp32 arithmetic on the 4-bit rows, 2 the
  * cache-streaming kernel (warp-level MMAs on the 4-bit rows), 3 the flash kernel (tcgen05) over expanded keys and values, as far as its
  * tiles have room (dim <= 192); 2 and 3 take bf16 only.  A number that is not finite reaches the rows that see its token, and may reach those of the same call and sequence before it. */
 int tbl_quantized_row_bytes(const tbl_quantized_mixer* mixer);

@@ -25,7 +25,7 @@ LIBRARIES = {
     "stack": (os.path.join(HERE, "libstack_b200.so"),
               ["runtime.cu", "stack.cu", "stack_glue.cu", "dense.cu", "dense_rows.cu", "dense_tcgen05.cu", "dense_split.cu", "delta_rule.cu",
                "latent_attention.cu", "latent_decode.cu", "latent_prefill.cu", "attention.cu", "attention_decode.cu",
-               "attention_prefill.cu", "head_rotation.cu", "quantized_attention.cu", "quantized_decode.cu", "decay_attention.cu", "decay_chunk.cu"]),
+               "attention_prefill.cu", "head_rotation.cu", "quantized_attention.cu", "quantized_decode.cu", "quantized_rows.cu", "decay_attention.cu", "decay_chunk.cu"]),
 }
 LIB, SOURCES = LIBRARIES["ternary"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const Attn
     for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
     const int row = tid >> 4, col = tid & 15;
     const int last = pos0 + min(first + row, total - 1) / p.group;           // last visible token of this thread's row
-    const T* cache = static_cast<const T*>(p.cache) + cache_row(p, p.by_seq ? seq : slot, g, 0);
+    const T* cache = static_cast<const T*>(p.cache) + cache_row(p, slot, g, 0);
     for (int t = t0; t < t1; t += kSimtTokens) {
         __syncthreads();
         for (int i = tid; i < kSimtTokens * p.d; i += kSimtThreads) {
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const Attn
 // ---- merge ----------------------------------------------------------------------------------------------------------------
 // One CTA per (row, head).  128 threads share a map's value columns; of a layer with one map the second half of the CTA
 // takes every other split.
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = 256, kMergeMaxSplits = 1024;
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) attention_merge_kernel(const AttnParams p) {
@@ -328,9 +328,6 @@ int run(const tbl_attention_mixer& m, AttnParams p, const Plan& w, int n_seq, cu
 
 }  // namespace
 
-int launch_attention_simt(const AttnParams& p, int precision, int n_seq, cudaStream_t st) {
-    return precision == TBL_BF16 ? launch_simt<bf16>(p, n_seq, st) : launch_simt<float>(p, n_seq, st);
-}
 int launch_attention_merge(const AttnParams& p, int precision, int rows, cudaStream_t st) {
     return precision == TBL_BF16 ? launch_merge<bf16>(p, rows, st) : launch_merge<float>(p, rows, st);
 }

@@ -24,7 +24,7 @@ struct AttnParams {
     int H, G, group, maps, d, vd, dp, vp, cw;
     int n_slots, capacity, temperature_positions, n_tok, splits, append, vec;
     float scale_log2, lambda, out_scale, eps;
-    // the merge and flash kernels' gate (null: none), and a factor of one map's output; by_seq: the cache belongs to the step's sequences, not to slots
+    // the merge and flash kernels' gate (null: none), and a factor of one map's output; by_seq (flash): the cache belongs to the step's sequences, not to slots
     const float* gate;
     int ldg, by_seq;
     float value_scale;
@@ -54,9 +54,7 @@ constexpr int kClusterSplits = 8;
 bool attention_stream_supported(const tbl_attention_mixer& m);
 int launch_attention_stream(const AttnParams& p, int n_seq, cudaStream_t st);
 
-// attention.cu: any sizes, split over the context into partial sums, which the merge brings together (p.splits of them)
-constexpr int kMergeMaxSplits = 1024;
-int launch_attention_simt(const AttnParams& p, int precision, int n_seq, cudaStream_t st);
+// attention.cu: brings p.splits partial sums together
 int launch_attention_merge(const AttnParams& p, int precision, int rows, cudaStream_t st);
 
 // attention_prefill.cu: flash attention on tcgen05

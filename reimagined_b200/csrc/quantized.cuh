@@ -1,4 +1,4 @@
-// Shared by the translation units of the attention over a 4-bit cache (quantized_attention.cu, quantized_decode.cu).
+// Shared by the translation units of the attention over a 4-bit cache (quantized_attention.cu, quantized_decode.cu, quantized_rows.cu).
 //
 // Cache of a layer: [slot][kv head][token][row], a row being, with n = the head size rounded up to 64, n/2 bytes of key codes, n/2 of value codes, n/16
 // scale bytes of the key, n/16 of the value, and zeros to a multiple of 16.  One token of a head is one contiguous row, so that a tile of tokens is one bulk copy.
@@ -122,6 +122,10 @@ struct StreamPlan {
 };
 StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
 int launch_quantized_stream(const QuantizedParams& p, const StreamPlan& plan, int vec, int n_seq, cudaStream_t st);
+
+// quantized_rows.cu: the same in fp32 arithmetic, any number of rows
+int quantized_rows_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
+int launch_quantized_rows(const QuantizedParams& p, int precision, int n_seq, cudaStream_t st);
 
 }  // namespace stack
 }  // namespace tbl

@@ -1,10 +1,10 @@
 // Softmax attention over a cache that holds keys and values in 4 bits (e2m1 codes, an e4m3 scale for every 16 numbers).
 //
 //   quantized_prep_kernel    norm and rotation of queries and keys, rounding of keys and values to 4 bits, append
-//   quantized_expand_kernel  the visible cache as numbers: code x scale has six bits, which fp16 and bf16 hold
+//   quantized_expand_kernel  the visible cache as numbers: code x scale has six bits between 2^-10 and 2688, which fp16 holds
 //   quantized_read_kernel    the same for single tokens, in the layer's units
-// Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, and weights need one term instead of two), fp32 and other sizes through the SIMT kernel of attention.cu, a few
-// query rows over the 4-bit rows themselves (quantized_decode.cu).  The layer's units enter as factors of the scores and of the output.
+// Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, and weights need one term instead of two), a few query rows
+// over the 4-bit rows themselves (quantized_decode.cu), fp32 and what else there is in fp32 arithmetic (quantized_rows.cu).  The layer's units enter as factors of the scores and of the output.
 #include <string.h>
 
 #include "attention.cuh"
@@ -62,22 +62,14 @@ __device__ __forceinline__ void numbers8(uint32_t codes, float scale, float (&v)
         v[2 * i + 1] = c.y * scale;
     }
 }
-__device__ __forceinline__ void put8(bf16* dst, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-}
 __device__ __forceinline__ void put8(__half* dst, const float (&v)[8]) {
     __align__(16) __half2 h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
 }
-__device__ __forceinline__ void put8(float* dst, const float (&v)[8]) {
-    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
 
 // [sequence][kv head][ctx][key, padded to 16 | value]; a thread per eight numbers, zeros behind the last visible token.
-template <typename T>
 __global__ void __launch_bounds__(256) quantized_expand_kernel(const QuantizedParams p, const int padded) {
     pdl_launch_dependents();
     pdl_wait();
@@ -93,7 +85,7 @@ __global__ void __launch_bounds__(256) quantized_expand_kernel(const QuantizedPa
         const uint32_t codes = reinterpret_cast<const uint32_t*>(row + is_v * (p.width / 2))[e];
         numbers8(codes, scale_of(row[p.width + is_v * (p.width / 16) + e / 2]), v);
     }
-    put8(static_cast<T*>(p.expanded) + ((static_cast<size_t>(blockIdx.y) * p.ctx + token) * per + c) * 8, v);
+    put8(static_cast<__half*>(p.expanded) + ((static_cast<size_t>(blockIdx.y) * p.ctx + token) * per + c) * 8, v);
 }
 
 template <typename T>
@@ -195,24 +187,21 @@ Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq
     const size_t rows = static_cast<size_t>(n_seq) * n_tok, dp = padded16(m.dim);
     w.route = route == kAuto ? pick_route(m, precision, n_tok) : route;
     w.splits = 1;
-    bool parts = w.route == kSimt || (w.route == kFlash && !attention_flash_whole(as_attention(m)));
+    bool parts = w.route == kFlash && !attention_flash_whole(as_attention(m));
     if (w.route == kStream) {
         w.stream = quantized_stream_plan(m, n_seq, n_tok, context);
         w.splits = w.stream.splits;
         parts = w.splits > 1;
     } else if (w.route == kSimt) {
-        const long long units = static_cast<long long>(ceil_div(static_cast<long long>(n_tok) * (m.heads / m.kv_heads), 16)) * n_seq * m.kv_heads;
-        long long s = 2LL * kNumSm / units;
-        const int tokens = ceil_div(context, 64);                // a split is worth at least 64 tokens
-        if (s > tokens) s = tokens;
-        w.splits = s < 1 ? 1 : static_cast<int>(s < kMergeMaxSplits ? s : kMergeMaxSplits);
+        w.splits = quantized_rows_splits(m, n_seq, n_tok, context);
+        parts = w.splits > 1;
     }
     w.ctx = static_cast<int>(round_up(context, 128));            // whole blocks of the flash kernel
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };
     w.q = take(w.route == kStream ? 2 * rows * m.heads * quantized_width(m.dim) : w.route == kFlash ? 2 * rows * m.heads * dp : 4 * rows * m.heads * m.dim);
     w.factor = take(w.route != kSimt ? sizeof(float) * rows * m.heads : 0);
-    w.expanded = take(w.route == kStream ? 0 : (precision == TBL_BF16 ? 2 : 4) * static_cast<size_t>(n_seq) * m.kv_heads * w.ctx * 2 * dp);
+    w.expanded = take(w.route == kFlash ? 2 * static_cast<size_t>(n_seq) * m.kv_heads * w.ctx * 2 * dp : 0);
     const size_t units = rows * m.heads * w.splits;
     w.pm = take(parts ? sizeof(float) * units : 0);
     w.pl = take(parts ? sizeof(float) * units : 0);
@@ -236,44 +225,29 @@ int launch_merge(const QuantizedParams& p, int precision, int rows, cudaStream_t
                                   : launch_dependent(quantized_merge_kernel<float>, grid, block, 0, st, p)) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
 
-// partial sums and outputs as attention.cu's merge takes them
-AttnParams merge_params(const QuantizedParams& p, const tbl_quantized_mixer& m) {
-    AttnParams a{};
-    a.slots = p.slots; a.positions = p.positions; a.part_m = p.part_m; a.part_l = p.part_l; a.part_o = p.part_o; a.out = p.out; a.status = p.status;
-    a.H = p.H; a.G = p.G; a.group = p.group; a.maps = 1; a.d = a.vd = p.d; a.dp = a.vp = padded16(p.d); a.n_tok = p.n_tok; a.splits = p.splits;
-    a.gate = p.g_off < 0 ? nullptr : p.proj + p.g_off; a.ldg = p.ld; a.value_scale = m.value_scale;
-    return a;
-}
-
 int run(const tbl_quantized_mixer& m, int precision, const QuantizedParams& p, const Plan& w, int n_seq, cudaStream_t st) {
     const int rows = n_seq * p.n_tok;
     const bool vec = vector_heads(m.rotation, p.d, p.proj, p.ld);
     const bool whole = w.route == kStream && w.stream.whole;
     const cudaError_t e = whole ? cudaSuccess : w.route == kSimt ? launch_prep<float>(p, rows, vec, st) : launch_prep<__half>(p, rows, vec, st);
     if (e != cudaSuccess) return TBL_ERR_CUDA;
-    AttnParams a = merge_params(p, m);
-    if (w.route == kStream) {
-        const int rc = launch_quantized_stream(p, w.stream, vec, n_seq, st);
+    if (w.route != kFlash) {
+        const int rc = w.route == kStream ? launch_quantized_stream(p, w.stream, vec, n_seq, st) : launch_quantized_rows(p, precision, n_seq, st);
         return rc != TBL_OK || w.splits == 1 ? rc : launch_merge(p, precision, rows, st);
     }
+    AttnParams a{};
+    a.slots = p.slots; a.positions = p.positions; a.part_m = p.part_m; a.part_l = p.part_l; a.part_o = p.part_o; a.out = p.out; a.status = p.status;
+    a.H = p.H; a.G = p.G; a.group = p.group; a.maps = 1; a.d = a.vd = p.d; a.dp = a.vp = padded16(p.d); a.n_tok = p.n_tok; a.splits = 1;
+    a.gate = p.g_off < 0 ? nullptr : p.proj + p.g_off; a.ldg = p.ld; a.value_scale = m.value_scale;
     const dim3 grid(ceil_div(static_cast<long long>(p.ctx) * (a.dp / 4), 256), n_seq * p.G);
-    const cudaError_t x = w.route == kFlash ? launch_dependent(quantized_expand_kernel<__half>, grid, dim3(256), 0, st, p, a.dp)
-                          : precision == TBL_BF16 ? launch_dependent(quantized_expand_kernel<bf16>, grid, dim3(256), 0, st, p, a.dp)
-                                                  : launch_dependent(quantized_expand_kernel<float>, grid, dim3(256), 0, st, p, a.dp);
-    if (x != cudaSuccess) return TBL_ERR_CUDA;
-    a.cache = p.expanded; a.cw = 2 * a.dp; a.n_slots = n_seq; a.capacity = p.ctx; a.by_seq = 1;
-    a.scale_log2 = p.scale_log2;
-    // the gate's columns decide whether the flash kernel's vector loads are aligned, as the projections' do where it reads them itself
+    if (launch_dependent(quantized_expand_kernel, grid, dim3(256), 0, st, p, a.dp) != cudaSuccess) return TBL_ERR_CUDA;
+    a.cache = p.expanded; a.cw = 2 * a.dp; a.n_slots = n_seq; a.capacity = p.ctx; a.by_seq = 1; a.scale_log2 = p.scale_log2;
+    a.q16 = static_cast<bf16*>(p.q);                             // sixteen bits either way
+    a.q_factor = p.q_factor;
+    // the gate's columns decide whether the flash kernel's vector loads are aligned
     a.vec = (p.ld | p.d) % 4 == 0 && aligned16(p.proj);
-    if (w.route == kFlash) {
-        a.q16 = static_cast<bf16*>(p.q);                         // sixteen bits either way
-        a.q_factor = p.q_factor;
-        const int rc = launch_attention_flash(a, n_seq, st);
-        return rc != TBL_OK || attention_flash_whole(as_attention(m)) ? rc : launch_attention_merge(a, precision, rows, st);
-    }
-    a.proj = static_cast<const float*>(p.q); a.ld = p.H * p.d;
-    const int rc = launch_attention_simt(a, precision, n_seq, st);
-    return rc != TBL_OK ? rc : launch_merge(p, precision, rows, st);
+    const int rc = launch_attention_flash(a, n_seq, st);
+    return rc != TBL_OK || attention_flash_whole(as_attention(m)) ? rc : launch_attention_merge(a, precision, rows, st);
 }
 
 QuantizedParams basic_params(const tbl_quantized_mixer& m, int capacity, const int32_t* slots, const int32_t* positions, int n_tok) {

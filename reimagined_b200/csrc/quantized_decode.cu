@@ -372,7 +372,7 @@ StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_
     const int tokens = ceil_div(context, 4 * kTile);             // a split is worth at least a tile of each warp
     long long s = 4LL * kNumSm / units;                          // four CTAs of four warps to an SM
     if (s > tokens) s = tokens;
-    if (s > kMergeMaxSplits) s = kMergeMaxSplits;
+    if (s > 1024) s = 1024;
     w.splits = s < 1 ? 1 : static_cast<int>(s);
     // Instead of splits, which another kernel has to join (some three tiles' time): one CTA of sixteen warps an SM.  Tiles that a warp takes one after the other:
     if (w.splits > 1 && m.dim <= 128) {
