@@ -443,7 +443,7 @@ int launch_decay(const tbl_decay_mixer& m, int precision, int route, float eps, 
     if (w.whole) return (precision == TBL_BF16 ? launch_step<bf16>(p, st) : launch_step<float>(p, st)) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
     float *q = reinterpret_cast<float*>(base + w.q), *k = reinterpret_cast<float*>(base + w.k);
     p.q = q; p.k = k; p.raw = reinterpret_cast<float*>(base + w.raw);
-    const RotationCall c{proj, p.ld, m.heads, m.heads, m.dim, slots, positions, n_seq, n_tok, eps, q, k};
+    const RotationCall c{proj, p.ld, m.heads, m.heads, m.dim, slots, positions, n_seq, n_tok, eps, q, k, nullptr, 0};
     const int rc = launch_head_rotation(m.rotation, TBL_F32, c, st);
     if (rc != TBL_OK) return rc;
     if (launch_scan(p, st) != cudaSuccess) return TBL_ERR_CUDA;

@@ -116,11 +116,7 @@ __device__ __forceinline__ float lanes_max(float v) {
     for (int o = LPH / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-// the power of two at or below v (1 for 0), and one over it
-__device__ __forceinline__ float power_of(float v) {
-    const uint32_t power = min(__float_as_uint(v) >> 23, 253u);
-    return power ? __uint_as_float(power << 23) : 1.0f;
-}
+// one over a power of two
 __device__ __forceinline__ float inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ float largest(const float (&x)[8]) {
     float m = fabsf(x[0]);
@@ -181,7 +177,7 @@ __device__ __forceinline__ int table_row(const DecayParams& p, int pos) { return
 // the power of two that a normed head's numbers are divided by: sqrt(d) times the largest weight bounds them
 template <int LPH>
 __device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
-    return power_of(sqrtf(static_cast<float>(dim)) * lanes_max<LPH>(largest(w)));
+    return power_below(sqrtf(static_cast<float>(dim)) * lanes_max<LPH>(largest(w)));
 }
 
 // ---- sums of the chunks -----------------------------------------------------------------------------------------------------------------
@@ -256,8 +252,8 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
                 for (int e = 0; e < 8; ++e) k[i][e] *= w[e];
             }
             kl.turn(p.r.interleaved != 0, cs, sn, k[i]);
-            if (!normed) power = power_of(lanes_max<Lane::kLph>(largest(k[i])));
-            const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_of(v_most);
+            if (!normed) power = power_below(lanes_max<Lane::kLph>(largest(k[i])));
+            const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_below(v_most);
             inv[i] = j < a.n ? inv[i] * inverse_power(power) * kUp : 0.0f;
             up[i] = weight_s[j] * power;
             most = fmaxf(most, v_most * up[i]);
@@ -278,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) most = fmaxf(most, most_s[tile][i]);
-        const float top = fmaxf(power_of(most), 7.8886091e-31f), down = inverse_power(top) * kUp;
+        const float top = fmaxf(power_below(most), 7.8886091e-31f), down = inverse_power(top) * kUp;
         back[tile] = top * (1.0f / (kUp * kUp));
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
@@ -376,7 +372,7 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[e]));
             most = lanes_max<kLph>(most);
-            const float power = power_of(most), inv = inverse_power(power);
+            const float power = power_below(most), inv = inverse_power(power);
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -475,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
                     for (int e = 0; e < 8; ++e) x[i][e] *= w[e];
                 }
                 ql.turn(p.r.interleaved != 0, cs, sn, x[i]);
-                if (!normed) power = power_of(lanes_max<Lane::kLph>(largest(x[i])));
+                if (!normed) power = power_below(lanes_max<Lane::kLph>(largest(x[i])));
                 const float f = inv * inverse_power(power);
 #pragma unroll
                 for (int u = 0; u < Lane::kRuns; ++u) {

@@ -1,6 +1,6 @@
 // Norm and rotation of query and key heads in one pass over stacked projections: y = x / sqrt(mean x^2 + eps) * w, then pairs of dimensions turn by
-// the angle of the row's position.  Bound by memory: every number is read once (4 bytes) and written once.  A CTA takes one row, so that its heads share the row's
-// entries of the tables in the first-level cache; a head lies in registers of 8, 16 or 32 lanes between the sum of squares and the stores.
+// the angle of the row's position.  Bound by memory: every number is read once (4 bytes) and written once.  A CTA takes a row at a time, so that a thread reads
+// the row's angles once for all its heads; a head lies in registers of 8, 16 or 32 lanes between the sum of squares and the stores.
 #include <string.h>
 
 #include "head_rotation.cuh"
@@ -13,52 +13,131 @@ struct RotationParams {
     const float *proj, *q_norm, *k_norm;
     const int32_t *slots, *positions;
     void *q, *k;
+    float* q_factor;
     int* status;
     Rotation r;
-    int ld, q_heads, heads, dim, n_tok;
-    float eps;
+    int ld, q_heads, heads, dim, n_tok, rows, ldq;
+    float eps, per_dim;
 };
 
-template <typename T, int V, int LPH>
-__global__ void __launch_bounds__(1024) head_rotation_kernel(const RotationParams p) {
+constexpr int kMostThreads = 256;
+
+// LPH lanes a head, U units a lane.  A thread has the same columns of every head it takes: their places and weights stay in registers, a row's angles for all its
+// heads.  HALVES: queries as fp16 under a power of two (RotationCall).
+template <typename T, int V, int LPH, int U, bool HALVES, bool EXACT>
+__global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_kernel(const RotationParams p) {
+    using Units = HeadUnits<V, LPH>;
+    constexpr int kRuns = 2 * U, kNumbers = V * kRuns;
+    const int dim = EXACT ? kNumbers * LPH : p.dim, limit = EXACT ? 1 << 30 : p.dim;         // limit: of the columns that are there
+    const int group = threadIdx.x / LPH, groups = blockDim.x / LPH, gl = threadIdx.x % LPH;
+    // a head's lanes: others of the warp may have heads without a norm
+    const uint32_t mates = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1u) << (threadIdx.x % 32 / LPH * LPH);
+    int at[kRuns];
+#pragma unroll
+    for (int u = 0; u < U; ++u) Units::runs(p.r, gl + LPH * u, at[2 * u], at[2 * u + 1]);
+    float bound = 1.0f;
+    if (HALVES && p.q_norm) {                                    // sqrt(dim) times the largest weight bounds a normed head
+        float most = 0.0f, w[kNumbers];
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u) Units::load_run(p.q_norm, at[u], limit, w + V * u);
+#pragma unroll
+        for (int e = 0; e < kNumbers; ++e) most = fmaxf(most, fabsf(w[e]));
+#pragma unroll
+        for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        bound = power_below(sqrtf(static_cast<float>(dim)) * most);
+    }
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x, group = threadIdx.x / LPH, groups = blockDim.x / LPH, lane = threadIdx.x % LPH;
+    const int row = blockIdx.x;
     const int pos = p.positions[p.slots[row / p.n_tok]] + row % p.n_tok;
-    if (p.r.half > 0 && (pos < 0 || pos >= p.r.positions)) {
-        if (threadIdx.x == 0) atomicOr(p.status, TBL_DEV_CACHE_FULL);
-        return;
+    const bool outside = p.r.half > 0 && (pos < 0 || pos >= p.r.positions);
+    if (outside && threadIdx.x == 0) atomicOr(p.status, TBL_DEV_CACHE_FULL);
+    if (outside && !HALVES) return;                          // (a step's rows are undefined then, an operator's stay as they were)
+    const int entry = p.r.half > 0 ? min(max(pos, 0), p.r.positions - 1) : 0;
+    float c[V * U], sn[V * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int n = V * (gl + LPH * u);
+#pragma unroll
+        for (int e = 0; e < V; ++e) { c[V * u + e] = 1.0f; sn[V * u + e] = 0.0f; }
+        if (n < p.r.half) {
+            Units::load_run(p.r.cos + static_cast<size_t>(entry) * p.r.half, n, 1 << 30, c + V * u);
+            Units::load_run(p.r.sin + static_cast<size_t>(entry) * p.r.half, n, 1 << 30, sn + V * u);
+        }
     }
     const float* src = p.proj + static_cast<size_t>(row) * p.ld;
-    // whole warps go round together: the sum of squares is exchanged between their lanes
-    for (int h0 = 0; h0 < p.heads; h0 += groups) {
-        const int h = h0 + group, hc = min(h, p.heads - 1);
-        HeadUnits<V, LPH> x;
-        x.load(p.r, src + hc * p.dim, p.dim, lane);
-        const bool is_q = hc < p.q_heads;
-        x.template turn<float>(p.r, is_q ? p.q_norm : p.k_norm, p.eps, pos, p.dim, lane);
+    // whole warps go round together: sums are exchanged between their lanes
+    for (int h = group; h - group < p.heads; h += groups) {
+        float x[kNumbers], f = 1.0f;
+        const bool is_k = h >= p.q_heads;
+        const float *head = src + min(h, p.heads - 1) * dim, *norm = is_k ? p.k_norm : p.q_norm;
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u) Units::load_run(head, at[u], limit, x + V * u);
+        if (norm) {
+            float ss = 0.0f, w[kNumbers];
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u) Units::load_run(norm, at[u], limit, w + V * u);
+#pragma unroll
+            for (int e = 0; e < kNumbers; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+            for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(mates, ss, o);
+            f = rsqrtf(fmaf(ss, p.per_dim, p.eps));
+#pragma unroll
+            for (int e = 0; e < kNumbers; ++e) x[e] *= w[e] * f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float *y = x + 2 * V * u, cj = c[V * u + j], sj = sn[V * u + j];
+                if (p.r.interleaved) {
+                    const float a = y[2 * j], b = y[2 * j + 1];
+                    y[2 * j] = a * cj - b * sj;
+                    y[2 * j + 1] = b * cj + a * sj;
+                } else {
+                    const float a = y[j], b = y[V + j];
+                    y[j] = a * cj - b * sj;
+                    y[V + j] = b * cj + a * sj;
+                }
+            }
+        float back = 1.0f;
+        if (HALVES) {
+            float power = bound;
+            if (!p.q_norm) {
+                float most = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kNumbers; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+                for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                power = power_below(most);
+            }
+            back = __uint_as_float((254u << 23) - __float_as_uint(power));
+            if (gl == 0 && h < p.heads) p.q_factor[static_cast<size_t>(row) * p.heads + h] = power;
+        }
         if (h >= p.heads) continue;
-        T* dst = is_q ? static_cast<T*>(p.q) + (static_cast<size_t>(row) * p.q_heads + h) * p.dim
-                      : static_cast<T*>(p.k) + (static_cast<size_t>(row) * (p.heads - p.q_heads) + h - p.q_heads) * p.dim;
-        x.store(p.r, dst, p.dim, lane);
+        T* dst = HALVES ? static_cast<T*>(p.q) + (static_cast<size_t>(row) * p.heads + h) * p.ldq
+                 : is_k ? static_cast<T*>(p.k) + (static_cast<size_t>(row) * (p.heads - p.q_heads) + h - p.q_heads) * dim
+                        : static_cast<T*>(p.q) + (static_cast<size_t>(row) * p.q_heads + h) * dim;
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u) Units::store_run(dst, at[u], HALVES ? p.ldq : limit, x + V * u, back);
     }
 }
 
-template <typename T, int V, int LPH>
-cudaError_t launch(const RotationParams& p, int rows, cudaStream_t st) {
-    // few rows: all heads at once; many: CTAs of up to 512 threads whose rounds are full
-    const int lanes = p.heads * LPH, most = rows < 2 * kNumSm ? 1024 : 512;
-    const int rounds = ceil_div(lanes, most), groups = ceil_div(p.heads, rounds);
+template <typename T, int V, int LPH, int U, bool HALVES, bool EXACT>
+cudaError_t launch(const RotationParams& p, cudaStream_t st) {
+    // (a CTA for several rows, its lanes' weights kept in registers: 57 to 65 us for 8192 rows of 40 heads of 128, since fewer loads are on their way)
+    const int rounds = ceil_div(p.heads * LPH, kMostThreads), groups = ceil_div(p.heads, rounds);
     const int threads = static_cast<int>(round_up(static_cast<size_t>(groups) * LPH, 32));
-    return launch_dependent(head_rotation_kernel<T, V, LPH>, dim3(rows), dim3(threads), 0, st, p);
+    return launch_dependent(head_rotation_kernel<T, V, LPH, U, HALVES, EXACT>, dim3(p.rows), dim3(threads), 0, st, p);
 }
 
-template <typename T>
-cudaError_t launch_type(const RotationParams& p, int rows, bool vec, cudaStream_t st) {
-    if (!vec) return launch<T, 1, 32>(p, rows, st);
-    if (p.dim <= 64) return launch<T, 4, 8>(p, rows, st);
-    if (p.dim <= 128) return launch<T, 4, 16>(p, rows, st);
-    return launch<T, 4, 32>(p, rows, st);
+template <typename T, bool HALVES>
+cudaError_t launch_type(const RotationParams& p, int run, cudaStream_t st) {
+    if (run == 1) return launch<T, 1, 32, 4, HALVES, false>(p, st);
+    if (run == 2) return p.dim <= 128 ? launch<T, 2, 32, 1, HALVES, false>(p, st) : launch<T, 2, 32, 2, HALVES, false>(p, st);
+    if (p.dim <= 64) return p.dim == 64 ? launch<T, 4, 8, 1, HALVES, true>(p, st) : launch<T, 4, 8, 1, HALVES, false>(p, st);
+    if (p.dim <= 128) return p.dim == 128 ? launch<T, 4, 16, 1, HALVES, true>(p, st) : launch<T, 4, 16, 1, HALVES, false>(p, st);
+    return launch<T, 4, 32, 1, HALVES, false>(p, st);
 }
 
 }  // namespace
@@ -67,11 +146,13 @@ int launch_head_rotation(const tbl_head_rotation& r, int precision, const Rotati
     RotationParams p{};
     p.status = device_status_ptr();
     if (!p.status) return TBL_ERR_CUDA;
-    p.proj = c.proj; p.q_norm = r.q_norm; p.k_norm = r.k_norm; p.slots = c.slots; p.positions = c.positions; p.q = c.q; p.k = c.k;
+    p.proj = c.proj; p.q_norm = r.q_norm; p.k_norm = r.k_norm; p.slots = c.slots; p.positions = c.positions; p.q = c.q; p.k = c.k; p.q_factor = c.q_factor;
     p.r = rotation_of(r); p.ld = c.ld; p.q_heads = c.q_heads; p.heads = c.q_heads + c.k_heads; p.dim = c.dim; p.n_tok = c.n_tok; p.eps = c.eps;
-    const bool vec = vector_heads(r, c.dim, c.proj, c.ld) && aligned16(c.q) && aligned16(c.k);
-    const int rows = c.n_seq * c.n_tok;
-    return (precision == TBL_BF16 ? launch_type<bf16>(p, rows, vec, st) : launch_type<float>(p, rows, vec, st)) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
+    p.rows = c.n_seq * c.n_tok; p.ldq = c.ldq; p.per_dim = 1.0f / static_cast<float>(c.dim);
+    // runs of four or two numbers where everything lies on their bytes
+    const int run = vector_heads(r, c.dim, c.proj, c.ld) && aligned16(c.q) && aligned16(c.k) ? 4 : paired_heads(r, c.dim, c.proj, c.ld, c.q, c.k) ? 2 : 1;
+    const cudaError_t e = c.q_factor ? launch_type<__half, true>(p, run, st) : precision == TBL_BF16 ? launch_type<bf16, false>(p, run, st) : launch_type<float, false>(p, run, st);
+    return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
 
 }  // namespace stack
@@ -92,6 +173,6 @@ extern "C" int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int 
     if (heads == 0) return TBL_ERR_INVALID_ARG;
     if (heads * dim > ld || static_cast<long long>(n_seq) * n_tok > 2147483647LL) return TBL_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(proj_dev) & 3) return TBL_ERR_ALIGNMENT;
-    RotationCall c{proj_dev, ld, q_heads, k_heads, dim, slots_dev, positions_dev, n_seq, n_tok, eps, q_heads > 0 ? q_dev : nullptr, k_heads > 0 ? k_dev : nullptr};
+    const RotationCall c{proj_dev, ld, q_heads, k_heads, dim, slots_dev, positions_dev, n_seq, n_tok, eps, q_heads > 0 ? q_dev : nullptr, k_heads > 0 ? k_dev : nullptr, nullptr, 0};
     return launch_head_rotation(*rotation, precision, c, static_cast<cudaStream_t>(stream));
 }

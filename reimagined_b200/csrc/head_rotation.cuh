@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_fp16.h>
+#include <string.h>
 
 #include "stack.cuh"
 
@@ -37,6 +38,9 @@ struct HeadUnits {
         if (V == 4) {
             const float4 f = at < dim ? *reinterpret_cast<const float4*>(src + at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             v[0] = f.x; v[V > 1 ? 1 : 0] = f.y; v[V > 2 ? 2 : 0] = f.z; v[V > 3 ? 3 : 0] = f.w;
+        } else if (V == 2) {
+            const float2 f = at < dim ? *reinterpret_cast<const float2*>(src + at) : make_float2(0.0f, 0.0f);
+            v[0] = f.x; v[V > 1 ? 1 : 0] = f.y;
         } else {
             v[0] = at < dim ? src[at] : 0.0f;
         }
@@ -112,6 +116,13 @@ struct HeadUnits {
             uint2 w;
             memcpy(&w, t, sizeof(w) < sizeof(t) ? sizeof(w) : sizeof(t));
             *reinterpret_cast<uint2*>(dst + at) = w;
+        } else if (V == 2 && sizeof(T) == 4) {
+            *reinterpret_cast<float2*>(dst + at) = make_float2(v[0] * f, v[V > 1 ? 1 : 0] * f);
+        } else if (V == 2) {
+            T t[2] = {from_f<T>(v[0] * f), from_f<T>(v[V > 1 ? 1 : 0] * f)};
+            uint32_t w;
+            memcpy(&w, t, sizeof(w) < sizeof(t) ? sizeof(w) : sizeof(t));
+            *reinterpret_cast<uint32_t*>(dst + at) = w;
         } else {
             dst[at] = from_f<T>(v[0] * f);
         }
@@ -137,6 +148,12 @@ inline bool vector_heads(const tbl_head_rotation& r, int dim, const void* proj, 
            aligned16(r.rope_sin);
 }
 
+// whether runs of two do (the last unit of four numbers may have only its first run)
+inline bool paired_heads(const tbl_head_rotation& r, int dim, const void* proj, int ld, const void* q, const void* k) {
+    auto on8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; };
+    return dim % 2 == 0 && r.rot_dim % 4 == 0 && ld % 2 == 0 && on8(proj) && on8(r.q_norm) && on8(r.k_norm) && on8(r.rope_cos) && on8(r.rope_sin) && on8(q) && on8(k);
+}
+
 inline int check_rotation(const tbl_head_rotation& r, int dim) {
     if (dim <= 0 || dim > TBL_MAX_ROTATED_DIM || r.rot_dim < 0 || r.rot_dim > dim || r.rot_dim % 2) return TBL_ERR_SHAPE;
     if (r.interleaved != 0 && r.interleaved != 1) return TBL_ERR_INVALID_ARG;
@@ -144,7 +161,14 @@ inline int check_rotation(const tbl_head_rotation& r, int dim) {
     return TBL_OK;
 }
 
-// head_rotation.cu: q_heads, then k_heads heads of `dim` from column 0 of proj on -> q, k [rows][heads][dim]
+// the power of two at or below v (1 for 0)
+__device__ __forceinline__ float power_below(float v) {
+    const uint32_t power = min(__float_as_uint(v) >> 23, 253u);
+    return power ? __uint_as_float(power << 23) : 1.0f;
+}
+
+// head_rotation.cu: q_heads, then k_heads heads of `dim` from column 0 of proj on -> q, k [rows][heads][dim].  With q_factor (k_heads 0): q is fp16
+// [rows][heads][ldq], zeros behind a head, each head divided by a power of two, q_factor [rows][heads], that leaves its numbers below 2.
 struct RotationCall {
     const float* proj;
     int ld, q_heads, k_heads, dim;
@@ -152,6 +176,8 @@ struct RotationCall {
     int n_seq, n_tok;
     float eps;
     void *q, *k;
+    float* q_factor;
+    int ldq;
 };
 int launch_head_rotation(const tbl_head_rotation& r, int precision, const RotationCall& c, cudaStream_t st);
 

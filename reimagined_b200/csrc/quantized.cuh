@@ -28,7 +28,7 @@ struct QuantizedParams {
     int* status;
     Rotation r;
     int ld, g_off;               // of proj; g_off: column of the output gate, < 0: none
-    int H, G, group, d, width, row, ldq, ldo, capacity, n_tok, splits, ctx;
+    int H, G, group, d, width, row, ldq, ldo, capacity, n_tok, splits, ctx, first_head;    // first_head: of the preparing kernel, H: queries are done already
     float scale_log2, key_unit, value_unit, eps;
 };
 
