@@ -24,7 +24,8 @@ namespace {
 
 using namespace tc05;
 
-constexpr int kTokens = 128, kThreads = 256, kWarps = kThreads / 32;
+constexpr int kTokens = 128;
+constexpr int kSumThreads = 256, kOutThreads = 512;      // of decay_sums_kernel (its registers would not do for more), of decay_chunk_kernel
 constexpr int kSub = 128 * 128;                  // 128 rows of 64 sixteen-bit numbers, 128-byte swizzle
 constexpr int kBox = 64 * 128;                   // 64 tokens of the same
 constexpr uint32_t kTransposeA = 1u << 15, kTransposeB = 1u << 16;
@@ -63,9 +64,9 @@ struct HeadLane {
 #pragma unroll
         for (int u = 0; u < kRuns; ++u) mix[u] = (((at[u] >> 3) & 7) ^ group) << 4;
     }
-    // byte of run u in row 8 k + i kSide + group of tiles of 64 columns, `tile` bytes each
-    __device__ __forceinline__ uint32_t place(int u, int k8, int i, int group, int tile) const {
-        return static_cast<uint32_t>((at[u] >> 6) * tile + (at[u] & 7) * 2 + (k8 + group) * 128) + (mix[u] ^ (((i * kSide) & 7) << 4)) + i * kSide * 128;
+    // byte of run u in row k4 + i kSide + group (k4 a multiple of 4) of tiles of 64 columns, `tile` bytes each
+    __device__ __forceinline__ uint32_t place(int u, int k4, int i, int group, int tile) const {
+        return static_cast<uint32_t>((at[u] >> 6) * tile + (at[u] & 7) * 2 + (k4 + group) * 128) + (mix[u] ^ (((k4 + i * kSide) & 7) << 4)) + i * kSide * 128;
     }
     __device__ __forceinline__ void load(const float* src, int dim, float (&x)[8]) const {
 #pragma unroll
@@ -172,6 +173,18 @@ __device__ __forceinline__ Place place_of(const ChunkParams& c, int unit, int ch
     a.row0 = static_cast<size_t>(a.seq) * c.d.n_tok + first;
     return a;
 }
+// Brings rows of 4 d bytes of the projections into the second-level cache for the CTA that will stand where this one does, a wave of two to an SM later: its
+// first loads would otherwise wait for memory with nothing else to do.
+__device__ __forceinline__ void fetch_ahead(const ChunkParams& c, int column0, int column1) {
+    const long long next = static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x + 2 * kNumSm;
+    const int unit = static_cast<int>(next / gridDim.x), chunk = static_cast<int>(next % gridDim.x);
+    if (unit >= gridDim.y || !c.d.vec || threadIdx.x >= 2 * kTokens) return;
+    const int first = c.first + chunk * kTokens, n = min(kTokens, c.d.n_tok - first), j = threadIdx.x % kTokens, column = threadIdx.x < kTokens ? column0 : column1;
+    if (j >= n || column < 0) return;
+    const float* row = c.d.proj + (static_cast<size_t>(unit / c.d.H) * c.d.n_tok + first + j) * c.d.ld + column + unit % c.d.H * c.d.d;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row), "r"(c.d.d * 4) : "memory");
+}
+
 __device__ __forceinline__ int table_row(const DecayParams& p, int pos) { return p.r.half > 0 ? min(max(pos, 0), p.r.positions - 1) : 0; }
 
 // the power of two that a normed head's numbers are divided by: sqrt(d) times the largest weight bounds them
@@ -187,14 +200,14 @@ __device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
 // go to decay_chunk_kernel on the way, as the tiles that it multiplies.  Bound by instructions, ten for a number; two CTAs to an SM.
 constexpr float kUp = 8192.0f;                           // 2^13: numbers below 2 end below 2^14
 template <int DP, int V, bool EXACT>
-__global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkParams c) {
+__global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
-    constexpr int kPiece = DP / 64 * kBox, kTile = DP / 64 * kSub, kPerWarp = 64 / kWarps, kRounds = kPerWarp / Lane::kSide, kRuns = Lane::kRuns;
+    constexpr int kSumWarps = kSumThreads / 32, kPiece = DP / 64 * kBox, kTile = DP / 64 * kSub, kPerWarp = 64 / kSumWarps, kRounds = kPerWarp / Lane::kSide, kRuns = Lane::kRuns;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(8) uint64_t done;
     __shared__ uint32_t tmem_slot;
-    __shared__ float weight_s[kTokens], most_s[2][kWarps];       // weight_s: decay from a token to the end of its chunk, 0 behind it
+    __shared__ float weight_s[kTokens], most_s[2][kSumWarps];       // weight_s: decay from a token to the end of its chunk, 0 behind it
     uint8_t *k_s = smem, *v_s = smem + 2 * kPiece;       // two terms each (the values' last tile may be read past its end: room for that is behind)
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const DecayParams& p = c.d;
@@ -213,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
     pdl_launch_dependents();                             // (after the allocation: a dependent's would otherwise stand in its way)
     pdl_wait();
     const Place a = place_of(c, blockIdx.y, blockIdx.x);
+    fetch_ahead(c, p.H * p.d, p.v_off);
     const float rate = p.log_decay[a.head];
     if (tid < kTokens) weight_s[tid] = tid < a.n - 1 ? expf(rate * static_cast<float>(a.n - 1 - tid)) : tid < a.n ? 1.0f : 0.0f;
     const int group = lane / Lane::kLph, gl = lane % Lane::kLph;
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_sums_kernel(const ChunkPara
         if (tile) alive = mbar_wait_bounded(&done, 0, p.status);          // the first tile's products have read their operands
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) most = fmaxf(most, most_s[tile][i]);
+        for (int i = 0; i < kSumWarps; ++i) most = fmaxf(most, most_s[tile][i]);
         const float top = fmaxf(power_below(most), 7.8886091e-31f), down = inverse_power(top) * kUp;
         back[tile] = top * (1.0f / (kUp * kUp));
 #pragma unroll
@@ -357,7 +371,7 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = row < p.d && 8 * gl + e < p.d ? c.states[state + 8 * gl + e] : 0.0f;
     const float4* src = reinterpret_cast<const float4*>(c.sums + static_cast<size_t>(unit) * c.chunks * DP * DP) + 2 * gl * DP + row;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     float4 x[kAhead][2];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
@@ -403,14 +417,14 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 // tokens' part of the outputs behind them, then the state's part over the weights.  Keys and values come by bulk copies while the queries are normed, the state's operand
 // by another into the keys' room.  Outputs are collected in shared memory, so that gates are read and rows are written whole.
 template <int DP, int V, bool EXACT>
-__global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkParams c) {
+__global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
-    constexpr int kTile = DP / 64 * kSub, kPerWarp = kTokens / kWarps, kLdo = DP + 4, kImage = DP * DP * 2;
-    constexpr int kRounds = kPerWarp / Lane::kSide, kFlight = kRounds < 4 ? kRounds : 4;
+    constexpr int kTile = DP / 64 * kSub, kPerWarp = kTokens / (kOutThreads / 32), kLdo = DP + 4, kImage = DP * DP * 2;
+    constexpr int kRounds = kPerWarp / Lane::kSide, kFlight = kRounds < 2 ? kRounds : 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(16) float kv_f[kTokens], scale_s[DP];
-    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[2][kTokens], most_s;       // power_s: y^n
+    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[4][kTokens], most_s;       // power_s: y^n
     __shared__ __align__(8) uint64_t bars[4];            // keys and values, scores, state's image, outputs
     __shared__ uint32_t tmem_slot;
     uint8_t *q_s = smem, *k_s = smem + kTile, *v_s = smem + 2 * kTile;
@@ -438,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
         bulk_g2s(k_s, c.tokens + a.at * 2 * kTile, 2 * kTile, &bars[0]);
     }
     __syncwarp();
+    fetch_ahead(c, 0, p.g_off);
     const float rate = p.log_decay[a.head];
     if (tid <= kTokens) power_s[tid] = tid ? expf(rate * static_cast<float>(tid)) : 1.0f;
     if (tid < DP) scale_s[tid] = c.scales[a.at * DP + tid];
@@ -520,10 +535,9 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
         bulk_g2s(k_s, c.images + a.at * kImage, kImage, &bars[2]);
     }
     __syncwarp();
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
+    const int row = (warp & 3) * 32 + lane, ch = warp >> 2;          // a thread has a row's fourth
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-#pragma unroll 1
-    for (int ch = 2 * half; ch < 2 * half + 2; ++ch) {
+    {
         uint32_t x[32], y[16];
         if (ch > (warp & 3)) {                           // nothing of it is visible to these rows
 #pragma unroll
@@ -567,18 +581,18 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
     if (alive) alive = mbar_wait_bounded(&bars[3], 0, p.status);
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
-    // a row's halves are two threads'; the sums of squares meet in shared memory
+    // the sums of squares of a row's fourths meet in shared memory
     const float f = q_f[row] * p.scale, inside = f * exp2f(most_s), before = f * power_s[min(row + 1, kTokens)];
     float ss = 0.0f;
 #pragma unroll 1
     for (int q = 0; q < DP / 64; ++q) {
-        const int col = half * (DP / 2) + 32 * q;
-        uint32_t x[32], y[32];
-        tmem_ld32(tmem + lanes + kTokens + col, x);
-        tmem_ld32(tmem + lanes + col, y);
+        const int col = ch * (DP / 4) + 16 * q;
+        uint32_t x[16], y[16];
+        tmem_ld16(tmem + lanes + kTokens + col, x);
+        tmem_ld16(tmem + lanes + col, y);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
+        for (int e = 0; e < 16; e += 4) {
             const float4 g = *reinterpret_cast<const float4*>(scale_s + col + e);
             float4 o;                                    // (columns from d on are zeros)
             o.x = fmaf(__uint_as_float(x[e]), inside, __uint_as_float(y[e]) * (before * g.x));
@@ -589,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
             *reinterpret_cast<float4*>(o_s + row * kLdo + col + e) = o;
         }
     }
-    ss_s[half][row] = ss;
+    ss_s[ch][row] = ss;
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
@@ -603,9 +617,9 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
     const bool vec = p.vec && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && (reinterpret_cast<uintptr_t>(p.norm) & 15) == 0;
     // (the gate's sigmoid by the fast exponential and reciprocal, 2^-21 each, before a rounding of 2^-9)
     auto open = [](float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); };
-    auto row_factor = [&](int j) { return norm ? rsqrtf((ss_s[0][j] + ss_s[1][j]) * c.per_dim + p.eps) : 1.0f; };
+    auto row_factor = [&](int j) { return norm ? rsqrtf(((ss_s[0][j] + ss_s[1][j]) + (ss_s[2][j] + ss_s[3][j])) * c.per_dim + p.eps) : 1.0f; };
     if (vec) {
-        constexpr int kLanes = DP / 4, kRows = kThreads / kLanes, kBatch = 8;            // lanes to a row, rows at a time
+        constexpr int kLanes = DP / 4, kRows = kOutThreads / kLanes, kBatch = 4;            // lanes to a row, rows at a time
         const int col = (tid % kLanes) * 4, j0 = tid / kLanes;
         if (col >= p.d) return;
         float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
@@ -630,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
             }
         }
     } else {
-        for (int i = tid; i < a.n * p.d; i += kThreads) {
+        for (int i = tid; i < a.n * p.d; i += kOutThreads) {
             const int j = i / p.d, col = i - j * p.d;
             out[static_cast<size_t>(j) * p.H * p.d + col] = __float2bfloat16_rn(o_s[j * kLdo + col] * row_factor(j) * (norm ? norm[col] : 1.0f) *
                                                                                 (gate ? open(gate[static_cast<size_t>(j) * p.ld + col]) : 1.0f));
@@ -641,13 +655,16 @@ __global__ void __launch_bounds__(kThreads, 2) decay_chunk_kernel(const ChunkPar
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
 int width_of(int dim) { return dim <= 64 ? 64 : 128; }
 
-// Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes.
+// Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes, and the two large kernels' last CTAs fill the GPU (8192
+// tokens of 32 heads: pieces of 9, 18, 37 and 64 chunks take 465, 440, 428 and 433 us, 39 chunks 436).
 constexpr size_t kPieceBytes = 352u << 20;
 int chunks_of(const tbl_decay_mixer& m, int n_seq, int n_tok) {
-    const size_t units = static_cast<size_t>(n_seq) * m.heads, w = width_of(m.dim);
+    const size_t units = static_cast<size_t>(n_seq) * m.heads, w = width_of(m.dim), wave = 2 * kNumSm;
     const size_t chunk = units * (kTokens * (m.dim * 8 + w * 4) + w * w * 6);
-    const int all = ceil_div(n_tok, kTokens), most = static_cast<int>(kPieceBytes / chunk);
-    return most < 1 ? 1 : (most < all ? most : all);
+    const size_t all = ceil_div(n_tok, kTokens), most = kPieceBytes / chunk;
+    if (most >= all) return static_cast<int>(all);
+    const size_t full = units * most / wave * wave / units, n = full ? full : most;
+    return n ? static_cast<int>(n) : 1;
 }
 
 struct Rooms { size_t sums, tokens, powers, images, scales, bytes; };
@@ -678,9 +695,9 @@ cudaError_t run(ChunkParams c, int per, cudaStream_t st) {
         c.first = at * kTokens;
         c.chunks = all - at < per ? all - at : per;
         c.states = at == 0 ? c.d.states : c.d.next;
-        e = launch_dependent(decay_sums_kernel<DP, V, EXACT>, dim3(c.chunks, units), dim3(kThreads), sums_smem, st, c);
+        e = launch_dependent(decay_sums_kernel<DP, V, EXACT>, dim3(c.chunks, units), dim3(kSumThreads), sums_smem, st, c);
         if (e == cudaSuccess) e = launch_dependent(decay_join_kernel<DP>, dim3(DP * DP / 8 / 128, units), dim3(128), 0, st, c);
-        if (e == cudaSuccess) e = launch_dependent(decay_chunk_kernel<DP, V, EXACT>, dim3(c.chunks, units), dim3(kThreads), chunk_smem, st, c);
+        if (e == cudaSuccess) e = launch_dependent(decay_chunk_kernel<DP, V, EXACT>, dim3(c.chunks, units), dim3(kOutThreads), chunk_smem, st, c);
     }
     return e;
 }
