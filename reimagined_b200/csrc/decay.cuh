@@ -10,6 +10,7 @@ struct DecayParams {
     const float* proj;           // [rows][ld]: q | k | v | gate
     const float *q, *k;          // scan: normed and turned, [rows][H][d]
     float* raw;                  // scan: scale S q, [rows][H][d]
+    float* starts;               // scan by segments: the states before them, [unit][segment][value][key]
     const float *log_decay, *norm;
     const float* states;         // [slots][H][value][key]
     float* next;                 // the same, after the last token
@@ -18,7 +19,7 @@ struct DecayParams {
     int* status;
     Rotation r;
     const float *q_norm, *k_norm;
-    int ld, H, d, v_off, g_off, n_seq, n_tok, vec;
+    int ld, H, d, v_off, g_off, n_seq, n_tok, vec, segments, segment;          // segments of `segment` tokens, the last one what is left
     float scale, eps;
 };
 

@@ -3,6 +3,7 @@
 //   decay_step_kernel        up to eight tokens, everything in one launch (heads of a multiple of four)
 //   decay_scan_kernel        the recurrence token by token, any size, between (head_rotation.cu), which norms and turns queries and keys, and
 //   decay_finish_kernel      head norm and output gate
+//   decay_starts_kernel      long scans of few heads: the states before segments of the tokens, which are then scanned side by side
 // Prompts in bf16 go by chunks (decay_chunk.cu).
 //
 // The decay enters as S + (exp(log_decay) - 1) S: 1 - exp(log_decay) has 24 bits however slow the decay is, whereas a decay rounded to fp32 would be off by 2^-25
@@ -18,7 +19,7 @@ using flash::fma2;
 using flash::pair_of;
 using flash::unpair;
 
-constexpr int kThreads = 256, kTile = 8;
+constexpr int kThreads = 256, kTile = 8, kMostSegments = 8;
 
 // LK lanes share a value row's keys: lane a holds 4 a + 4 LK j + e for j < C, in pairs of fp32.  A lane holds R rows, a warp 32 / LK times as many.  Lanes along
 // the keys, so that what all rows multiply with comes out of shared memory in whole lines (eight lanes a row: 328 lines a token for 32 rows of 90, and
@@ -30,6 +31,12 @@ struct State {
 
     static __device__ __forceinline__ bool wide(const DecayParams& p) {
         return p.d % 4 == 0 && (reinterpret_cast<uintptr_t>(p.states) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.next) & 15) == 0;
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < 2 * C; ++j) s[r][j] = 0;
     }
     // rows from `row` on of a head's state in global memory
     __device__ __forceinline__ void load(const DecayParams& p, const float* head, int row, int share) {
@@ -79,6 +86,24 @@ struct State {
             }
         }
     }
+    // the same in rows of kKeys, zeros behind a row's numbers
+    __device__ __forceinline__ void load_padded(int d, const float* head, int row, int share) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const ulonglong2 f = row + r < d ? *reinterpret_cast<const ulonglong2*>(head + (row + r) * kKeys + 4 * share + 4 * LK * j) : make_ulonglong2(0, 0);
+                s[r][2 * j] = f.x;
+                s[r][2 * j + 1] = f.y;
+            }
+    }
+    __device__ __forceinline__ void store_padded(int d, float* head, int row, int share) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (row + r < d) *reinterpret_cast<ulonglong2*>(head + (row + r) * kKeys + 4 * share + 4 * LK * j) = make_ulonglong2(s[r][2 * j], s[r][2 * j + 1]);
+    }
     // one token: the state, and this lane's share of its rows' outputs; v: the rows' values (R floats, R a multiple of 4 on 16 bytes)
     __device__ __forceinline__ void step(uint64_t less, const float* q, const float* k, const float* v, int share, float (&a)[R]) {
         ulonglong2 qq[C], kk[C];
@@ -106,6 +131,27 @@ struct State {
                 float lo, hi;
                 unpair(acc, lo, hi);
                 a[r + e] = lo + hi;
+            }
+        }
+    }
+    // one token's part of a sum, w: its decay
+    __device__ __forceinline__ void add(float w, const float* k, const float* v, int share) {
+        ulonglong2 kk[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) kk[j] = *reinterpret_cast<const ulonglong2*>(k + 4 * share + 4 * LK * j);
+#pragma unroll
+        for (int r = 0; r < R; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(v + r);
+            const float vr[4] = {f.x * w, f.y * w, f.z * w, f.w * w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint64_t vv = pair_of(vr[e], vr[e]);
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    uint64_t &x = s[r + e][2 * j], &y = s[r + e][2 * j + 1];
+                    x = fma2(kk[j].x, vv, x);
+                    y = fma2(kk[j].y, vv, y);
+                }
             }
         }
     }
@@ -250,35 +296,38 @@ __device__ __forceinline__ void copy4(float* dst, const float* src, bool ok) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
 
-// Any number of tokens: a CTA of four warps has 4 State::kRows rows of a head.  The tokens' vectors come by tiles of kTile ahead of their use, a thread the same columns of every
-// token; two tokens' instructions mix.
+// Any number of tokens: a CTA of four warps has 4 State::kRows rows of a head, and a segment of the tokens.  Their vectors come by tiles of kTile ahead of their
+// use, a thread the same columns of every token; two tokens' instructions mix.  SUMS: from an empty state, and only the state after the segment, which is the start of
+// the next (decay_starts_kernel adds what came before).
 constexpr int kScanThreads = 128;
-template <int LK, int C, int R>
+template <int LK, int C, int R, bool SUMS>
 __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayParams p) {
     using S = State<LK, C, R>;
-    constexpr int kRows = kScanThreads / 32 * S::kRows, kCols = 2 * S::kKeys + kRows, kPer = (kCols + kScanThreads - 1) / kScanThreads;
+    constexpr int kRows = kScanThreads / 32 * S::kRows, kFirst = SUMS ? S::kKeys : 0, kCols = 2 * S::kKeys + kRows, kPer = (kCols - kFirst + kScanThreads - 1) / kScanThreads;
     __shared__ __align__(16) float vec_s[2][kTile][kCols];       // queries, keys, values
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = lane % LK, first = warp * S::kRows + lane / LK * R;
-    const int head = blockIdx.x % p.H, seq = blockIdx.x / p.H, row0 = blockIdx.y * kRows;
+    const int head = blockIdx.x % p.H, seq = blockIdx.x / p.H, row0 = blockIdx.y * kRows, part = blockIdx.z;
+    const int tokens = min(p.segment, p.n_tok - part * p.segment);
     pdl_wait();
-    const int slot = p.slots[seq];
-    const size_t state = (static_cast<size_t>(slot) * p.H + head) * p.d * p.d, token0 = static_cast<size_t>(seq) * p.n_tok;
+    const size_t numbers = static_cast<size_t>(p.d) * p.d, token0 = static_cast<size_t>(seq) * p.n_tok + static_cast<size_t>(part) * p.segment;
+    const size_t state = (static_cast<size_t>(p.slots[seq]) * p.H + head) * numbers;
+    float* starts = p.starts + (static_cast<size_t>(blockIdx.x) * p.segments + part) * p.d * S::kKeys;
     const float* src[kPer];
     size_t stride[kPer];
     bool in[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int c = tid + i * kScanThreads, e = c < S::kKeys ? c : c < 2 * S::kKeys ? c - S::kKeys : row0 + c - 2 * S::kKeys;
+        const int c = kFirst + tid + i * kScanThreads, e = c < S::kKeys ? c : c < 2 * S::kKeys ? c - S::kKeys : row0 + c - 2 * S::kKeys;
         in[i] = c < kCols && e < p.d;
         const size_t at = (token0 * p.H + head) * p.d + (in[i] ? e : 0);
         src[i] = c < S::kKeys ? p.q + at : c < 2 * S::kKeys ? p.k + at : p.proj + token0 * p.ld + p.v_off + head * p.d + (in[i] ? e : 0);
         stride[i] = c < 2 * S::kKeys ? static_cast<size_t>(p.H) * p.d : p.ld;
     }
     auto fetch = [&](int t0, int buf) {
-        const int n = min(kTile, p.n_tok - t0);
+        const int n = min(kTile, tokens - t0);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int c = tid + i * kScanThreads;
+            const int c = kFirst + tid + i * kScanThreads;
             if (c >= kCols) break;
 #pragma unroll
             for (int t = 0; t < kTile; ++t) {
@@ -291,17 +340,25 @@ __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayPar
     };
     fetch(0, 0);
     S s;
-    s.load(p, p.states + state, row0 + first, share);
-    const float l = expm1f(p.log_decay[head]);
+    if constexpr (SUMS) s.clear();
+    else if (p.segments > 1) s.load_padded(p.d, starts, row0 + first, share);
+    else s.load(p, p.states + state, row0 + first, share);
+    const float rate = p.log_decay[head], l = expm1f(rate);
     const uint64_t less = pair_of(l, l);
     const int row = row0 + first + S::row_at(share);
     const bool writes = S::writes(share) && row < p.d;
     float* raw = p.raw + (token0 * p.H + head) * p.d + row;
-    for (int t0 = 0, buf = 0; t0 < p.n_tok; t0 += kTile, buf ^= 1) {
+    for (int t0 = 0, buf = 0; t0 < tokens; t0 += kTile, buf ^= 1) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();                                         // this tile is there, the one before it is no longer read
-        if (t0 + kTile < p.n_tok) fetch(t0 + kTile, buf ^ 1);
-        const int n = min(kTile, p.n_tok - t0);
+        if (t0 + kTile < tokens) fetch(t0 + kTile, buf ^ 1);
+        const int n = min(kTile, tokens - t0);
+        if constexpr (SUMS) {
+#pragma unroll 2
+            for (int t = 0; t < n; ++t)
+                s.add(expf(t0 + t == tokens - 1 ? 0.0f : rate * static_cast<float>(tokens - 1 - t0 - t)), vec_s[buf][t] + S::kKeys, vec_s[buf][t] + 2 * S::kKeys + first, share);
+            continue;
+        }
         auto token = [&](int t, float (&a)[R]) {
             const float* v = vec_s[buf][t];
             s.step(less, v, v + S::kKeys, v + 2 * S::kKeys + first, share, a);
@@ -327,7 +384,30 @@ __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayPar
         }
     }
     pdl_launch_dependents();
-    s.store(p, p.next + state, row0 + first, share);
+    if constexpr (SUMS) s.store_padded(p.d, starts + p.d * S::kKeys, row0 + first, share);
+    else if (part == p.segments - 1) s.store(p, p.next + state, row0 + first, share);
+}
+
+// The states before the segments, a thread per number of rows of `keys`: entry s > 0 holds what segment s - 1 adds to an empty state.
+__global__ void __launch_bounds__(256) decay_starts_kernel(const DecayParams p, int keys) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int unit = blockIdx.y, numbers = p.d * keys, i = blockIdx.x * 256 + threadIdx.x, row = i / keys, col = i % keys;
+    if (i >= numbers) return;
+    const int head = unit % p.H, slot = p.slots[unit / p.H];
+    float* at = p.starts + static_cast<size_t>(unit) * p.segments * numbers + i;
+    const float less = expm1f(p.log_decay[head] * static_cast<float>(p.segment));
+    float s = col < p.d ? p.states[((static_cast<size_t>(slot) * p.H + head) * p.d + row) * p.d + col] : 0.0f;
+    float x[kMostSegments];
+#pragma unroll
+    for (int k = 1; k < kMostSegments; ++k) x[k] = k < p.segments ? at[static_cast<size_t>(k) * numbers] : 0.0f;
+    at[0] = s;
+#pragma unroll
+    for (int k = 1; k < kMostSegments; ++k)
+        if (k < p.segments) {
+            s = fmaf(less, s, s) + x[k];
+            at[static_cast<size_t>(k) * numbers] = s;
+        }
 }
 
 // A warp per head of a row.
@@ -366,33 +446,48 @@ cudaError_t launch_step(const DecayParams& p, cudaStream_t st) {
 
 template <int LK, int C, int R>
 cudaError_t launch_scan_r(const DecayParams& p, cudaStream_t st) {
+    const unsigned units = p.n_seq * p.H, rows = ceil_div(p.d, kScanThreads / 32 * State<LK, C, R>::kRows);
+    if (p.n_tok <= kTile) return launch_dependent(decay_scan_kernel<LK, C, R, false>, dim3(units, rows), dim3(kScanThreads), 0, st, p);
     // Behind a kernel of many rows an early launch finds room on few SMs and stays there, several blocks to one (three prompts of 301 tokens, 10 heads of 90: 288
     // and 150 us).
-    const dim3 grid(p.n_seq * p.H, ceil_div(p.d, kScanThreads / 32 * State<LK, C, R>::kRows));
-    if (p.n_tok > kTile) {
-        decay_scan_kernel<LK, C, R><<<grid, kScanThreads, 0, st>>>(p);
+    if (p.segments > 1) {
+        decay_scan_kernel<LK, C, R, true><<<dim3(units, rows, p.segments - 1), kScanThreads, 0, st>>>(p);
         note_launch();
-        return cudaGetLastError();
+        const cudaError_t e = launch_dependent(decay_starts_kernel, dim3(ceil_div(p.d * State<LK, C, R>::kKeys, 256), units), dim3(256), 0, st, p, State<LK, C, R>::kKeys);
+        if (e != cudaSuccess) return e;
     }
-    return launch_dependent(decay_scan_kernel<LK, C, R>, grid, dim3(kScanThreads), 0, st, p);
+    decay_scan_kernel<LK, C, R, false><<<dim3(units, rows, p.segments), kScanThreads, 0, st>>>(p);
+    note_launch();
+    return cudaGetLastError();
 }
+// rows of a lane: twice as many once that leaves every SM two blocks
+int scan_rows(long long units, int d) { return keys_of(d) == 128 && units >= 2 * kNumSm ? 16 : keys_of(d) <= 64 ? 4 : 8; }
 cudaError_t launch_scan(const DecayParams& p, cudaStream_t st) {
-    // twice the rows to a lane once that leaves every SM two blocks
-    const long long units = static_cast<long long>(p.n_seq) * p.H;
     switch (keys_of(p.d)) {
         case 32: return launch_scan_r<8, 1, 4>(p, st);
         case 64: return launch_scan_r<16, 1, 4>(p, st);
-        case 128: return units >= 2 * kNumSm ? launch_scan_r<32, 1, 16>(p, st) : launch_scan_r<32, 1, 8>(p, st);
+        case 128: return scan_rows(static_cast<long long>(p.n_seq) * p.H, p.d) == 16 ? launch_scan_r<32, 1, 16>(p, st) : launch_scan_r<32, 1, 8>(p, st);
         default: return launch_scan_r<32, 2, 8>(p, st);
     }
+}
+// Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; the tokens are then read twice.  Six blocks to an SM, 32 tokens to
+// a segment or more (three prompts of 301 tokens, 10 heads of 90: no segments 76 us, two, four and six blocks to an SM 65, 61 and 58).
+int scan_segments(int heads, int d, int n_seq, int n_tok) {
+    const long long units = static_cast<long long>(n_seq) * heads;
+    const int keys = keys_of(d), lanes = keys <= 32 ? 8 : keys <= 64 ? 16 : 32;
+    const long long blocks = units * ceil_div(d, kScanThreads / 32 * (32 / lanes) * scan_rows(units, d));
+    long long s = 6LL * kNumSm / blocks;
+    if (s > n_tok / 32) s = n_tok / 32;
+    if (s > kMostSegments) s = kMostSegments;
+    return s > 1 && units <= 65535 ? static_cast<int>(s) : 1;
 }
 
 enum Route { kAuto = 0, kScan = 1, kChunk = 2 };
 constexpr int kChunkMinTokens = 48;
 
 struct Plan {
-    int route, whole;            // whole: the scan of a few tokens in one launch
-    size_t q, k, raw, chunk, bytes;
+    int route, whole, segments;  // whole: the scan of a few tokens in one launch
+    size_t q, k, raw, starts, chunk, bytes;
 };
 
 Plan make_plan(const tbl_decay_mixer& m, int precision, int route, int n_seq, int n_tok) {
@@ -405,6 +500,8 @@ Plan make_plan(const tbl_decay_mixer& m, int precision, int route, int n_seq, in
     w.q = take(4 * numbers);
     w.k = take(4 * numbers);
     w.raw = take(4 * numbers);
+    w.segments = numbers ? scan_segments(m.heads, m.dim, n_seq, n_tok) : 1;
+    w.starts = take(w.segments > 1 ? sizeof(float) * n_seq * m.heads * w.segments * m.dim * keys_of(m.dim) : 0);
     w.chunk = take(w.route == kChunk ? decay_chunk_workspace(m, n_seq, n_tok) : 0);
     w.bytes = off > 0 ? off : 256;
     return w;
@@ -443,6 +540,9 @@ int launch_decay(const tbl_decay_mixer& m, int precision, int route, float eps, 
     if (w.whole) return (precision == TBL_BF16 ? launch_step<bf16>(p, st) : launch_step<float>(p, st)) == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
     float *q = reinterpret_cast<float*>(base + w.q), *k = reinterpret_cast<float*>(base + w.k);
     p.q = q; p.k = k; p.raw = reinterpret_cast<float*>(base + w.raw);
+    p.starts = reinterpret_cast<float*>(base + w.starts);
+    p.segment = ceil_div(n_tok, w.segments);
+    p.segments = ceil_div(n_tok, p.segment);
     const RotationCall c{proj, p.ld, m.heads, m.heads, m.dim, slots, positions, n_seq, n_tok, eps, q, k, nullptr, 0};
     const int rc = launch_head_rotation(m.rotation, TBL_F32, c, st);
     if (rc != TBL_OK) return rc;
