@@ -262,7 +262,7 @@ int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int precision, 
                               void* q_dev, void* k_dev, void* stream);
 /* Attention over the 4-bit cache on stacked projections proj fp32 [rows, in.outputs]: norm, rotation, rounding and append at
  * positions_dev[slot] .., attention, output gate -> out (precision's type) [rows, heads*dim].  cache_dev [slots][kv_heads][capacity]
- * [row bytes], 16-byte aligned; rows behind a sequence's last token are neither used nor written, whatever they hold.  A token past the capacity or the
+ * [row bytes], 16-byte aligned; slots_dev names distinct slots, context covers every sequence's tokens; rows behind a sequence's last token are neither used nor written, whatever they hold.  A token past the capacity or the
  * rotary tables sets TBL_DEV_CACHE_FULL; the rows of its sequence are undefined, the cache holds what has room.  positions_dev is not
  * advanced, so that a repeated call writes the same rows again.  route: 0 as the step, 1 fp32 arithmetic on the 4-bit rows, 2 the
  * cache-streaming kernel (warp-level MMAs on the 4-bit rows), 3 the flash kernel (tcgen05) over expanded keys and values, as far as its
@@ -279,7 +279,7 @@ int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const vo
                        void* stream);
 /* Linear attention with decay on stacked projections proj fp32 [rows, in.outputs]: norm, rotation, recurrence, head norm, output gate -> out
  * (precision's type) [rows, heads*dim].  states_dev fp32 [slots][heads][dim][dim] are read, next_states_dev (the same array, or another of
- * its shape) receives those after the last token; slots not named are not touched.  A token past the rotary tables sets TBL_DEV_CACHE_FULL; the rows and
+ * its shape) receives those after the last token; slots_dev names distinct slots, the others are not touched.  A token past the rotary tables sets TBL_DEV_CACHE_FULL; the rows and
  * states of its sequence are undefined.  Projections are finite: a prompt is worked out in blocks, in which one that is not spoils other rows.  route: 0 as the step, 1 the scan kernel (any size, fp32
  * arithmetic), 2 the chunk kernels (tcgen05; bf16, dim <= 128). */
 size_t tbl_decay_workspace_bytes(const tbl_decay_mixer* mixer, int precision, int route, int n_seq, int n_tok);

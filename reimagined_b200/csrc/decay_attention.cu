@@ -492,7 +492,7 @@ struct Plan {
 
 Plan make_plan(const tbl_decay_mixer& m, int precision, int route, int n_seq, int n_tok) {
     Plan w{};
-    w.route = route != kAuto ? route : precision == TBL_BF16 && n_tok >= kChunkMinTokens && decay_chunk_supported(m) ? kChunk : kScan;
+    w.route = route != kAuto ? route : precision == TBL_BF16 && n_tok >= kChunkMinTokens && decay_chunk_supported(m) && static_cast<long long>(n_seq) * m.heads <= 65535 ? kChunk : kScan;
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };
     w.whole = w.route == kScan && step_supported(m, n_tok);

@@ -172,7 +172,10 @@ extern "C" int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int 
     const long long heads = static_cast<long long>(q_heads) + k_heads;
     if (heads == 0) return TBL_ERR_INVALID_ARG;
     if (heads * dim > ld || static_cast<long long>(n_seq) * n_tok > 2147483647LL) return TBL_ERR_SHAPE;
-    if (reinterpret_cast<uintptr_t>(proj_dev) & 3) return TBL_ERR_ALIGNMENT;
+    const uintptr_t own = precision == TBL_BF16 ? 1 : 3;
+    if ((reinterpret_cast<uintptr_t>(proj_dev) & 3) || (q_heads > 0 && (reinterpret_cast<uintptr_t>(q_dev) & own)) ||
+        (k_heads > 0 && (reinterpret_cast<uintptr_t>(k_dev) & own)))
+        return TBL_ERR_ALIGNMENT;
     const RotationCall c{proj_dev, ld, q_heads, k_heads, dim, slots_dev, positions_dev, n_seq, n_tok, eps, q_heads > 0 ? q_dev : nullptr, k_heads > 0 ? k_dev : nullptr, nullptr, 0};
     return launch_head_rotation(*rotation, precision, c, static_cast<cudaStream_t>(stream));
 }

@@ -349,7 +349,8 @@ int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const vo
     if (rc != TBL_OK) return rc;
     const long long rows = static_cast<long long>(n_seq) * n_tok;
     if (rows > 2147483647LL) return TBL_ERR_SHAPE;
-    if (!aligned16(cache_dev)) return TBL_ERR_ALIGNMENT;
+    const uintptr_t own = precision == TBL_BF16 ? 1 : 3;
+    if (!aligned16(cache_dev) || ((reinterpret_cast<uintptr_t>(keys_dev) | reinterpret_cast<uintptr_t>(values_dev)) & own)) return TBL_ERR_ALIGNMENT;
     QuantizedParams p = basic_params(*mixer, capacity, slots_dev, positions_dev, n_tok);
     if (!p.status) return TBL_ERR_CUDA;
     p.cache = static_cast<uint8_t*>(const_cast<void*>(cache_dev));

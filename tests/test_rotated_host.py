@@ -68,6 +68,14 @@ def quantized(**kw):
                                d["dim"], d["gated"], d["scale"], d["key_scale"], d["value_scale"])
 
 
+def test_results_lie_on_their_types_bytes(stack_lib):
+    before = stack_lib.tbl_launch_count()
+    for precision, q, k, rc in ((0, 4098, 4096, -6), (0, 4096, 4098, -6), (1, 4097, 4096, -6), (1, 4096, 4099, -6)):
+        assert stack_lib.tbl_head_rotation_forward(C.byref(rotated()), precision, 1e-5, 4096, 192, 4, 2, 32, 4096, 4096, 1, 1, q, k, None) == rc
+        assert stack_lib.tbl_quantized_read(C.byref(quantized()), precision, 4096, 2, 16, 4096, 4096, 1, 1, q, k, None) == rc
+    assert stack_lib.tbl_launch_count() == before
+
+
 def test_quantized_attention_refuses_before_it_touches_a_device(stack_lib):
     L, before = stack_lib, stack_lib.tbl_launch_count()
     call = lambda m=None, **k: L.tbl_quantized_forward(C.byref(m or quantized()), k.get("precision", 1), k.get("route", 0), 1e-5, k.get("proj", 4096), k.get("cache", 4096), 2, 16,
