@@ -118,7 +118,7 @@ typedef struct tbl_head_rotation {
  * key_scale or value_scale, for every 16 neighbouring dimensions of a head:
  *   s = e4m3(min(max |x| / (6 u), 448)),   code = e2m1(x / (s u)),   the number is code s u;
  * all roundings to nearest, ties to even, e2m1 ends at 6; s = 0 makes all codes 0; a group with a number that is not finite is 16 NaNs.
- * key_scale and value_scale are finite and > 0: chosen so that max |x| / (6 u) of ordinary groups is far from e4m3's ends, 2^-9 and 448.
+ * scale, key_scale and value_scale are finite and > 0; the latter two chosen so that max |x| / (6 u) of ordinary groups is far from e4m3's ends, 2^-9 and 448.
  * A cached token of a head is a row of tbl_quantized_row_bytes: with n = dim rounded up to 64, n/2 bytes of key codes (the even
  * dimension in the low half of a byte), n/2 of value codes, n/16 scales of the key, n/16 of the value, then zeros to a multiple of 16. */
 typedef struct tbl_quantized_mixer {

@@ -8,6 +8,8 @@
 //
 // The decay enters as S + (exp(log_decay) - 1) S: 1 - exp(log_decay) has 24 bits however slow the decay is, whereas a decay rounded to fp32 would be off by 2^-25
 // every token, all in one direction.
+#include <float.h>
+
 #include "decay.cuh"
 #include "flash.cuh"
 
@@ -514,6 +516,7 @@ int check_decay(const tbl_decay_mixer& m, int width) {
     const int rc = check_rotation(m.rotation, m.dim);
     if (rc != TBL_OK) return rc;
     if (!m.log_decay || (m.gated != 0 && m.gated != 1)) return TBL_ERR_INVALID_ARG;
+    if (!(fabsf(m.scale) <= FLT_MAX)) return TBL_ERR_SCALE;
     if (m.in.inputs != width || m.in.outputs != static_cast<long long>(3 + m.gated) * m.heads * m.dim || m.out.inputs != m.heads * m.dim || m.out.outputs != width)
         return TBL_ERR_SHAPE;
     return m.in.weight && m.out.weight ? TBL_OK : TBL_ERR_INVALID_ARG;

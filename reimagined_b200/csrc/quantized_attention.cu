@@ -274,6 +274,8 @@ int check_quantized(const tbl_quantized_mixer& m, int width) {
     const int rc = check_rotation(m.rotation, m.dim);
     if (rc != TBL_OK) return rc;
     if (!(m.key_scale > 0.0f) || !(m.value_scale > 0.0f) || m.key_scale > 1e30f || m.value_scale > 1e30f || m.key_scale < 1e-30f || m.value_scale < 1e-30f) return TBL_ERR_SCALE;
+    const double factor = static_cast<double>(m.scale) * m.key_scale;       // of the scores: the flash kernel takes their largest before it
+    if (!(factor >= 1e-30 && factor <= 1e30)) return TBL_ERR_SCALE;
     if (m.gated != 0 && m.gated != 1) return TBL_ERR_INVALID_ARG;
     const long long cols = (static_cast<long long>(m.heads) * (1 + m.gated) + 2LL * m.kv_heads) * m.dim;
     if (m.in.inputs != width || m.in.outputs != cols || m.out.inputs != m.heads * m.dim || m.out.outputs != width) return TBL_ERR_SHAPE;

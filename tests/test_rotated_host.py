@@ -68,6 +68,19 @@ def quantized(**kw):
                                d["dim"], d["gated"], d["scale"], d["key_scale"], d["value_scale"])
 
 
+def test_factors_of_scores_and_outputs(stack_lib):
+    before = stack_lib.tbl_launch_count()
+    for scale in (0.0, -0.2, float("nan"), float("inf"), 1e38, 1e-38):
+        assert stack_lib.tbl_quantized_forward(C.byref(quantized(scale=scale)), 1, 0, 1e-5, 4096, 4096, 2, 16, 4096, 4096, 1, 1, 16, 4096, 4096, 1 << 40, None) == -4
+        assert stack_lib.tbl_quantized_workspace_bytes(C.byref(quantized(scale=scale)), 1, 0, 1, 1, 16) == 0
+    m = decay()
+    for m.scale in (float("nan"), float("inf")):
+        assert stack_lib.tbl_decay_forward(C.byref(m), 1, 0, 1e-5, 4096, 4096, 4096, 4096, 4096, 1, 1, 4096, 4096, 1 << 40, None) == -4
+    m.scale = -0.5
+    assert stack_lib.tbl_decay_workspace_bytes(C.byref(m), 1, 0, 1, 1) > 0
+    assert stack_lib.tbl_launch_count() == before
+
+
 def test_results_lie_on_their_types_bytes(stack_lib):
     before = stack_lib.tbl_launch_count()
     for precision, q, k, rc in ((0, 4098, 4096, -6), (0, 4096, 4098, -6), (1, 4097, 4096, -6), (1, 4096, 4099, -6)):
