@@ -13,6 +13,8 @@
 //
 // Bound: the cache's bytes.  A tile of 16 tokens of a head of 128 (2304 bytes, 100 cycles of an SM's share of the memory) costs 64 conversions and some 40 logic
 // operations on one pipe (two warps a cycle) and 64 multiplications on another.
+#include <float.h>
+
 #include "attention.cuh"
 #include "quantized.cuh"
 #include "tc05.cuh"
@@ -49,7 +51,17 @@ __device__ __forceinline__ __half2 scales_of(uint32_t bytes) {
     return *reinterpret_cast<const __half2*>(&h);
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
-__device__ __forceinline__ uint32_t lds8(uint32_t a) { uint32_t v; asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
+// N words from a place of 4 bytes on, pairs at once where it is one of 8
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[i]), "=r"(v[i + 1]) : "r"(a + 4 * i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = lds32(a + 4 * i);
+    }
+}
 __device__ __forceinline__ uint2 lds64(uint32_t a) { uint2 v; asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a)); return v; }
 
 // The token (of 16) that stands in row i of an MMA: with rows of 144 bytes the 16 or 32 lanes that a shared-memory access serves together then hit every bank once,
@@ -170,7 +182,8 @@ __global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const Quantize
             for (int e = 0; e < 4; ++e) o[i][u][e] = 0.0f;
     float mx[NT][2], sum[NT][2];
 #pragma unroll
-    for (int u = 0; u < NT; ++u) { mx[u][0] = mx[u][1] = -INFINITY; sum[u][0] = sum[u][1] = 0.0f; }
+    for (int u = 0; u < NT; ++u) { mx[u][0] = mx[u][1] = -FLT_MAX; sum[u][0] = sum[u][1] = 0.0f; }
+    const uint32_t key_byte = t4 | (4 + t4) << 4, value_byte = (g8 >> 1) | (4 + (g8 >> 1)) << 4;   // that byte of either word
     const int ka = token_of(g8), va = token_of(2 * t4), vb = token_of(2 * t4 + 1);               // MMA rows 8 .. 15: one token further on
     bool alive = true;
     uint32_t phase = 0;
@@ -192,10 +205,13 @@ __global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const Quantize
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[h][u][e] = 0.0f;
             const uint32_t row = tile + (16 * h + ka) * L::kRow;
+            uint32_t sx4[kBlocks], sy4[kBlocks];                 // scales of a block, a byte each
+            lds_words<kBlocks>(row + DP, sx4);
+            lds_words<kBlocks>(row + L::kRow + DP, sy4);
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const uint2 x = lds64(row + 32 * b + 8 * t4), y = lds64(row + L::kRow + 32 * b + 8 * t4);
-                const __half2 both = scales_of(lds8(row + DP + 4 * b + t4) | lds8(row + L::kRow + DP + 4 * b + t4) << 8);
+                const __half2 both = scales_of(__byte_perm(sx4[b], sy4[b], key_byte));
                 const __half2 sx = __low2half2(both), sy = __high2half2(both);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
@@ -211,11 +227,10 @@ __global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const Quantize
             }
         }
         const bool whole = t + kTile - 1 <= all_see;             // nothing of the tile is masked
-        uint32_t pt[2][NT][2];
-        float f[NT][2];
+        float top[NT][2];
         bool grown = false;
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float x[4];                                      // tokens ka, ka + 1 of either half
@@ -223,21 +238,39 @@ __global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const Quantize
                 for (int i = 0; i < 4; ++i) {
                     x[i] = s[i >> 1][u][2 * (i & 1) + e] * c[u][e];
                     if (!whole && t + 16 * (i >> 1) + ka + (i & 1) > last[u][e]) x[i] = -INFINITY;
+                    s[i >> 1][u][2 * (i & 1) + e] = x[i];
                 }
-                float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                // the maximum only moves when it grows by 2^8: then output and sum are rescaled
-                const float mn = top > mx[u][e] + kRescale ? top : mx[u][e], base = mn == -INFINITY ? 0.0f : mn;     // nothing seen yet: all weights zero
-                f[u][e] = mn == mx[u][e] ? 1.0f : ex2(mx[u][e] - base);
-                grown = grown || f[u][e] != 1.0f;
-                mx[u][e] = mn;
+                top[u][e] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                grown = grown || top[u][e] > mx[u][e] + kRescale;
+            }
+        // the maximum only moves when it grows by 2^8, so that lanes need not ask each other for most tiles; then output and sum are rescaled
+        if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - base);
-                sum[u][e] = fmaf(sum[u][e], f[u][e], (x[0] + x[1]) + (x[2] + x[3]));
+            for (int u = 0; u < NT; ++u) {
+                float f[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[i >> 1][u][2 * (i & 1) + e] = x[i];
+                for (int e = 0; e < 2; ++e) {
+                    float m = top[u][e];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    m = m > mx[u][e] + kRescale ? m : mx[u][e];
+                    f[e] = ex2(mx[u][e] - m);
+                    mx[u][e] = m;
+                    sum[u][e] *= f[e];
+                }
+#pragma unroll
+                for (int i = 0; i < kBlocks * 4; ++i) { o[i][u][0] *= f[0]; o[i][u][1] *= f[1]; o[i][u][2] *= f[0]; o[i][u][3] *= f[1]; }
+            }
+        }
+        uint32_t pt[2][NT][2];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i >> 1][u][2 * (i & 1) + e] = x[i] = ex2(s[i >> 1][u][2 * (i & 1) + e] - mx[u][e]);
+                sum[u][e] += (x[0] + x[1]) + (x[2] + x[3]);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -247,29 +280,31 @@ __global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const Quantize
                     pt[h][u][r] = transposed(*reinterpret_cast<const uint32_t*>(&w));
                 }
         }
-        if (__any_sync(0xffffffffu, grown)) {
+        // rows nobody has written may hold anything: a weight of zero needs a finite value beside it (the split's last tile: nothing is loaded over it any more)
+        if (t + kTile > t1) {
+            if (t + lane >= t1)
 #pragma unroll
-            for (int i = 0; i < kBlocks * 4; ++i)
-#pragma unroll
-                for (int u = 0; u < NT; ++u) { o[i][u][0] *= f[u][0]; o[i][u][1] *= f[u][1]; o[i][u][2] *= f[u][0]; o[i][u][3] *= f[u][1]; }
+                for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<uint32_t*>(ring + stage * L::kTileBytes + lane * L::kRow + DP + DP / 16 + 4 * b) = 0;
+            __syncwarp();
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             // MMA columns 2 t4, 2 t4 + 1 are tokens va, vb, columns 2 t4 + 8, 2 t4 + 9 the ones behind them
             const uint32_t ra = tile + (16 * h + va) * L::kRow, rb = tile + (16 * h + vb) * L::kRow;
-            const uint32_t codes = DP / 2 + 4 * g8, scale = DP + DP / 16 + (g8 >> 1);
+            const uint32_t codes = DP / 2 + 4 * g8, scale = DP + DP / 16;
+            uint32_t sa4[2][kBlocks], sb4[2][kBlocks];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                lds_words<kBlocks>(ra + d * L::kRow + scale, sa4[d]);
+                lds_words<kBlocks>(rb + d * L::kRow + scale, sb4[d]);
+            }
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 uint32_t a[2][8];
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                     const uint32_t wa = lds32(ra + d * L::kRow + codes + 32 * b), wb = lds32(rb + d * L::kRow + codes + 32 * b);
-                    uint32_t sa = lds8(ra + d * L::kRow + scale + 4 * b), sb = lds8(rb + d * L::kRow + scale + 4 * b);
-                    if (!whole) {                                // rows nobody has written may hold anything: a weight of zero needs a finite value beside it
-                        if (t + 16 * h + va + d >= t1) sa = 0;
-                        if (t + 16 * h + vb + d >= t1) sb = 0;
-                    }
-                    const __half2 sc = scales_of(sa | sb << 8);
+                    const __half2 sc = scales_of(__byte_perm(sa4[d][b], sb4[d][b], value_byte));
                     uint32_t even[4], odd[4];
                     widen((wa & 0x0f0f0f0fu) | ((wb << 4) & 0xf0f0f0f0u), sc, even);
                     widen(((wa >> 4) & 0x0f0f0f0fu) | (wb & 0xf0f0f0f0u), sc, odd);
@@ -315,7 +350,7 @@ __global__ void __launch_bounds__(32 * W) quantized_stream_kernel(const Quantize
         float l = 0.0f;
 #pragma unroll
         for (int k = 0; k < W; ++k) {
-            const float w = m_s[k][r] == -INFINITY ? 0.0f : ex2(m_s[k][r] - top);
+            const float w = ex2(m_s[k][r] - top);
             const float4 x = *reinterpret_cast<const float4*>(o_s + (k * kRows + r) * L::kLdo + col);
             v.x = fmaf(x.x, w, v.x); v.y = fmaf(x.y, w, v.y); v.z = fmaf(x.z, w, v.z); v.w = fmaf(x.w, w, v.w);
             l = fmaf(l_s[k][r], w, l);
