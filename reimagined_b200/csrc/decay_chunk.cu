@@ -244,16 +244,18 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
     __syncthreads();
     bool alive = true;
     float back[2];                                       // from a tile's sums to theirs
+    float k[kRounds][8], v[kRounds][8];
+    // (rows behind the last token: that one again, times 0)
+    auto row_of = [&](int tile, int i) { return base + static_cast<size_t>(min(tile * 64 + warp * kPerWarp + group + i * Lane::kSide, a.n - 1)) * p.ld; };
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        kl.load(row_of(0, i) + p.H * p.d, p.d, k[i]);
+        vl.load(row_of(0, i) + p.v_off, p.d, v[i]);
+    }
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
-        float k[kRounds][8], v[kRounds][8], inv[kRounds], up[kRounds], most = 0.0f;
+        float inv[kRounds], up[kRounds], most = 0.0f;
         const int j0 = tile * 64 + warp * kPerWarp + group;
-#pragma unroll
-        for (int i = 0; i < kRounds; ++i) {              // (rows behind the last token: that one again, times 0)
-            const float* src = base + static_cast<size_t>(min(j0 + i * Lane::kSide, a.n - 1)) * p.ld;
-            kl.load(src + p.H * p.d, p.d, k[i]);
-            vl.load(src + p.v_off, p.d, v[i]);
-        }
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
             const int j = j0 + i * Lane::kSide;
@@ -303,6 +305,10 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
 #pragma unroll
                 for (int e = 0; e < V; ++e) y[e] = v[i][V * u + e] * f;
                 if (vl.at[u] < DP) put_terms<V>(v_s + vl.place(u, warp * kPerWarp, i, group, kBox), kPiece, y, nullptr);
+            }
+            if (tile == 0) {                             // these registers are free: the second tile's numbers come under what is left of the first
+                kl.load(row_of(1, i) + p.H * p.d, p.d, k[i]);
+                vl.load(row_of(1, i) + p.v_off, p.d, v[i]);
             }
         }
         fence_proxy_async();
