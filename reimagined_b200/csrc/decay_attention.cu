@@ -1,6 +1,6 @@
 // Linear attention with a constant decay for each head: S <- exp(log_decay) S + v k^T, o = scale S q.
 //
-//   decay_step_kernel        up to eight tokens, everything in one launch (heads of a multiple of four)
+//   decay_step_kernel        up to four tokens, everything in one launch (heads of a multiple of four)
 //   decay_scan_kernel        the recurrence token by token, any size, between (head_rotation.cu), which norms and turns queries and keys, and
 //   decay_finish_kernel      head norm and output gate
 //   decay_starts_kernel      long scans of few heads: the states before segments of the tokens, which are then scanned side by side
@@ -21,7 +21,7 @@ using flash::fma2;
 using flash::pair_of;
 using flash::unpair;
 
-constexpr int kThreads = 256, kTile = 8, kMostSegments = 8;
+constexpr int kThreads = 256, kTile = 8, kStepTokens = 4, kMostSegments = 8;
 
 // LK lanes share a value row's keys: lane a holds 4 a + 4 LK j + e for j < C, in pairs of fp32.  A lane holds R rows, a warp 32 / LK times as many.  Lanes along
 // the keys, so that what all rows multiply with comes out of shared memory in whole lines (eight lanes a row: 328 lines a token for 32 rows of 90, and
@@ -203,7 +203,7 @@ __device__ __forceinline__ void finish_head(const DecayParams& p, const float* s
     }
 }
 
-// Up to eight tokens of a head in one launch.  A CTA has the whole head: its state comes into shared memory by one bulk copy and goes back by another, so that registers
+// Up to four tokens of a head in one launch (32 heads of 128, four tokens 9.2 us, eight 14.1, the scan of nine 11.0; 16 sequences 21.8, 34.7 and 31.7).  A CTA has the whole head: its state comes into shared memory by one bulk copy and goes back by another, so that registers
 // hold a few rows at a time and three CTAs of heads of 128 share an SM; while it comes, a warp each norms and turns the tokens' queries and keys.  Bound by the
 // state's bytes: the projections are asked for first, or they would queue behind the states of the whole batch.
 constexpr size_t kStepRoom = 200 * 1024;
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(256) decay_finish_kernel(const DecayParams p) 
 }
 
 int keys_of(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-bool step_supported(const tbl_decay_mixer& m, int n_tok) { return n_tok <= kTile && m.dim % 4 == 0 && step_smem(keys_of(m.dim), m.dim, n_tok) <= kStepRoom; }
+bool step_supported(const tbl_decay_mixer& m, int n_tok) { return n_tok <= kStepTokens && m.dim % 4 == 0 && step_smem(keys_of(m.dim), m.dim, n_tok) <= kStepRoom; }
 template <typename T, int V, int LK, int C>
 cudaError_t launch_step_lk(const DecayParams& p, cudaStream_t st) {
     static bool done[64] = {};
@@ -450,8 +450,8 @@ template <int LK, int C, int R>
 cudaError_t launch_scan_r(const DecayParams& p, cudaStream_t st) {
     const unsigned units = p.n_seq * p.H, rows = ceil_div(p.d, kScanThreads / 32 * State<LK, C, R>::kRows);
     if (p.n_tok <= kTile) return launch_dependent(decay_scan_kernel<LK, C, R, false>, dim3(units, rows), dim3(kScanThreads), 0, st, p);
-    // Behind a kernel of many rows an early launch finds room on few SMs and stays there, several blocks to one (three prompts of 301 tokens, 10 heads of 90: 288
-    // and 150 us).
+    // Behind a kernel of many rows an early launch finds room on few SMs and stays there, several blocks to one (2000 tokens of 8 heads of 128: 263 and 119 us, three
+    // prompts of 301 tokens, 10 heads of 90, 59 and 54).
     if (p.segments > 1) {
         decay_scan_kernel<LK, C, R, true><<<dim3(units, rows, p.segments - 1), kScanThreads, 0, st>>>(p);
         note_launch();
@@ -472,20 +472,27 @@ cudaError_t launch_scan(const DecayParams& p, cudaStream_t st) {
         default: return launch_scan_r<32, 2, 8>(p, st);
     }
 }
-// Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; the tokens are then read twice.  Six blocks to an SM, 32 tokens to
-// a segment or more (three prompts of 301 tokens, 10 heads of 90: no segments 76 us, two, four and six blocks to an SM 65, 61 and 58).
+// Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; with segments the tokens are read twice, by more blocks.  Times in us: a
+// token 0.2 where a block has an SM to itself, 0.1 for each block where they share one, sums alone half of that; the other two launches 9.5.  Fewest of that wins (fp32,
+// without and with: three prompts of 301 tokens, 10 heads of 90, 71 and 54; 32 heads of 128, 64 tokens 23 and 28, 300 tokens 77 and 68).
 int scan_segments(int heads, int d, int n_seq, int n_tok) {
     const long long units = static_cast<long long>(n_seq) * heads;
     const int keys = keys_of(d), lanes = keys <= 32 ? 8 : keys <= 64 ? 16 : 32;
-    const long long blocks = units * ceil_div(d, kScanThreads / 32 * (32 / lanes) * scan_rows(units, d));
-    long long s = 6LL * kNumSm / blocks;
-    if (s > n_tok / 32) s = n_tok / 32;
-    if (s > kMostSegments) s = kMostSegments;
-    return s > 1 && units <= 65535 ? static_cast<int>(s) : 1;
+    const double share = static_cast<double>(units) * ceil_div(d, kScanThreads / 32 * (32 / lanes) * scan_rows(units, d)) / kNumSm;       // blocks to an SM
+    auto alone = [](double token, double shared) { return token > shared ? token : shared; };
+    int best = 1;
+    double least = n_tok * alone(0.2, 0.1 * share);
+    for (int s = 2; s <= kMostSegments && units <= 65535; ++s) {
+        const double t = 9.5 + round_up(ceil_div(n_tok, s), kTile) * (alone(0.2, 0.1 * share * s) + alone(0.1, 0.05 * share * s));
+        if (t <= 1.01 * least) { least = t; best = s; }
+    }
+    return best;
 }
 
 enum Route { kAuto = 0, kScan = 1, kChunk = 2 };
-constexpr int kChunkMinTokens = 48;
+// Tokens from which the chunks are faster than the scan: few heads leave both waiting for one chain (32 heads of 128, scan and chunks: 48 tokens 19 and 23 us, 64 27 and
+// 24; 256 heads: 48 tokens 55 and 50).
+int chunk_min_tokens(long long units) { return units >= kNumSm ? 48 : 64; }
 
 struct Plan {
     int route, whole, segments;  // whole: the scan of a few tokens in one launch
@@ -494,7 +501,8 @@ struct Plan {
 
 Plan make_plan(const tbl_decay_mixer& m, int precision, int route, int n_seq, int n_tok) {
     Plan w{};
-    w.route = route != kAuto ? route : precision == TBL_BF16 && n_tok >= kChunkMinTokens && decay_chunk_supported(m) && static_cast<long long>(n_seq) * m.heads <= 65535 ? kChunk : kScan;
+    const long long units = static_cast<long long>(n_seq) * m.heads;
+    w.route = route != kAuto ? route : precision == TBL_BF16 && n_tok >= chunk_min_tokens(units) && decay_chunk_supported(m) && units <= 65535 ? kChunk : kScan;
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };
     w.whole = w.route == kScan && step_supported(m, n_tok);

@@ -120,6 +120,7 @@ struct StreamPlan {
     int warps, splits;           // of a CTA; of the context
     int whole;                   // one token of a sequence, no splits: the kernel norms, rounds, appends and finishes by itself
 };
+int quantized_stream_rows(const tbl_quantized_mixer& m, int n_tok);      // query rows of a CTA
 StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
 int launch_quantized_stream(const QuantizedParams& p, const StreamPlan& plan, int vec, int n_seq, cudaStream_t st);
 

@@ -5,6 +5,7 @@
 //   quantized_read_kernel    the same for single tokens, in the layer's units
 // Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, and weights need one term instead of two), a few query rows
 // over the 4-bit rows themselves (quantized_decode.cu), fp32 and what else there is in fp32 arithmetic (quantized_rows.cu).  The layer's units enter as factors of the scores and of the output.
+#include <math.h>
 #include <string.h>
 
 #include "attention.cuh"
@@ -160,7 +161,6 @@ static_assert(32 * kMergeWarps >= TBL_MAX_ROTATED_DIM, "a thread per number");
 
 // ---- plan -------------------------------------------------------------------------------------------------------------------
 enum Route { kAuto = 0, kSimt = 1, kStream = 2, kFlash = 3 };
-constexpr int kFlashMinTokens = 48;
 
 int padded16(int n) { return static_cast<int>(round_up(n, 16)); }
 
@@ -171,9 +171,18 @@ tbl_attention_mixer as_attention(const tbl_quantized_mixer& m) {
     return a;
 }
 
-int pick_route(const tbl_quantized_mixer& m, int precision, int n_tok) {
+// bf16: the flash kernel where its time, worked out from what it took, is shorter than the streaming kernel's (32 query and 8 key/value heads of 128, in us, streaming and
+// flash kernel: one sequence of 64 tokens over 1024 20 and 43, over 16384 97 and 287; 256 over 4096 115 and 109; 512 over 512 58 and 45; eight sequences of 64 over
+// 4096 193 and 233, of 128 over 128 86 and 64, over 4096 372 and 244).  Both read or walk the context: the one for every block of 8 or 16 query rows, the other a wave of CTAs at a time.
+int pick_route(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context) {
     if (precision != TBL_BF16) return kSimt;
-    return n_tok >= kFlashMinTokens && attention_flash_supported(as_attention(m)) ? kFlash : kStream;
+    if (!attention_flash_supported(as_attention(m))) return kStream;
+    const double rows = static_cast<double>(n_seq) * n_tok, caches = static_cast<double>(n_seq) * m.kv_heads * quantized_width(m.dim) / 128;
+    const double seen = context - 0.5 * n_tok, group = m.heads / m.kv_heads;
+    const double blocks = ceil(n_tok * group / quantized_stream_rows(m, n_tok)), waves = ceil(n_seq * static_cast<double>(m.heads) * ceil_div(n_tok, 256) / kNumSm);
+    const double stream = 11 + 1.8e-3 * rows * m.heads + 42e-6 * caches * blocks * seen * (m.dim > 128 ? 0.7 : 1.0);
+    const double flash = 23 + 0.57e-3 * rows * (m.heads + 2 * m.kv_heads) + 250e-6 * caches * context + 0.014 * waves * seen;
+    return flash < stream ? kFlash : kStream;
 }
 
 struct Plan {
@@ -185,7 +194,7 @@ struct Plan {
 Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq, int n_tok, int context) {
     Plan w{};
     const size_t rows = static_cast<size_t>(n_seq) * n_tok, dp = padded16(m.dim);
-    w.route = route == kAuto ? pick_route(m, precision, n_tok) : route;
+    w.route = route == kAuto ? pick_route(m, precision, n_seq, n_tok, context) : route;
     w.splits = 1;
     bool parts = w.route == kFlash && !attention_flash_whole(as_attention(m));
     if (w.route == kStream) {

@@ -401,9 +401,14 @@ cudaError_t launch_plan(const QuantizedParams& p, const StreamPlan& plan, int ve
 
 }  // namespace
 
+int quantized_stream_rows(const tbl_quantized_mixer& m, int n_tok) {
+    const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
+    return rows_of(m.dim, static_cast<int>(total < 64 ? total : 64));
+}
+
 StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
-    const int rows = rows_of(m.dim, static_cast<int>(total < 64 ? total : 64));
+    const int rows = quantized_stream_rows(m, n_tok);
     const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows);
     StreamPlan w{4, 1, 0};
     const int tokens = ceil_div(context, 4 * kTile);             // a split is worth at least a tile of each warp
@@ -411,13 +416,17 @@ StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_
     if (s > tokens) s = tokens;
     if (s > 1024) s = 1024;
     w.splits = s < 1 ? 1 : static_cast<int>(s);
-    // Instead of splits, which another kernel has to join (some three tiles' time): one CTA of sixteen warps an SM.  Tiles that a warp takes one after the other:
+    // Instead of splits, whose sums another kernel joins: one CTA of sixteen warps an SM.  In the time of a tile (1.7 us with sixteen warps to an SM): what a warp takes
+    // one after the other, and 1.4 tiles for the other kernel, more with its blocks (a 64th for a unit up to 80) and splits (a 20th each).  One token of 32 and 8 heads,
+    // sixteen warps and splits: one sequence over 900 9.7 and 9.8 us, 2000 13.2 and 10.6, 8192 33.5 and 14.7; 8 over 2048 13.9 and 15.0, 4096 20.7 and 18.7;
+    // 18 over 4096 22 and 27; 30 over 4096 43 and 45.
     if (w.splits > 1 && m.dim <= 128) {
-        const double wide = ceil_div(context, 16 * kTile) * static_cast<double>(ceil_div(units, kNumSm)), split = ceil_div(context, 4LL * kTile * w.splits) + 3.0;
+        const double wide = ceil_div(context, 16 * kTile) * static_cast<double>(ceil_div(units, kNumSm));
+        const double split = ceil_div(context, 4LL * kTile * w.splits) + 1.4 + (units < 80 ? units : 80) / 64.0 + w.splits / 20.0;
         if (wide <= split) { w.warps = 16; w.splits = 1; }
     }
     // As a whole one launch less, but fewer CTAs to an SM, whose own chains before the first tile show once they take turns (64 sequences of 8 heads over 4096 tokens
-    // 95 and 83 us)
+    // 82 and 72 us, over 600 26 and 20, 37 over 4096 46 and 44)
     w.whole = n_tok == 1 && w.splits == 1 && total <= rows && units <= (w.warps == 16 ? 1 : 2) * kNumSm;
     return w;
 }

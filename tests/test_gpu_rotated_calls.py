@@ -116,7 +116,7 @@ def captured(torch, call, outs):
 
 
 # one token whole, one token of a long context (splits, or sixteen warps), several tokens, a portion, fp32
-@pytest.mark.parametrize("precision,route,n,before,size", [(1, 0, 1, 300, "plain"), (1, 0, 1, 3000, "plain"), (1, STREAM, 3, 3000, "group12"), (1, 0, 64, 300, "plain"),
+@pytest.mark.parametrize("precision,route,n,before,size", [(1, 0, 1, 300, "plain"), (1, 0, 1, 3000, "plain"), (1, STREAM, 3, 3000, "group12"), (1, 0, 64, 300, "plain"), (1, FLASH, 64, 300, "plain"),
                                                            (0, 0, 2, 900, "odd"), (1, 0, 1, 700, "wide")])
 def test_quantized_captured(cuda, stack_lib, precision, route, n, before, size):
     torch = cuda
