@@ -3,7 +3,7 @@
 // A CTA has up to 16 query rows that share a key/value head and a split of the context; each of its four warps takes tiles of 32 tokens by itself, with its own maxima,
 // sums and outputs.  For the scores a lane has a token and turns its codes into numbers sixteen at a time (one scale), for all rows at once; for the outputs a lane
 // has neighbouring dimensions, and the tokens' weights come from shared memory.  Cached numbers so are read as they lie, 4 bits each, once per 16 rows.
-// Bound by its multiplications, one for a number and row, and for few tokens by latency.
+// Bound by its multiplications, one for a number and row, and for few tokens by latency (five sequences of three tokens over 777: 22 us of the chain of one tile a warp).
 #include "quantized.cuh"
 
 namespace tbl {
@@ -139,7 +139,15 @@ __global__ void __launch_bounds__(kThreads) quantized_rows_kernel(const Quantize
     }
 }
 
-int rows_of(int width, long long total) { return total <= 4 ? 4 : total <= 8 || width > 128 ? 8 : 16; }
+// Query rows of a CTA.  Many of them share what a cached number costs; few of them are done sooner, where the CTAs at hand (`tiles`: splits at most, times sequences and
+// key/value heads) leave SMs empty (fp32, sixteen rows and as here: five sequences of three tokens over 777, 10 and 2 heads of 90, 28 and 22 us; four tokens over 300, 32 and 8
+// heads of 128, 27 and 17; 16 over 4000, 8 and 2 heads, 34 with sixteen rows, 36 with eight).
+int rows_of(int width, long long total, long long tiles) {
+    int r = total <= 4 ? 4 : total <= 8 || width > 128 ? 8 : 16;
+    while (r > 4 && tiles * ceil_div(total, r) < 3 * kNumSm / 2) r /= 2;
+    return r;
+}
+long long tiles_of(int n_seq, int kv_heads, int context) { return static_cast<long long>(n_seq) * kv_heads * ceil_div(context, kWarps * kTile); }
 
 template <typename T, int W, int R>
 cudaError_t launch(const QuantizedParams& p, int n_seq, cudaStream_t st) {
@@ -149,7 +157,7 @@ cudaError_t launch(const QuantizedParams& p, int n_seq, cudaStream_t st) {
 }
 template <typename T, int W>
 cudaError_t launch_rows(const QuantizedParams& p, int n_seq, cudaStream_t st) {
-    const int r = rows_of(p.width, static_cast<long long>(p.n_tok) * p.group);
+    const int r = rows_of(p.width, static_cast<long long>(p.n_tok) * p.group, tiles_of(n_seq, p.G, p.ctx));
     if constexpr (W <= 2) {
         if (r == 16) return launch<T, W, 16>(p, n_seq, st);
     }
@@ -169,7 +177,7 @@ cudaError_t launch_width(const QuantizedParams& p, int n_seq, cudaStream_t st) {
 
 int quantized_rows_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
-    const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows_of(quantized_width(m.dim), total));
+    const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows_of(quantized_width(m.dim), total, tiles_of(n_seq, m.kv_heads, context)));
     const int tokens = ceil_div(context, kWarps * kTile);        // a split is worth at least a tile of each warp
     long long s = 4LL * kNumSm / units;
     if (s > tokens) s = tokens;
