@@ -197,7 +197,9 @@ __device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
 // One CTA per (unit, chunk), two tiles of 64 tokens: D[value][key] = sum over a tile's tokens, M = 128 values (of which DP count), N = DP keys; both operands lie as they
 // come, a row per token.  Keys are divided by their power of two, values (times the decay to the chunk's end) by the tile's largest, both then brought up to 2^14, where
 // fp16 has room below: two terms hold 22 bits, three products 22 bits of the sums, which a tile has in columns of its own.  The keys' first terms and the values
-// go to decay_chunk_kernel on the way, as the tiles that it multiplies.  Bound by instructions, ten for a number; two CTAs to an SM.
+// go to decay_chunk_kernel on the way, as the tiles that it multiplies.  The second tile's rows are asked for as soon as the first one's registers are free.  Bound by the
+// way of the rows to the registers (35 % of the issue slots, 40 % of the stalls wait for loads); registers and tensor memory leave two CTAs to an SM.  64 chunks of 32 heads:
+// 149 us for 537 MB in and out, 3.6 TB/s.
 constexpr float kUp = 8192.0f;                           // 2^13: numbers below 2 end below 2^14
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkParams c) {
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
 }
 
 // ---- states before the chunks -----------------------------------------------------------------------------------------------------------
-// DP / 8 lanes share a row (a value's keys), eight neighbouring keys each.
+// DP / 8 lanes share a row (a value's keys), eight neighbouring keys each; the next eight chunks' sums are on their way.  64 chunks of 32 heads: 53 us for 201 MB.
 template <int DP>
 __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
     constexpr int kLph = DP / 8, kSide = 32 / kLph;
@@ -421,7 +423,8 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 // ---- outputs of the chunks ----------------------------------------------------------------------------------------------------------------
 // One CTA per (unit, chunk).  Scores Q K^T in the first 128 columns of its tensor memory, weights in their place (fp16, the A operand of the second product), the
 // tokens' part of the outputs behind them, then the state's part over the weights.  Keys and values come by bulk copies while the queries are normed, the state's operand
-// by another into the keys' room.  Outputs are collected in shared memory, so that gates are read and rows are written whole.
+// by another into the keys' room.  Outputs are collected in shared memory, so that gates are read and rows are written whole.  512 threads, since it is their loads and
+// barriers that take the time (43 % of the issue slots; with 256 threads 174 instead of 163 us): 64 chunks of 32 heads 156 us for 537 MB, 3.4 TB/s.
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
@@ -662,7 +665,7 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
 int width_of(int dim) { return dim <= 64 ? 64 : 128; }
 
 // Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes, and the two large kernels' last CTAs fill the GPU (8192
-// tokens of 32 heads: pieces of 9, 18, 37 and 64 chunks take 465, 440, 428 and 433 us, 39 chunks 436).
+// tokens of 32 heads: pieces of 9, 18, 37 and 64 chunks take 433, 414, 404 and 411 us, 39 chunks 418).
 constexpr size_t kPieceBytes = 352u << 20;
 int chunks_of(const tbl_decay_mixer& m, int n_seq, int n_tok) {
     const size_t units = static_cast<size_t>(n_seq) * m.heads, w = width_of(m.dim), wave = 2 * kNumSm;
