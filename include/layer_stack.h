@@ -266,7 +266,7 @@ int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int precision, 
  * rotary tables sets TBL_DEV_CACHE_FULL; the rows of its sequence are undefined, the cache holds what has room.  positions_dev is not
  * advanced, so that a repeated call writes the same rows again.  route: 0 as the step, 1 fp32 arithmetic on the 4-bit rows, 2 the
  * cache-streaming kernel (warp-level MMAs on the 4-bit rows), 3 the flash kernel (tcgen05) over expanded keys and values, as far as its
- * tiles have room (dim <= 192); 2 and 3 take bf16 only.  A number that is not finite reaches the rows that see its token, and may reach those of the same call and sequence before it. */
+ * tiles have room (dim <= 192); 2 and 3 take bf16 only.  With route 0 the workspace of a context serves every shorter one.  A number that is not finite reaches the rows that see its token, and may reach those of the same call and sequence before it. */
 int tbl_quantized_row_bytes(const tbl_quantized_mixer* mixer);
 size_t tbl_quantized_workspace_bytes(const tbl_quantized_mixer* mixer, int precision, int route, int n_seq, int n_tok, int context);
 int tbl_quantized_forward(const tbl_quantized_mixer* mixer, int precision, int route, float eps, const float* proj_dev, void* cache_dev,
@@ -281,7 +281,7 @@ int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const vo
  * (precision's type) [rows, heads*dim].  states_dev fp32 [slots][heads][dim][dim] are read, next_states_dev (the same array, or another of
  * its shape) receives those after the last token; slots_dev names distinct slots, the others are not touched.  A token past the rotary tables sets TBL_DEV_CACHE_FULL; the rows and
  * states of its sequence are undefined.  Projections are finite: a prompt is worked out in blocks, in which one that is not spoils other rows.  route: 0 as the step, 1 the scan kernel (any size, fp32
- * arithmetic), 2 the chunk kernels (tcgen05; bf16, dim <= 128). */
+ * arithmetic), 2 the chunk kernels (tcgen05; bf16, dim <= 128).  With route 0 the workspace of a number of tokens serves every smaller one. */
 size_t tbl_decay_workspace_bytes(const tbl_decay_mixer* mixer, int precision, int route, int n_seq, int n_tok);
 int tbl_decay_forward(const tbl_decay_mixer* mixer, int precision, int route, float eps, const float* proj_dev, const float* states_dev,
                       float* next_states_dev, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok, void* out_dev,

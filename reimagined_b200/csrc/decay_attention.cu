@@ -476,19 +476,16 @@ cudaError_t launch_scan(const DecayParams& p, cudaStream_t st) {
 }
 // Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; with segments the tokens are read twice, by more blocks.  Times in us: a
 // token 0.2 where a block has an SM to itself, 0.1 for each block where they share one, sums alone half of that; the other two launches 9.5.  Fewest of that wins (fp32,
-// without and with: three prompts of 301 tokens, 10 heads of 90, 71 and 54; 32 heads of 128, 64 tokens 23 and 28, 300 tokens 77 and 68).
+// without and with: three prompts of 301 tokens, 10 heads of 90, 71 and 54; 32 heads of 128, 64 tokens 22 and 28, 300 tokens 73 and 64).
 int scan_segments(int heads, int d, int n_seq, int n_tok) {
     const long long units = static_cast<long long>(n_seq) * heads;
     const int keys = keys_of(d), lanes = keys <= 32 ? 8 : keys <= 64 ? 16 : 32;
     const double share = static_cast<double>(units) * ceil_div(d, kScanThreads / 32 * (32 / lanes) * scan_rows(units, d)) / kNumSm;       // blocks to an SM
-    auto alone = [](double token, double shared) { return token > shared ? token : shared; };
-    int best = 1;
-    double least = n_tok * alone(0.2, 0.1 * share);
-    for (int s = 2; s <= kMostSegments && units <= 65535; ++s) {
-        const double t = 9.5 + round_up(ceil_div(n_tok, s), kTile) * (alone(0.2, 0.1 * share * s) + alone(0.1, 0.05 * share * s));
-        if (t <= 1.01 * least) { least = t; best = s; }
-    }
-    return best;
+    auto token = [&](int s) { return (0.1 * share * s > 0.2 ? 0.1 * share * s : 0.2) / s; };
+    int best = 2;
+    for (int s = 3; s <= kMostSegments; ++s)
+        if (token(s) <= 1.01 * token(best)) best = s;
+    return units <= 65535 && 9.5 + 1.5 * n_tok * token(best) < n_tok * token(1) ? best : 1;
 }
 
 enum Route { kAuto = 0, kScan = 1, kChunk = 2 };
@@ -519,6 +516,14 @@ Plan make_plan(const tbl_decay_mixer& m, int precision, int route, int n_seq, in
     return w;
 }
 
+// Bytes of a route.  Without one (0), room for whatever as many tokens or fewer take: a host may ask once for its longest portion.
+size_t bytes_of(const tbl_decay_mixer& m, int precision, int route, int n_seq, int n_tok) {
+    const Plan w = make_plan(m, precision, route, n_seq, n_tok);
+    if (route != kAuto || w.route != kChunk) return w.bytes;
+    const size_t scan = make_plan(m, precision, kScan, n_seq, chunk_min_tokens(static_cast<long long>(n_seq) * m.heads) - 1).bytes;
+    return w.bytes > scan ? w.bytes : scan;
+}
+
 }  // namespace
 
 int check_decay(const tbl_decay_mixer& m, int width) {
@@ -534,7 +539,7 @@ int check_decay(const tbl_decay_mixer& m, int width) {
 
 size_t decay_slot_bytes(const tbl_decay_mixer& m) { return sizeof(float) * static_cast<size_t>(m.heads) * m.dim * m.dim; }
 
-size_t decay_workspace(const tbl_decay_mixer& m, int precision, int n_seq, int n_tok) { return make_plan(m, precision, kAuto, n_seq, n_tok).bytes; }
+size_t decay_workspace(const tbl_decay_mixer& m, int precision, int n_seq, int n_tok) { return bytes_of(m, precision, kAuto, n_seq, n_tok); }
 
 int launch_decay(const tbl_decay_mixer& m, int precision, int route, float eps, const float* proj, const float* states, float* next, const int32_t* slots,
                  const int32_t* positions, int n_seq, int n_tok, void* out, void* ws, cudaStream_t st) {
@@ -577,7 +582,7 @@ size_t tbl_decay_workspace_bytes(const tbl_decay_mixer* mixer, int precision, in
     if (!mixer || (precision != TBL_F32 && precision != TBL_BF16) || route < kAuto || route > kChunk || n_seq <= 0 || n_tok <= 0 ||
         check_decay(*mixer, mixer->in.inputs) != TBL_OK)
         return 0;
-    return make_plan(*mixer, precision, route, n_seq, n_tok).bytes;
+    return bytes_of(*mixer, precision, route, n_seq, n_tok);
 }
 
 int tbl_decay_forward(const tbl_decay_mixer* mixer, int precision, int route, float eps, const float* proj_dev, const float* states_dev,

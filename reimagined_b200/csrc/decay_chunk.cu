@@ -667,18 +667,21 @@ int width_of(int dim) { return dim <= 64 ? 64 : 128; }
 // Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes, and the two large kernels' last CTAs fill the GPU (8192
 // tokens of 32 heads: pieces of 9, 18, 37 and 64 chunks take 433, 414, 404 and 411 us, 39 chunks 418).
 constexpr size_t kPieceBytes = 352u << 20;
+int most_chunks(const tbl_decay_mixer& m, int n_seq, int n_tok) {
+    const size_t w = width_of(m.dim), chunk = static_cast<size_t>(n_seq) * m.heads * (kTokens * (m.dim * 8 + w * 4) + w * w * 6), most = kPieceBytes / chunk;
+    const int all = ceil_div(n_tok, kTokens);
+    return most >= static_cast<size_t>(all) ? all : most ? static_cast<int>(most) : 1;
+}
 int chunks_of(const tbl_decay_mixer& m, int n_seq, int n_tok) {
-    const size_t units = static_cast<size_t>(n_seq) * m.heads, w = width_of(m.dim), wave = 2 * kNumSm;
-    const size_t chunk = units * (kTokens * (m.dim * 8 + w * 4) + w * w * 6);
-    const size_t all = ceil_div(n_tok, kTokens), most = kPieceBytes / chunk;
-    if (most >= all) return static_cast<int>(all);
-    const size_t full = units * most / wave * wave / units, n = full ? full : most;
-    return n ? static_cast<int>(n) : 1;
+    const int most = most_chunks(m, n_seq, n_tok);
+    if (most == ceil_div(n_tok, kTokens)) return most;
+    const size_t units = static_cast<size_t>(n_seq) * m.heads, wave = 2 * kNumSm, full = units * most / wave * wave / units;
+    return full ? static_cast<int>(full) : most;
 }
 
 struct Rooms { size_t sums, tokens, powers, images, scales, bytes; };
 Rooms rooms_of(const tbl_decay_mixer& m, int n_seq, int n_tok) {
-    const size_t w = width_of(m.dim), blocks = static_cast<size_t>(n_seq) * m.heads * chunks_of(m, n_seq, n_tok);
+    const size_t w = width_of(m.dim), blocks = static_cast<size_t>(n_seq) * m.heads * most_chunks(m, n_seq, n_tok);
     Rooms r{};
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 256); return at; };

@@ -118,6 +118,7 @@ __device__ __forceinline__ float query_power(const HeadUnits<V, 32>& x, float& f
 // quantized_decode.cu: streams the 4-bit rows for a few query rows
 struct StreamPlan {
     int warps, splits;           // of a CTA; of the context
+    int most;                    // splits that no shorter context passes (for workspaces)
     int whole;                   // one token of a sequence, no splits: the kernel norms, rounds, appends and finishes by itself
 };
 int quantized_stream_rows(const tbl_quantized_mixer& m, int n_tok);      // query rows of a CTA

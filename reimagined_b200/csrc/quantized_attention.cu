@@ -196,14 +196,16 @@ Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq
     const size_t rows = static_cast<size_t>(n_seq) * n_tok, dp = padded16(m.dim);
     w.route = route == kAuto ? pick_route(m, precision, n_seq, n_tok, context) : route;
     w.splits = 1;
+    int most = 1;                                                // splits to make room for
     bool parts = w.route == kFlash && !attention_flash_whole(as_attention(m));
     if (w.route == kStream) {
         w.stream = quantized_stream_plan(m, n_seq, n_tok, context);
         w.splits = w.stream.splits;
-        parts = w.splits > 1;
+        most = w.stream.most;
+        parts = most > 1;
     } else if (w.route == kSimt) {
-        w.splits = quantized_rows_splits(m, n_seq, n_tok, context);
-        parts = w.splits > 1;
+        w.splits = most = quantized_rows_splits(m, n_seq, n_tok, context);
+        parts = most > 1;
     }
     w.ctx = static_cast<int>(round_up(context, 128));            // whole blocks of the flash kernel
     size_t off = 0;
@@ -211,12 +213,22 @@ Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq
     w.q = take(w.route == kStream ? 2 * rows * m.heads * quantized_width(m.dim) : w.route == kFlash ? 2 * rows * m.heads * dp : 4 * rows * m.heads * m.dim);
     w.factor = take(w.route != kSimt ? sizeof(float) * rows * m.heads : 0);
     w.expanded = take(w.route == kFlash ? 2 * static_cast<size_t>(n_seq) * m.kv_heads * w.ctx * 2 * dp : 0);
-    const size_t units = rows * m.heads * w.splits;
+    const size_t units = rows * m.heads * most;
     w.pm = take(parts ? sizeof(float) * units : 0);
     w.pl = take(parts ? sizeof(float) * units : 0);
     w.po = take(parts ? sizeof(float) * units * dp : 0);
     w.bytes = off;
     return w;
+}
+
+// Bytes of a route.  Without one (0), room for whatever a context no longer than this one takes: a host may ask once for the longest.  (Both times in pick_route are
+// straight lines over the context, so the flash kernel is taken somewhere below only if it is at one end.)
+size_t bytes_of(const tbl_quantized_mixer& m, int precision, int route, int n_seq, int n_tok, int context) {
+    if (route != kAuto || precision != TBL_BF16) return make_plan(m, precision, route, n_seq, n_tok, context).bytes;
+    const size_t bytes = make_plan(m, precision, kStream, n_seq, n_tok, context).bytes;
+    if (pick_route(m, precision, n_seq, n_tok, n_tok) != kFlash && pick_route(m, precision, n_seq, n_tok, context) != kFlash) return bytes;
+    const size_t flash = make_plan(m, precision, kFlash, n_seq, n_tok, context).bytes;
+    return bytes > flash ? bytes : flash;
 }
 
 template <typename T, int V>
@@ -296,7 +308,7 @@ size_t quantized_slot_bytes(const tbl_quantized_mixer& m, int capacity) {
 }
 
 size_t quantized_workspace(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context) {
-    return make_plan(m, precision, kAuto, n_seq, n_tok, context).bytes;
+    return bytes_of(m, precision, kAuto, n_seq, n_tok, context);
 }
 
 int launch_quantized(const tbl_quantized_mixer& m, int precision, int route, float eps, const float* proj, void* cache, int capacity, const int32_t* slots,
@@ -331,7 +343,7 @@ size_t tbl_quantized_workspace_bytes(const tbl_quantized_mixer* mixer, int preci
     if (!mixer || (precision != TBL_F32 && precision != TBL_BF16) || route < kAuto || route > kFlash || n_seq <= 0 || n_tok <= 0 || context <= 0 ||
         check_quantized(*mixer, mixer->in.inputs) != TBL_OK)
         return 0;
-    return make_plan(*mixer, precision, route, n_seq, n_tok, context).bytes;
+    return bytes_of(*mixer, precision, route, n_seq, n_tok, context);
 }
 
 int tbl_quantized_forward(const tbl_quantized_mixer* mixer, int precision, int route, float eps, const float* proj_dev, void* cache_dev, int slots,

@@ -411,12 +411,12 @@ StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
     const int rows = quantized_stream_rows(m, n_tok);
     const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows);
-    StreamPlan w{4, 1, 0};
+    StreamPlan w{4, 1, 1, 0};
     const int tokens = ceil_div(context, 4 * kTile);             // a split is worth at least a tile of each warp
     long long s = 4LL * kNumSm / units;                          // four CTAs of four warps to an SM
     if (s > tokens) s = tokens;
     if (s > 1024) s = 1024;
-    w.splits = s < 1 ? 1 : static_cast<int>(s);
+    w.splits = w.most = s < 1 ? 1 : static_cast<int>(s);
     // Instead of splits, whose sums another kernel joins: one CTA of sixteen warps an SM.  In the time of a tile (1.7 us with sixteen warps to an SM): what a warp takes
     // one after the other, and 1.4 tiles for the other kernel, more with its blocks (a 64th for a unit up to 80) and splits (a 20th each).  One token of 32 and 8 heads,
     // sixteen warps and splits: one sequence over 900 9.7 and 9.8 us, 2000 13.2 and 10.6, 8192 33.5 and 14.7; 8 over 2048 13.9 and 15.0, 4096 20.7 and 18.7;

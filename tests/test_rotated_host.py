@@ -163,3 +163,20 @@ def test_state_of_these_layers(stack_lib):
     assert size(layer, 1) == size(layer, 0) == 256 + 3 * 4 * 32 * 32 * 4
     layer.decay.heads = 5
     assert size(layer, 1) == 0
+
+
+def test_a_workspace_for_the_longest_serves_shorter_calls(stack_lib):
+    """Whatever route a shorter context, or a shorter portion, takes."""
+    L = stack_lib
+    for heads, kv, dim in ((32, 8, 128), (8, 8, 64), (16, 1, 128), (12, 2, 192), (4, 2, 256)):
+        m = quantized(heads=heads, kv_heads=kv, dim=dim, rotation=rotated(rot_dim=dim))
+        for precision in (0, 1):
+            for n_seq, n_tok in ((1, 1), (9, 1), (150, 1), (1, 5), (3, 64), (8, 192), (1, 600)):
+                sizes = [L.tbl_quantized_workspace_bytes(C.byref(m), precision, 0, n_seq, n_tok, n_tok + extra) for extra in [*range(0, 3000, 37), 5000, 8000, 16000, 131000]]
+                assert sizes[0] > 0 and sizes == sorted(sizes), (heads, dim, precision, n_seq, n_tok)
+    for heads, dim in ((32, 128), (10, 90), (4, 64), (2, 256), (300, 64)):
+        m = decay(heads=heads, dim=dim, rotation=rotated(rot_dim=2))
+        for precision in (0, 1):
+            for n_seq in (1, 3, 40):
+                sizes = [L.tbl_decay_workspace_bytes(C.byref(m), precision, 0, n_seq, n) for n in [*range(1, 700), 1024, 4096, 4999, 5000, 5120, 8192]]
+                assert sizes[0] > 0 and sizes == sorted(sizes), (heads, dim, precision, n_seq)
