@@ -476,7 +476,7 @@ cudaError_t launch_scan(const DecayParams& p, cudaStream_t st) {
 }
 // Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; with segments the tokens are read twice, by more blocks.  Times in us: a
 // token 0.2 where a block has an SM to itself, 0.1 for each block where they share one, sums alone half of that; the other two launches 9.5.  Fewest of that wins (fp32,
-// without and with: three prompts of 301 tokens, 10 heads of 90, 71 and 54; 32 heads of 128, 64 tokens 22 and 28, 300 tokens 73 and 64).
+// without and with: three prompts of 301 tokens, 10 heads of 90, 75 and 54; 32 heads of 128, 64 tokens 22 and 28, 300 tokens 72 and 64; 8 heads, 2000 tokens 405 and 119).
 int scan_segments(int heads, int d, int n_seq, int n_tok) {
     const long long units = static_cast<long long>(n_seq) * heads;
     const int keys = keys_of(d), lanes = keys <= 32 ? 8 : keys <= 64 ? 16 : 32;

@@ -1,6 +1,6 @@
 """Time the layer-stack operators and models, each beside the like operator of the ternary hybrid at the same size.
 
-    python -m reimagined_b200.stack_shapes --width 4096 [--only dense,delta,latent,attention,norm,model] [--model guselix,goguvik]
+    python -m reimagined_b200.stack_shapes --width 4096 [--only dense,delta,latent,attention,turned,norm,model] [--model guselix,goguvik]
 
 One JSON line per record.  Every operator runs from a CUDA graph over several copies of its weights, states or caches, so
 that a call never finds them in L2.  `roofline` is the share of min(bytes / copy bandwidth, FLOPs / bf16 GEMM rate) that
@@ -231,6 +231,61 @@ def attention(n_seq: int, context: int, heads: int, dim: int) -> dict:
     return record("hybrid: attention step", us, cache, 4.0 * n_seq * context * kv, FP32_TFLOPS, sequences=n_seq, tokens=1, context=context, heads=heads)
 
 
+def _turned(dim: int, positions: int) -> capi.HeadRotation:
+    """Norms of ones, a rotation of all dimensions (what the tables hold costs nothing)."""
+    one, table = torch.ones(dim, device="cuda"), torch.ones(positions, dim // 2, device="cuda")
+    r = capi.HeadRotation(one.data_ptr(), one.data_ptr(), table.data_ptr(), table.data_ptr(), dim, positions, 0)
+    r.keep = one, table
+    return r
+
+
+def head_rotation(rows: int, heads: int, kv_heads: int, dim: int) -> dict:
+    L, cols = capi.stack_lib(), (heads + kv_heads) * dim
+    r, pos = _turned(dim, rows + 8), torch.zeros(1, dtype=torch.int32, device="cuda")
+    xs = [torch.randn(rows, cols, device="cuda") for _ in range(copies(4.0 * rows * cols, 8))]
+    q, k = (torch.empty(rows, n * dim, device="cuda", dtype=torch.bfloat16) for n in (heads, kv_heads))
+    us = time_calls([lambda a=a: check(L.tbl_head_rotation_forward(C.byref(r), capi.BF16, 1e-6, a.data_ptr(), cols, heads, kv_heads, dim, pos.data_ptr(), pos.data_ptr(),
+                                                                   1, rows, q.data_ptr(), k.data_ptr(), stream()), "tbl_head_rotation_forward") for a in xs])
+    return record("head norm + rotation", us, 6.0 * rows * cols, rows=rows, heads=heads, kv_heads=kv_heads, dim=dim)
+
+
+def quantized(n_seq: int, n_tok: int, context: int, heads: int, kv_heads: int, dim: int) -> dict:
+    """Attention over a 4-bit cache between its stacked projection and W_o: norm, rotation, append, attention, gate."""
+    L, rows, cols = capi.stack_lib(), n_seq * n_tok, 2 * (heads + kv_heads) * dim
+    some, r = bf16(1, 8), _turned(dim, context)
+    m = capi.QuantizedMixer(capi.DenseView(some.data_ptr(), None, 8, cols), capi.DenseView(some.data_ptr(), None, heads * dim, 8), r, heads, kv_heads, dim, 1, dim ** -0.5, 0.1, 0.1)
+    per_token = kv_heads * L.tbl_quantized_row_bytes(C.byref(m))
+    cache = 1.0 * n_seq * context * per_token
+    caches = [torch.randint(0, 120, (n_seq, context * per_token), dtype=torch.uint8, device="cuda") for _ in range(copies(cache, 16) if n_tok == 1 else 1)]
+    pos = torch.full((n_seq,), context - n_tok, dtype=torch.int32, device="cuda")
+    slots = torch.arange(n_seq, dtype=torch.int32, device="cuda")
+    proj, out = torch.randn(rows, cols, device="cuda"), torch.empty(rows, heads * dim, device="cuda", dtype=torch.bfloat16)
+    size = L.tbl_quantized_workspace_bytes(C.byref(m), capi.BF16, 0, n_seq, n_tok, context)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    us = time_calls([lambda c=c: check(L.tbl_quantized_forward(C.byref(m), capi.BF16, 0, 1e-6, proj.data_ptr(), c.data_ptr(), n_seq, context, slots.data_ptr(), pos.data_ptr(),
+                                                               n_seq, n_tok, context, out.data_ptr(), ws.data_ptr(), size, stream()),
+                                       "tbl_quantized_forward") for c in caches], 16 if n_tok <= 8 else 4)
+    pairs = n_seq * sum(range(context - n_tok + 1, context + 1))
+    return record("4-bit attention", us, cache + 4.0 * rows * cols + 2.0 * rows * heads * dim, 4.0 * heads * pairs * dim, sequences=n_seq, tokens=n_tok, context=context,
+                  heads=heads, kv_heads=kv_heads)
+
+
+def decay(n_seq: int, n_tok: int, heads: int, dim: int) -> dict:
+    """Linear attention with decay between its stacked projection and W_o: norm, rotation, recurrence, head norm, gate."""
+    L, rows, cols = capi.stack_lib(), n_seq * n_tok, 4 * heads * dim
+    some, r, rates, norm = bf16(1, 8), _turned(dim, n_tok + 8), torch.full((heads,), -0.01, device="cuda"), torch.ones(heads * dim, device="cuda")
+    m = capi.DecayMixer(capi.DenseView(some.data_ptr(), None, 8, cols), capi.DenseView(some.data_ptr(), None, heads * dim, 8), r, rates.data_ptr(), norm.data_ptr(), heads, dim, 1,
+                        dim ** -0.5)
+    states = [torch.zeros(n_seq, heads, dim, dim, device="cuda") for _ in range(copies(8.0 * n_seq * heads * dim * dim, 16) if n_tok == 1 else 1)]
+    pos, slots = torch.zeros(n_seq, dtype=torch.int32, device="cuda"), torch.arange(n_seq, dtype=torch.int32, device="cuda")
+    proj, out = torch.randn(rows, cols, device="cuda"), torch.empty(rows, heads * dim, device="cuda", dtype=torch.bfloat16)
+    size = L.tbl_decay_workspace_bytes(C.byref(m), capi.BF16, 0, n_seq, n_tok)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    us = time_calls([lambda c=c: check(L.tbl_decay_forward(C.byref(m), capi.BF16, 0, 1e-6, proj.data_ptr(), c.data_ptr(), c.data_ptr(), slots.data_ptr(), pos.data_ptr(), n_seq,
+                                                           n_tok, out.data_ptr(), ws.data_ptr(), size, stream()), "tbl_decay_forward") for c in states], 16 if n_tok <= 8 else 4)
+    return record("decay attention", us, 8.0 * n_seq * heads * dim * dim + 4.0 * rows * cols + 2.0 * rows * heads * dim, sequences=n_seq, tokens=n_tok, heads=heads)
+
+
 # ---- norms --------------------------------------------------------------------------------------------------------------------
 def depth(rows: int, width: int, count: int) -> dict:
     L = capi.stack_lib()
@@ -353,7 +408,7 @@ def time_hybrid(width: int, layers: int, batches=(1, 8, 64), context: int = 512,
     return out
 
 
-def operators(width: int, only=("dense", "delta", "latent", "attention", "norm")):
+def operators(width: int, only=("dense", "delta", "latent", "attention", "turned", "norm")):
     """Generator of records at one model width."""
     heads, ff = width // 128, 3 * width
     if "dense" in only:
@@ -386,6 +441,16 @@ def operators(width: int, only=("dense", "delta", "latent", "attention", "norm")
                 yield attention(n_seq, context, heads, 128)
         for n_tok in (512, 2048, 8192):
             yield differential(1, n_tok, n_tok, heads, max(1, heads // 4))
+    if "turned" in only:
+        for rows in (1, 64, 8192):
+            yield head_rotation(rows, heads, max(1, heads // 4), 128)
+        for n_seq, context in ((1, 1024), (1, 8192), (8, 8192), (64, 4096)):
+            yield quantized(n_seq, 1, context, heads, max(1, heads // 4), 128)
+        for n_seq in (1, 8, 64):
+            yield decay(n_seq, 1, heads, 128)
+        for n_tok in (512, 2048, 8192):
+            yield quantized(1, n_tok, n_tok, heads, max(1, heads // 4), 128)
+            yield decay(1, n_tok, heads, 128)
     if "norm" in only:
         for rows in (1, 64, 8192):
             yield streams(rows, width, 2)
@@ -398,7 +463,7 @@ def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--width", type=int, default=4096)
     ap.add_argument("--layers", type=int, default=4, help="layers of the whole-model timings")
-    ap.add_argument("--only", default="dense,delta,latent,attention,norm,model")
+    ap.add_argument("--only", default="dense,delta,latent,attention,turned,norm,model")
     ap.add_argument("--model", default="guselix,goguvik", help="layer-stack models of the whole-model timings")
     args = ap.parse_args()
     use_measured_peaks()
