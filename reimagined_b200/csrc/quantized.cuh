@@ -126,6 +126,7 @@ StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_
 int launch_quantized_stream(const QuantizedParams& p, const StreamPlan& plan, int vec, int n_seq, cudaStream_t st);
 
 // quantized_rows.cu: the same in fp32 arithmetic, any number of rows
+long long quantized_rows_blocks(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);     // of query rows
 int quantized_rows_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context);
 int launch_quantized_rows(const QuantizedParams& p, int precision, int n_seq, cudaStream_t st);
 

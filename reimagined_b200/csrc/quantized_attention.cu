@@ -316,6 +316,9 @@ int launch_quantized(const tbl_quantized_mixer& m, int precision, int route, flo
     const Plan w = make_plan(m, precision, route, n_seq, n_tok, context);
     const long long rows = static_cast<long long>(n_seq) * n_tok;
     if (rows > 2147483647LL || static_cast<long long>(n_seq) * m.kv_heads > 65535 || ceil_div(m.heads + 2 * m.kv_heads, kPrepWarps) > 65535 || w.splits > 65535) return TBL_ERR_SHAPE;
+    // blocks of query rows are one side of a grid
+    const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads), stream_rows = quantized_stream_rows(m, n_tok);
+    if ((w.route == kStream && (total + stream_rows - 1) / stream_rows > 65535) || (w.route == kSimt && quantized_rows_blocks(m, n_seq, n_tok, context) > 65535)) return TBL_ERR_SHAPE;
     QuantizedParams p = basic_params(m, capacity, slots, positions, n_tok);
     if (!p.status) return TBL_ERR_CUDA;
     uint8_t* base = static_cast<uint8_t*>(ws);

@@ -175,9 +175,13 @@ cudaError_t launch_width(const QuantizedParams& p, int n_seq, cudaStream_t st) {
 
 }  // namespace
 
-int quantized_rows_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
+long long quantized_rows_blocks(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads);
-    const long long units = static_cast<long long>(n_seq) * m.kv_heads * ceil_div(total, rows_of(quantized_width(m.dim), total, tiles_of(n_seq, m.kv_heads, context)));
+    const int rows = rows_of(quantized_width(m.dim), total, tiles_of(n_seq, m.kv_heads, context));
+    return (total + rows - 1) / rows;
+}
+int quantized_rows_splits(const tbl_quantized_mixer& m, int n_seq, int n_tok, int context) {
+    const long long units = static_cast<long long>(n_seq) * m.kv_heads * quantized_rows_blocks(m, n_seq, n_tok, context);
     const int tokens = ceil_div(context, kWarps * kTile);        // a split is worth at least a tile of each warp
     long long s = 4LL * kNumSm / units;
     if (s > tokens) s = tokens;

@@ -180,3 +180,11 @@ def test_a_workspace_for_the_longest_serves_shorter_calls(stack_lib):
             for n_seq in (1, 3, 40):
                 sizes = [L.tbl_decay_workspace_bytes(C.byref(m), precision, 0, n_seq, n) for n in [*range(1, 700), 1024, 4096, 4999, 5000, 5120, 8192]]
                 assert sizes[0] > 0 and sizes == sorted(sizes), (heads, dim, precision, n_seq)
+
+
+def test_more_query_rows_than_a_grid_has(stack_lib):
+    """65536 blocks of sixteen rows: refused before anything is appended."""
+    before, n, m = stack_lib.tbl_launch_count(), 4 << 16, quantized(heads=4, kv_heads=1)
+    for precision, route in ((0, 0), (0, 1), (1, 1), (1, 2)):
+        assert stack_lib.tbl_quantized_forward(C.byref(m), precision, route, 1e-5, 4096, 4096, 2, n, 4096, 4096, 1, n, n, 4096, 4096, 1 << 60, None) == -2
+    assert stack_lib.tbl_launch_count() == before
