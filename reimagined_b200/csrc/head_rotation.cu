@@ -2,7 +2,6 @@
 // the angle of the row's position.  Bound by memory: every number is read once (4 bytes) and written once.  A CTA takes a row at a time, so that a thread reads
 // the row's angles once for all its heads; a head lies in registers of 8, 16 or 32 lanes between the sum of squares and the stores.
 // 8192 rows of 32 + 8 heads of 128, bf16: 50 us for 252 MB, 5.0 TB/s.
-#include <string.h>
 
 #include "head_rotation.cuh"
 

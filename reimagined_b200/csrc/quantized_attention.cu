@@ -6,7 +6,6 @@
 // Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, and weights need one term instead of two), a few query rows
 // over the 4-bit rows themselves (quantized_decode.cu), fp32 and what else there is in fp32 arithmetic (quantized_rows.cu).  The layer's units enter as factors of the scores and of the output.
 #include <math.h>
-#include <string.h>
 
 #include "attention.cuh"
 #include "quantized.cuh"
