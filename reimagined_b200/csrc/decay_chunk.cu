@@ -11,8 +11,8 @@
 //
 // Precision.  The states are sums over the whole sequence and stay fp32: their products take both operands as two fp16 terms each (22 bits, three products; numbers
 // 2^-14 below a tile's largest keep fewer).  Outputs are rounded to bf16, so their operands are single fp16 terms under a power of two for every token, and for every
-// row of a state (errors of 2^-12; a weight carries the factors of its key and value beside the largest of the chunk, which only costs numbers 2^-14
-// below that their last bits).
+// row of a state (errors of 2^-12).  A weight y^(i-j) (q_i . k_j) carries the factors of its key and value beside the largest that the row sees, decay included: a
+// token that a row does not see, or has forgotten, takes no bits from it.
 #include <cuda_fp16.h>
 
 #include "decay.cuh"
@@ -117,6 +117,9 @@ __device__ __forceinline__ float lanes_max(float v) {
     for (int o = LPH / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// The power of two at or below a head's largest number, 2^-113 at least (also for a head of zeros, which so counts less than any other); times kUp its inverse
+// is a number.
+__device__ __forceinline__ float power_of(float most) { return power_below(fmaxf(most, 0x1p-113f)); }
 // one over a power of two
 __device__ __forceinline__ float inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ float largest(const float (&x)[8]) {
@@ -200,7 +203,7 @@ __device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
 // go to decay_chunk_kernel on the way, as the tiles that it multiplies.  The second tile's rows are asked for as soon as the first one's registers are free.  Bound by the
 // way of the rows to the registers (35 % of the issue slots, 40 % of the stalls wait for loads); registers and tensor memory leave two CTAs to an SM.  64 chunks of 32 heads:
 // 149 us for 537 MB in and out, 3.6 TB/s.
-constexpr float kUp = 8192.0f;                           // 2^13: numbers below 2 end below 2^14
+constexpr float kUp = 8192.0f, kUpBits = 13.0f;          // numbers below 2 end below 2^14
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
@@ -235,12 +238,9 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
     const Lane kl(p.r, gl, group), vl(Rotation{nullptr, nullptr, 0, 0, 0}, gl, group);
     const float* base = p.proj + a.row0 * p.ld + a.head * p.d;
     if (p.r.half > 0 && tid == 0 && (a.pos0 < 0 || a.pos0 + a.n > p.r.positions)) atomicOr(p.status, TBL_DEV_CACHE_FULL);
-    float w[8], bound = 1.0f;
+    float w[8];
     const bool normed = p.k_norm != nullptr;
-    if (normed) {
-        kl.load(p.k_norm, p.d, w);
-        bound = bound_of<Lane::kLph>(w, p.d);
-    }
+    if (normed) kl.load(p.k_norm, p.d, w);
     uint8_t* keys = c.tokens + a.at * 2 * kTile;
     float* powers = c.powers + a.at * 2 * kTokens;
     __syncthreads();
@@ -256,25 +256,22 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
     }
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
-        float inv[kRounds], up[kRounds], most = 0.0f;
+        float power[kRounds], most = 0.0f;               // power: of two, of a token's key
         const int j0 = tile * 64 + warp * kPerWarp + group;
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
             const int j = j0 + i * Lane::kSide;
-            float cs[4], sn[4], power = bound;
+            float cs[4], sn[4];
             kl.angles(p.r, gl, table_row(p, a.pos0 + min(j, a.n - 1)), cs, sn);
-            inv[i] = 1.0f;
             if (normed) {
-                inv[i] = rsqrtf(lanes_sum<Lane::kLph>(squares(k[i])) * c.per_dim + p.eps);
+                const float f = rsqrtf(lanes_sum<Lane::kLph>(squares(k[i])) * c.per_dim + p.eps);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) k[i][e] *= w[e];
+                for (int e = 0; e < 8; ++e) k[i][e] *= w[e] * f;
             }
             kl.turn(p.r.interleaved != 0, cs, sn, k[i]);
-            if (!normed) power = power_below(lanes_max<Lane::kLph>(largest(k[i])));
-            const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_below(v_most);
-            inv[i] = j < a.n ? inv[i] * inverse_power(power) * kUp : 0.0f;
-            up[i] = weight_s[j] * power;
-            most = fmaxf(most, v_most * up[i]);
+            power[i] = power_of(lanes_max<Lane::kLph>(largest(k[i])));
+            const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_of(v_most);
+            most = fmaxf(most, v_most * (weight_s[j] * power[i]));
             // the values as they are, for the products inside the chunk
             const float f = j < a.n ? inverse_power(v_power) : 0.0f;
 #pragma unroll
@@ -284,7 +281,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
                 for (int e = 0; e < V; ++e) y[e] = v[i][V * u + e] * f;
                 if (vl.at[u] < DP) put_halves<V>(keys + kTile + vl.place(u, tile * 64 + warp * kPerWarp, i, group, kSub), y);
             }
-            if (gl == 0) { powers[j] = power; powers[kTokens + j] = v_power; }
+            if (gl == 0) { powers[j] = power[i]; powers[kTokens + j] = v_power; }
         }
         most = warp_max(most);
         if (lane == 0) most_s[tile][warp] = most;
@@ -296,12 +293,13 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
         back[tile] = top * (1.0f / (kUp * kUp));
 #pragma unroll
         for (int i = 0; i < kRounds; ++i) {
-            const float f = up[i] * down;
+            const int j = j0 + i * Lane::kSide;
+            const float inv = j < a.n ? inverse_power(power[i]) * kUp : 0.0f, f = weight_s[j] * power[i] * down;
 #pragma unroll
             for (int u = 0; u < kRuns; ++u) {
                 float y[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = k[i][V * u + e] * inv[i];
+                for (int e = 0; e < V; ++e) y[e] = k[i][V * u + e] * inv;
                 if (kl.at[u] < DP)
                     put_terms<V>(k_s + kl.place(u, warp * kPerWarp, i, group, kBox), kPiece, y, keys + kl.place(u, tile * 64 + warp * kPerWarp, i, group, kSub));
 #pragma unroll
@@ -432,8 +430,8 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
     constexpr int kRounds = kPerWarp / Lane::kSide, kFlight = kRounds < 2 ? kRounds : 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(16) float kv_f[kTokens], scale_s[DP];
-    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[4][kTokens], most_s;       // power_s: y^n
+    __shared__ __align__(16) float kv_e[kTokens], most_e[kTokens], scale_s[DP];          // exponents: of a token's key and value, the largest that a row sees
+    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[4][kTokens];               // power_s: y^n
     __shared__ __align__(8) uint64_t bars[4];            // keys and values, scores, state's image, outputs
     __shared__ uint32_t tmem_slot;
     uint8_t *q_s = smem, *k_s = smem + kTile, *v_s = smem + 2 * kTile;
@@ -519,21 +517,34 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
             umma_commit(&bars[1]);
         }
         __syncwarp();
-    } else if (warp == 1) {                              // the largest factor of a token's key and value together
+    } else if (warp == 1) {
+        // Exponents (the product of two powers of two may pass the ends of fp32): e_j of a token's key and value together, and for row i the largest e_j + (i - j) log2 y
+        // of the tokens j <= i.  A lane has four neighbouring tokens, lanes meet in a scan.
         const float* powers = c.powers + a.at * 2 * kTokens;
-        float f[kTokens / 32], most = 0.0f;
+        const float4 k = reinterpret_cast<const float4*>(powers)[lane], v = reinterpret_cast<const float4*>(powers + kTokens)[lane];
+        const float step = rate * 1.44269504f;
+        auto exponent = [&](int i, float x, float y) {
+            return 4 * lane + i < a.n ? static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) + static_cast<int>(__float_as_uint(y) >> 23) - 254) : -INFINITY;
+        };
+        const float e[4] = {exponent(0, k.x, v.x), exponent(1, k.y, v.y), exponent(2, k.z, v.z), exponent(3, k.w, v.w)};
+        float m[4];
+        m[0] = e[0];
 #pragma unroll
-        for (int i = 0; i < kTokens / 32; ++i) {
-            const int j = lane + 32 * i;
-            // (as exponents: the product of two powers of two may pass the ends of fp32)
-            f[i] = static_cast<float>(static_cast<int>(__float_as_uint(powers[j]) >> 23) + static_cast<int>(__float_as_uint(powers[kTokens + j]) >> 23));
-            if (j >= a.n) f[i] = 0.0f;
-            most = fmaxf(most, f[i]);
+        for (int i = 1; i < 4; ++i) m[i] = fmaxf(e[i], m[i - 1] + step);
+        float last = m[3];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float before = __shfl_up_sync(0xffffffffu, last, o);
+            if (lane >= o) last = fmaxf(last, before + step * static_cast<float>(4 * o));
         }
-        most = warp_max(most);
+        float before = __shfl_up_sync(0xffffffffu, last, 1);
 #pragma unroll
-        for (int i = 0; i < kTokens / 32; ++i) kv_f[lane + 32 * i] = exp2f(f[i] - most) * (1.0f / kUp);     // (keys come brought up by kUp)
-        if (lane == 0) most_s = most - 254.0f;
+        for (int i = 0; i < 4; ++i) {                    // (whole exponents, so that a factor and its inverse are exact)
+            before += step;
+            m[i] = ceilf(lane ? fmaxf(m[i], before) : m[i]);
+        }
+        reinterpret_cast<float4*>(kv_e)[lane] = make_float4(e[0], e[1], e[2], e[3]);
+        reinterpret_cast<float4*>(most_e)[lane] = make_float4(m[0], m[1], m[2], m[3]);
     }
     __syncthreads();
     alive = mbar_wait_bounded(&bars[1], 0, p.status);
@@ -554,10 +565,12 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
         } else {
             tmem_ld32(tmem + lanes + ch * 32, x);
             tmem_ld_wait();
-            const float* power = power_s + (row - ch * 32);
+            const float *power = power_s + (row - ch * 32), most = most_e[row] + kUpBits;      // (keys come brought up by kUp)
+            // (a factor past 2^126 stands beside a power that is zero)
+            auto factor = [&](float e) { return ex2(fminf(e - most, 126.0f)); };
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(kv_f + ch * 32 + e);
+                const float4 f = *reinterpret_cast<const float4*>(kv_e + ch * 32 + e);
                 float w[4];
                 if (ch == (warp & 3)) {
 #pragma unroll
@@ -566,7 +579,7 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = __uint_as_float(x[e + k]) * power[-(e + k)];
                 }
-                const __half2 h0 = __floats2half2_rn(w[0] * f.x, w[1] * f.y), h1 = __floats2half2_rn(w[2] * f.z, w[3] * f.w);
+                const __half2 h0 = __floats2half2_rn(w[0] * factor(f.x), w[1] * factor(f.y)), h1 = __floats2half2_rn(w[2] * factor(f.z), w[3] * factor(f.w));
                 y[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
                 y[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
             }
@@ -591,7 +604,7 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     // the sums of squares of a row's fourths meet in shared memory
-    const float f = q_f[row] * p.scale, inside = f * exp2f(most_s), before = f * power_s[min(row + 1, kTokens)];
+    const float f = q_f[row] * p.scale, inside = f * exp2f(most_e[row]), before = f * power_s[min(row + 1, kTokens)];
     float ss = 0.0f;
 #pragma unroll 1
     for (int q = 0; q < DP / 64; ++q) {

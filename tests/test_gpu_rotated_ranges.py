@@ -1,0 +1,95 @@
+"""Normed and rotated heads, 4-bit cache, decay attention: numbers of very different sizes side by side.  Every row is held to its own size.
+
+Tolerances.  A bf16 result is rounded by half a step, 2^-8 of it at most; fp16 operands by 2^-12 of themselves (standard deviation 2^-12 / sqrt(3)), at random."""
+import numpy as np
+import pytest
+
+from rotated_helpers import Decay, f64, stream
+from test_gpu_rotated_mixers import CHUNK, cfgd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built(cuda, stack_lib):
+    stack_lib.tbl_device_status(stream(cuda))
+    yield
+    assert stack_lib.tbl_device_status(stream(cuda)) == 0
+
+
+def own_rows_close(got, want, tol, what):
+    err = np.sqrt(((got - want) ** 2).mean(axis=1)) / np.sqrt((want ** 2).mean(axis=1))
+    worst = int((err / tol).argmax())
+    assert np.isfinite(got).all() and (err < tol).all(), (what, worst, err[worst], np.broadcast_to(tol, err.shape)[worst])
+
+
+def chunk_tolerance(a, proj):
+    """What operands of fp16 may do to the rows of a prompt from an empty state: four standard deviations, and the result's rounding.  A weight
+    y^(i-j) (q . k) has the errors of q and k, which meet in sqrt(sum q^2 k^2), and its own; a value has one more."""
+    q, k, v, _ = a.heads(proj, 0)
+    age = np.arange(len(proj))[:, None] - np.arange(len(proj))[None]
+    errors, sizes = 0.0, 0.0
+    for h in range(a.H):
+        with np.errstate(invalid="ignore"):
+            keep = np.where(age >= 0, np.where(age == 0, 1.0, np.exp(np.maximum(age, 1) * float(a.rates[h]))), 0.0)
+        s, mag = q[:, h] @ k[:, h].T, np.sqrt((q[:, h] ** 2) @ (k[:, h] ** 2).T)
+        scale = float(np.float32(a.cfg["scale"]))
+        o = scale * (keep * s) @ v[:, h]
+        err = 2.0 ** -12 * np.sqrt(2 / 3) * scale * np.sqrt((keep ** 2 * (mag ** 2 + s ** 2)) @ (v[:, h] ** 2).mean(axis=1))
+        size = np.sqrt((o ** 2).mean(axis=1))
+        f = 1 / np.sqrt(size ** 2 + a.eps) if a.norm is not None else 1.0
+        errors, sizes = errors + (f * err) ** 2, sizes + (f * size) ** 2
+    return 2.0 ** -8 + 4 * np.sqrt(errors / sizes)
+
+
+def states_near(a, slot):
+    """fp32 sums (see states_close), every head beside its own largest number."""
+    got, want, n = f64(a.states[slot]), a.memory[slot]["S"], a.memory[slot]["at"]
+    for h in range(a.H):
+        assert np.abs(got[h] - want[h]).max() <= 5 * np.sqrt(2 * n / 12) * 2.0 ** -23 * np.abs(want[h]).max(), h
+
+
+def parts(a, proj):
+    """Columns of keys and of values."""
+    n = a.H * a.d
+    return proj[:, n:2 * n], proj[:, 2 * n:3 * n]
+
+
+RATES = [-0.01, -0.5, 0.0, -20.0]
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("head_norm", [True, False])
+@pytest.mark.parametrize("n,at,power,dim", [(128, 127, 20, 128), (200, 199, 24, 64), (200, 40, 24, 90), (128, 64, 20, 128)])
+def test_decay_rows_that_do_not_see_a_large_token(cuda, stack_lib, norm, head_norm, n, at, power, dim):
+    """A token whose value is 2^20 times the others' reaches the rows behind it, as long as they remember it, and no others."""
+    a = Decay(cuda, stack_lib, cfgd(4, dim, 44, 0.1, gated=False, norm=norm), 1, norm=head_norm, rates=RATES)
+    proj = np.random.default_rng(n + at).standard_normal((n, a.cols)).astype(np.float32)
+    parts(a, proj)[1][at] *= 2.0 ** power
+    if not norm:
+        parts(a, proj)[0][at] *= 2.0 ** 6
+    tol, want = chunk_tolerance(a, proj), a.oracle([1], proj)
+    own_rows_close(a.forward(CHUNK, [1], proj), want, tol, "rows")
+    states_near(a, 1)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("power", [-16, -20, -30])
+def test_decay_tokens_of_zeros_among_small_ones(cuda, stack_lib, norm, power):
+    """Rows of zeros (padding, say) change nothing for the others, however small those are."""
+    a = Decay(cuda, stack_lib, cfgd(4, 128, 64, 0.1, gated=False, norm=norm), 1, norm=False, rates=RATES)
+    proj = np.random.default_rng(-power).standard_normal((200, a.cols)).astype(np.float32)
+    parts(a, proj)[1][:] *= 2.0 ** power
+    if not norm:
+        parts(a, proj)[0][:] *= 2.0 ** power
+    proj[[3, 70, 150]] = 0
+    proj[[5, 71], :] *= np.float32(1e-3)
+    parts(a, proj)[0][90] = 0                                   # a key alone
+    parts(a, proj)[1][160] = 0                                  # a value alone
+    rows = np.setdiff1d(np.arange(200), [3, 70, 150])           # (no query: zeros)
+    with np.errstate(invalid="ignore"):
+        tol, want = chunk_tolerance(a, proj)[rows], a.oracle([1], proj)
+    got = a.forward(CHUNK, [1], proj)
+    own_rows_close(got[rows], want[rows], tol, "rows")
+    assert (got[[3, 70, 150]] == 0).all()
+    states_near(a, 1)
