@@ -11,7 +11,7 @@
 //
 // Precision.  The states are sums over the whole sequence and stay fp32: their products take both operands as two fp16 terms each (22 bits, three products; numbers
 // 2^-14 below a tile's largest keep fewer).  Outputs are rounded to bf16, so their operands are single fp16 terms under a power of two for every token, and for every
-// row of a state (errors of 2^-12).  A weight y^(i-j) (q_i . k_j) carries the factors of its key and value beside the largest that the row sees, decay included: a
+// row of a state: errors of 2^-12.  They are brought up to 2^14, so that numbers down to 2^-28 of the largest beside them keep their bits.  A weight y^(i-j) (q_i . k_j) carries the factors of its key and value, and is an fp16 beside the largest weight of its row: a
 // token that a row does not see, or has forgotten, takes no bits from it.
 #include <cuda_fp16.h>
 
@@ -190,12 +190,6 @@ __device__ __forceinline__ void fetch_ahead(const ChunkParams& c, int column0, i
 
 __device__ __forceinline__ int table_row(const DecayParams& p, int pos) { return p.r.half > 0 ? min(max(pos, 0), p.r.positions - 1) : 0; }
 
-// the power of two that a normed head's numbers are divided by: sqrt(d) times the largest weight bounds them
-template <int LPH>
-__device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
-    return power_below(sqrtf(static_cast<float>(dim)) * lanes_max<LPH>(largest(w)));
-}
-
 // ---- sums of the chunks -----------------------------------------------------------------------------------------------------------------
 // One CTA per (unit, chunk), two tiles of 64 tokens: D[value][key] = sum over a tile's tokens, M = 128 values (of which DP count), N = DP keys; both operands lie as they
 // come, a row per token.  Keys are divided by their power of two, values (times the decay to the chunk's end) by the tile's largest, both then brought up to 2^14, where
@@ -204,6 +198,7 @@ __device__ __forceinline__ float bound_of(const float (&w)[8], int dim) {
 // way of the rows to the registers (35 % of the issue slots, 40 % of the stalls wait for loads); registers and tensor memory leave two CTAs to an SM.  64 chunks of 32 heads:
 // 149 us for 537 MB in and out, 3.6 TB/s.
 constexpr float kUp = 8192.0f, kUpBits = 13.0f;          // numbers below 2 end below 2^14
+constexpr float kHighest = 60.0f;                        // (a score of two such heads ends below 2^35)
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
@@ -273,7 +268,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
             const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_of(v_most);
             most = fmaxf(most, v_most * (weight_s[j] * power[i]));
             // the values as they are, for the products inside the chunk
-            const float f = j < a.n ? inverse_power(v_power) : 0.0f;
+            const float f = j < a.n ? inverse_power(v_power) * kUp : 0.0f;
 #pragma unroll
             for (int u = 0; u < kRuns; ++u) {
                 float y[V];
@@ -392,7 +387,7 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[e]));
             most = lanes_max<kLph>(most);
-            const float power = power_below(most), inv = inverse_power(power);
+            const float power = power_of(most), inv = inverse_power(power) * kUp;
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -430,8 +425,8 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
     constexpr int kRounds = kPerWarp / Lane::kSide, kFlight = kRounds < 2 ? kRounds : 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(16) float kv_e[kTokens], most_e[kTokens], scale_s[DP];          // exponents: of a token's key and value, the largest that a row sees
-    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[4][kTokens];               // power_s: y^n
+    __shared__ __align__(16) float kv_f[kTokens], scale_s[DP];
+    __shared__ float power_s[kTokens + 1], q_f[kTokens], ss_s[4][kTokens], most_s;       // power_s: y^n; ss_s: first the weights' maxima, then sums of squares
     __shared__ __align__(8) uint64_t bars[4];            // keys and values, scores, state's image, outputs
     __shared__ uint32_t tmem_slot;
     uint8_t *q_s = smem, *k_s = smem + kTile, *v_s = smem + 2 * kTile;
@@ -467,12 +462,9 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
     const float* base = p.proj + a.row0 * p.ld + a.head * p.d;
     {
         const Lane ql(p.r, gl, group);
-        float w[8], bound = 1.0f;
+        float w[8];
         const bool normed = p.q_norm != nullptr;
-        if (normed) {
-            ql.load(p.q_norm, p.d, w);
-            bound = bound_of<Lane::kLph>(w, p.d);
-        }
+        if (normed) ql.load(p.q_norm, p.d, w);
 #pragma unroll 1
         for (int i0 = 0; i0 < kRounds; i0 += kFlight) {
             float x[kFlight][8];
@@ -486,15 +478,13 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
                 const int j = warp * kPerWarp + (i0 + i) * Lane::kSide + group;
                 float cs[4], sn[4];
                 ql.angles(p.r, gl, table_row(p, a.pos0 + min(j, a.n - 1)), cs, sn);
-                float inv = 1.0f, power = bound;
                 if (normed) {
-                    inv = rsqrtf(lanes_sum<Lane::kLph>(squares(x[i])) * c.per_dim + p.eps);
+                    const float inv = rsqrtf(lanes_sum<Lane::kLph>(squares(x[i])) * c.per_dim + p.eps);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[i][e] *= w[e];
+                    for (int e = 0; e < 8; ++e) x[i][e] *= w[e] * inv;
                 }
                 ql.turn(p.r.interleaved != 0, cs, sn, x[i]);
-                if (!normed) power = power_below(lanes_max<Lane::kLph>(largest(x[i])));
-                const float f = inv * inverse_power(power);
+                const float power = power_of(lanes_max<Lane::kLph>(largest(x[i]))), f = inverse_power(power) * kUp;
 #pragma unroll
                 for (int u = 0; u < Lane::kRuns; ++u) {
                     float y[V];
@@ -517,34 +507,20 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
             umma_commit(&bars[1]);
         }
         __syncwarp();
-    } else if (warp == 1) {
-        // Exponents (the product of two powers of two may pass the ends of fp32): e_j of a token's key and value together, and for row i the largest e_j + (i - j) log2 y
-        // of the tokens j <= i.  A lane has four neighbouring tokens, lanes meet in a scan.
+    } else if (warp == 1) {                              // the factors of a token's key and value together, 2^kHighest for the largest
         const float* powers = c.powers + a.at * 2 * kTokens;
-        const float4 k = reinterpret_cast<const float4*>(powers)[lane], v = reinterpret_cast<const float4*>(powers + kTokens)[lane];
-        const float step = rate * 1.44269504f;
-        auto exponent = [&](int i, float x, float y) {
-            return 4 * lane + i < a.n ? static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) + static_cast<int>(__float_as_uint(y) >> 23) - 254) : -INFINITY;
-        };
-        const float e[4] = {exponent(0, k.x, v.x), exponent(1, k.y, v.y), exponent(2, k.z, v.z), exponent(3, k.w, v.w)};
-        float m[4];
-        m[0] = e[0];
+        float f[kTokens / 32], most = -254.0f;
 #pragma unroll
-        for (int i = 1; i < 4; ++i) m[i] = fmaxf(e[i], m[i - 1] + step);
-        float last = m[3];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float before = __shfl_up_sync(0xffffffffu, last, o);
-            if (lane >= o) last = fmaxf(last, before + step * static_cast<float>(4 * o));
+        for (int i = 0; i < kTokens / 32; ++i) {
+            const int j = lane + 32 * i;
+            // (as exponents: the product of two powers of two may pass the ends of fp32)
+            f[i] = static_cast<float>(static_cast<int>(__float_as_uint(powers[j]) >> 23) + static_cast<int>(__float_as_uint(powers[kTokens + j]) >> 23) - 254);
+            if (j < a.n) most = fmaxf(most, f[i]);
         }
-        float before = __shfl_up_sync(0xffffffffu, last, 1);
+        most = warp_max(most);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                    // (whole exponents, so that a factor and its inverse are exact)
-            before += step;
-            m[i] = ceilf(lane ? fmaxf(m[i], before) : m[i]);
-        }
-        reinterpret_cast<float4*>(kv_e)[lane] = make_float4(e[0], e[1], e[2], e[3]);
-        reinterpret_cast<float4*>(most_e)[lane] = make_float4(m[0], m[1], m[2], m[3]);
+        for (int i = 0; i < kTokens / 32; ++i) kv_f[lane + 32 * i] = lane + 32 * i < a.n ? exp2f(f[i] - most + kHighest) : 0.0f;
+        if (lane == 0) most_s = most;
     }
     __syncthreads();
     alive = mbar_wait_bounded(&bars[1], 0, p.status);
@@ -557,33 +533,34 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
     __syncwarp();
     const int row = (warp & 3) * 32 + lane, ch = warp >> 2;          // a thread has a row's fourth
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float row_power;                                     // of the row's largest weight
     {
-        uint32_t x[32], y[16];
-        if (ch > (warp & 3)) {                           // nothing of it is visible to these rows
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = 0;
-        } else {
+        uint32_t x[32];
+        float most = 0.0f;
+        if (ch <= (warp & 3)) {                          // otherwise nothing of it is visible to these rows
             tmem_ld32(tmem + lanes + ch * 32, x);
             tmem_ld_wait();
-            const float *power = power_s + (row - ch * 32), most = most_e[row] + kUpBits;      // (keys come brought up by kUp)
-            // (a factor past 2^126 stands beside a power that is zero)
-            auto factor = [&](float e) { return ex2(fminf(e - most, 126.0f)); };
+            const float* power = power_s + (row - ch * 32);
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(kv_e + ch * 32 + e);
-                float w[4];
-                if (ch == (warp & 3)) {
+                const float4 f4 = *reinterpret_cast<const float4*>(kv_f + ch * 32 + e);
+                const float f[4] = {f4.x, f4.y, f4.z, f4.w};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = e + k <= lane ? __uint_as_float(x[e + k]) * power[-(e + k <= lane ? e + k : 0)] : 0.0f;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = __uint_as_float(x[e + k]) * power[-(e + k)];
+                for (int k = 0; k < 4; ++k) {
+                    const bool seen = ch < (warp & 3) || e + k <= lane;
+                    const float w = seen ? __uint_as_float(x[e + k]) * power[-(seen ? e + k : 0)] * f[k] : 0.0f;
+                    most = fmaxf(most, fabsf(w));
+                    x[e + k] = __float_as_uint(w);
                 }
-                const __half2 h0 = __floats2half2_rn(w[0] * factor(f.x), w[1] * factor(f.y)), h1 = __floats2half2_rn(w[2] * factor(f.z), w[3] * factor(f.w));
-                y[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-                y[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
             }
         }
+        ss_s[ch][row] = most;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + (warp & 3)) : "memory");           // the four warps that share these rows
+        row_power = power_of(fmaxf(fmaxf(ss_s[0][row], ss_s[1][row]), fmaxf(ss_s[2][row], ss_s[3][row])));
+        const float f = inverse_power(row_power) * kUp;
+        uint32_t y[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = ch <= (warp & 3) ? bits_of(__floats2half2_rn(__uint_as_float(x[2 * e]) * f, __uint_as_float(x[2 * e + 1]) * f)) : 0u;
         tmem_st16(tmem + lanes + ch * 32, y);
     }
     tmem_st_wait();
@@ -604,7 +581,9 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     // the sums of squares of a row's fourths meet in shared memory
-    const float f = q_f[row] * p.scale, inside = f * exp2f(most_e[row]), before = f * power_s[min(row + 1, kTokens)];
+    const float row_bits = static_cast<float>(static_cast<int>(__float_as_uint(row_power) >> 23) - 127);
+    const float f = q_f[row] * p.scale, inside = f * exp2f(most_s + row_bits - (kHighest + 4 * kUpBits));
+    const float before = f * power_s[min(row + 1, kTokens)] * (1.0f / (kUp * kUp));
     float ss = 0.0f;
 #pragma unroll 1
     for (int q = 0; q < DP / 64; ++q) {

@@ -4,7 +4,7 @@ Tolerances.  A bf16 result is rounded by half a step, 2^-8 of it at most; fp16 o
 import numpy as np
 import pytest
 
-from rotated_helpers import Decay, f64, stream
+from rotated_helpers import Decay, f64, stream, tables
 from test_gpu_rotated_mixers import CHUNK, cfgd
 
 pytestmark = pytest.mark.gpu
@@ -23,12 +23,12 @@ def own_rows_close(got, want, tol, what):
     assert np.isfinite(got).all() and (err < tol).all(), (what, worst, err[worst], np.broadcast_to(tol, err.shape)[worst])
 
 
-def chunk_tolerance(a, proj):
+def chunk_tolerance(a, proj, by_head=False):
     """What operands of fp16 may do to the rows of a prompt from an empty state: four standard deviations, and the result's rounding.  A weight
-    y^(i-j) (q . k) has the errors of q and k, which meet in sqrt(sum q^2 k^2), and its own; a value has one more."""
+    y^(i-j) (q . k) has the errors of q and k, which meet in sqrt(sum q^2 k^2), and its own; a value has one more.  Whole rows, or every head of them."""
     q, k, v, _ = a.heads(proj, 0)
     age = np.arange(len(proj))[:, None] - np.arange(len(proj))[None]
-    errors, sizes = 0.0, 0.0
+    errors, sizes = [], []
     for h in range(a.H):
         with np.errstate(invalid="ignore"):
             keep = np.where(age >= 0, np.where(age == 0, 1.0, np.exp(np.maximum(age, 1) * float(a.rates[h]))), 0.0)
@@ -38,8 +38,10 @@ def chunk_tolerance(a, proj):
         err = 2.0 ** -12 * np.sqrt(2 / 3) * scale * np.sqrt((keep ** 2 * (mag ** 2 + s ** 2)) @ (v[:, h] ** 2).mean(axis=1))
         size = np.sqrt((o ** 2).mean(axis=1))
         f = 1 / np.sqrt(size ** 2 + a.eps) if a.norm is not None else 1.0
-        errors, sizes = errors + (f * err) ** 2, sizes + (f * size) ** 2
-    return 2.0 ** -8 + 4 * np.sqrt(errors / sizes)
+        errors.append((f * err) ** 2)
+        sizes.append((f * size) ** 2)
+    errors, sizes = np.array(errors).T, np.array(sizes).T
+    return 2.0 ** -8 + 4 * np.sqrt(errors / sizes if by_head else errors.sum(axis=1) / sizes.sum(axis=1))
 
 
 def states_near(a, slot):
@@ -47,6 +49,22 @@ def states_near(a, slot):
     got, want, n = f64(a.states[slot]), a.memory[slot]["S"], a.memory[slot]["at"]
     for h in range(a.H):
         assert np.abs(got[h] - want[h]).max() <= 5 * np.sqrt(2 * n / 12) * 2.0 ** -23 * np.abs(want[h]).max(), h
+
+
+def scale_tables(a, factor):
+    """Rotary tables times a factor, on the device and for the oracle (whose parts that turn are so much larger)."""
+    cos, sin = tables(a.rot, a.capacity)
+    for r in (a.rotation, a.m.rotation):
+        r.rope_cos, r.rope_sin = a.b.f32(factor * cos), a.b.f32(factor * sin)
+    heads, n = a.heads, a.rot["dims"]
+
+    def scaled(proj, first):
+        q, k, v, g = heads(proj, first)
+        q[..., :n] *= factor
+        k[..., :n] *= factor
+        return q, k, v, g
+
+    a.heads = scaled
 
 
 def parts(a, proj):
@@ -93,3 +111,49 @@ def test_decay_tokens_of_zeros_among_small_ones(cuda, stack_lib, norm, power):
     own_rows_close(got[rows], want[rows], tol, "rows")
     assert (got[[3, 70, 150]] == 0).all()
     states_near(a, 1)
+
+
+def uneven(a, which, power):
+    """Weights of the norm `which`: 2^power times as large in the first eight dimensions (a turning pair has both or neither)."""
+    half = a.rot["dims"] // 2 if a.rot else 0
+    w = getattr(a, which).copy()
+    w[np.r_[0:4, half:half + 4]] *= np.float32(2.0 ** power)
+    setattr(a, which, w)
+    for r in (a.rotation, a.m.rotation):
+        setattr(r, which, a.b.f32(w))
+
+
+@pytest.mark.parametrize("dim", [128, 64, 90])
+def test_decay_dimensions_of_very_different_sizes(cuda, stack_lib, dim):
+    """Keys large where queries are small, values with one number far above the others: no number is lost beside a large one."""
+    a = Decay(cuda, stack_lib, cfgd(3, dim, 44, 0.1, gated=False), 1, rates=[-0.01, -0.001, -0.3])
+    uneven(a, "k_norm", 17)
+    uneven(a, "q_norm", -17)
+    proj = np.random.default_rng(dim).standard_normal((300, a.cols)).astype(np.float32)
+    parts(a, proj)[1][:, 5::dim] *= 2.0 ** 18
+    # every head by itself: its norm is that of its large number, whose error the others of the head share beside their own (a head whose large number is small
+    # by chance has large others, of a large error)
+    tol, want = chunk_tolerance(a, proj, by_head=True).ravel(), a.oracle([1], proj).reshape(-1, dim)
+    got = a.forward(CHUNK, [1], proj).reshape(-1, dim)
+    own_rows_close(got[:, 5:6], want[:, 5:6], tol, "the large numbers")
+    rest = np.r_[0:5, 6:dim]
+    own_rows_close(got[:, rest], want[:, rest], 2 * tol, "the others")
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_decay_queries_far_below_the_norms_epsilon(cuda, stack_lib, norm):
+    a = Decay(cuda, stack_lib, cfgd(3, 128, 64, 0.1, gated=False, norm=norm), 1, norm=False, rates=[-0.01, -0.001, -0.3])
+    proj = np.random.default_rng(2).standard_normal((200, a.cols)).astype(np.float32)
+    proj[10:190, :3 * 128] *= np.exp2(-np.arange(180) / 8).astype(np.float32)[:, None]
+    tol, want = chunk_tolerance(a, proj), a.oracle([1], proj)
+    own_rows_close(a.forward(CHUNK, [1], proj), want, tol, "rows")
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_decay_with_tables_that_scale(cuda, stack_lib, norm):
+    """Tables may hold more than cosines and sines: a factor of 16, say."""
+    a = Decay(cuda, stack_lib, cfgd(3, 128, 64, 0.1, gated=False, norm=norm), 1, rates=[-0.01, -0.001, -0.3])
+    scale_tables(a, 16)
+    proj = np.random.default_rng(3).standard_normal((200, a.cols)).astype(np.float32)
+    tol, want = chunk_tolerance(a, proj), a.oracle([1], proj)
+    own_rows_close(a.forward(CHUNK, [1], proj), want, tol, "rows")
