@@ -3,7 +3,9 @@
 // A CTA works on two tiles of 128 query rows that take turns on the tensor cores.  S = Q K^T of tile w accumulates in the
 // 128 columns at 128 w; the weights go back into the columns S came from as two bf16 terms (p = hi + lo, both multiplied:
 // 16 bits of mantissa), as the A operand of O += P V; O of tile w is at 256 + 128 w.  Row maxima are only moved when they
-// grow by 2^8 (then O and the sum are rescaled).
+// grow by 2^8 (then O and the sum are rescaled).  With fp16 operands (HALF) the weights are one fp16 term: the largest stands at 2^11
+// and may grow by 2^4, so that weights down to 2^-25 of it keep their 11 bits (a sum of many such beside one that takes nearly everything),
+// and sums carry the same factor.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -23,7 +25,7 @@ constexpr int kSoftWarps = 8;                // warps 0-3 and 4-7: softmax of ti
 constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1;
 constexpr int kThreads = 32 * (kSoftWarps + 2);
 constexpr int kOCol = 256;
-constexpr float kRescale = 8.0f;
+constexpr float kRescale = 8.0f, kHalfRescale = 4.0f, kHalfTop = 11.0f;
 
 // two fp32 numbers per instruction
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -61,8 +63,8 @@ __device__ __forceinline__ void products(uint32_t d_tmem, uint64_t a, uint64_t b
 
 // One block of 128 scores of this thread's row -> weights in place; columns past `last` are not visible.  c = scale log2 e,
 // m the row's maximum (times c), l its sum.  vd: output columns to rescale.  p_full: two barriers, one for each half of the
-// weights, so that the second product starts under the second half's exponentials.  HALF: the weights as one fp16 term (12 bits, where operands are
-// fp16 too) in the first 16 of every 32 columns.
+// weights, so that the second product starts under the second half's exponentials.  HALF: the weights as one fp16 term in the first 16 of
+// every 32 columns.
 template <bool HALF = false>
 __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, int vd, int last, float c, bool first, float& m, float& l,
                                               uint64_t* p_full, int lane) {
@@ -89,7 +91,7 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, in
     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
     if (first) {
         m = top;
-    } else if (__any_sync(0xffffffffu, top > m + kRescale)) {
+    } else if (__any_sync(0xffffffffu, top > m + (HALF ? kHalfRescale : kRescale))) {
         const float mn = fmaxf(m, top), f = ex2(m - mn);
         m = mn;
         l *= f;
@@ -103,7 +105,8 @@ __device__ __forceinline__ void softmax_block(uint32_t s_col, uint32_t o_col, in
             tmem_st32(o_col + ch * 32, y);
         }
     }
-    const uint64_t cc = pair_of(c, c), mm = pair_of(-m, -m);
+    const float zero = HALF ? kHalfTop - m : -m;
+    const uint64_t cc = pair_of(c, c), mm = pair_of(zero, zero);
     uint64_t sums[2] = {0, 0};
 #pragma unroll
     for (int ch = 0; ch < 4; ++ch) {

@@ -3,7 +3,7 @@
 //
 // Code x scale (e2m1 x e4m3: six bits between 2^-10 and 2688) is exact in fp16, so the products are warp-level MMAs (16 x 8 x 16, fp16 operands, fp32
 // sums) of exact keys and values; queries are rounded to fp16 under a power of two per head, softmax weights to fp16 (2^-12 each, where the bf16 result is rounded by
-// 2^-9).  Scores are made as S^T = K Q^T and outputs as O^T = V^T P^T: cached numbers are the A operand, whose 16 x 16 numbers a step cost the fewest MMAs, and the
+// 2^-9): the largest weight stands at 2^11, so that one down to 2^-25 of it keeps its bits, 2^-35 is left out.  Scores are made as S^T = K Q^T and outputs as O^T = V^T P^T: cached numbers are the A operand, whose 16 x 16 numbers a step cost the fewest MMAs, and the
 // fragments of S^T turn into those of P^T by one transposed 8 x 8 move each.
 //
 // The order of the dimensions inside an MMA is free as long as both operands agree, so a lane takes 16 neighbouring dimensions of a token's key -- one scale -- for four steps, and
@@ -25,7 +25,7 @@ namespace stack {
 namespace {
 
 constexpr int kTile = 32;
-constexpr float kRescale = 8.0f;
+constexpr float kRescale = 4.0f, kTop = 11.0f;           // a weight stays below 2^15
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(32 * W, W == 16 || DP > 128 ? 1 : NT == 1 ? 4 
                 top[u][e] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
                 grown = grown || top[u][e] > mx[u][e] + kRescale;
             }
-        // the maximum only moves when it grows by 2^8, so that lanes need not ask each other for most tiles; then output and sum are rescaled
+        // the maximum only moves when it grows by 2^4, so that lanes need not ask each other for most tiles; then output and sum are rescaled
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(32 * W, W == 16 || DP > 128 ? 1 : NT == 1 ? 4 
             for (int e = 0; e < 2; ++e) {
                 float x[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[i >> 1][u][2 * (i & 1) + e] = x[i] = ex2(s[i >> 1][u][2 * (i & 1) + e] - mx[u][e]);
+                for (int i = 0; i < 4; ++i) s[i >> 1][u][2 * (i & 1) + e] = x[i] = ex2(s[i >> 1][u][2 * (i & 1) + e] - (mx[u][e] - kTop));
                 sum[u][e] += (x[0] + x[1]) + (x[2] + x[3]);
             }
 #pragma unroll

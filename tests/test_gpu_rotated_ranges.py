@@ -4,8 +4,9 @@ Tolerances.  A bf16 result is rounded by half a step, 2^-8 of it at most; fp16 o
 import numpy as np
 import pytest
 
-from rotated_helpers import Decay, f64, stream, tables
-from test_gpu_rotated_mixers import CHUNK, cfgd
+from oracle import layer_stack as O
+from rotated_helpers import Decay, Quantized, f64, stream, tables
+from test_gpu_rotated_mixers import CHUNK, FLASH, SIMT, STREAM, cfg4, cfgd
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +158,28 @@ def test_decay_with_tables_that_scale(cuda, stack_lib, norm):
     proj = np.random.default_rng(3).standard_normal((200, a.cols)).astype(np.float32)
     tol, want = chunk_tolerance(a, proj), a.oracle([1], proj)
     own_rows_close(a.forward(CHUNK, [1], proj), want, tol, "rows")
+
+
+@pytest.mark.parametrize("precision,route,n", [(0, SIMT, 3), (1, SIMT, 3), (1, STREAM, 1), (1, STREAM, 3), (1, FLASH, 80)])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 16.0, 18.0, 20.0])
+@pytest.mark.parametrize("place", [0, 40, 510])
+def test_quantized_weights_beside_one_that_takes_nearly_everything(cuda, stack_lib, precision, route, n, gap, place):
+    """A key far above the others whose value is zero: the output is the others' small sum.  Weights e^-gap of the largest, which in fp16 stand at 2^11 or above: at
+    e^-20 = 2^-28.9 half a step of 2^-24 is 2^-7.1 of them (standard deviation 2^-7.9, many tokens), beside the result's 2^-8; in fp32 the 2e-5 of other tests."""
+    a = Quantized(cuda, stack_lib, cfg4(4, 2, 64, 0, 1.0, gated=False, norm=False), precision, capacity=700)
+    rng = np.random.default_rng(int(gap) + place)
+    T, d, G = 600, 64, 2
+    proj = rng.standard_normal((T + n, a.cols)).astype(np.float32)
+    keys, values = proj[:, 4 * d:6 * d], proj[:, 6 * d:8 * d]
+    sign = np.where(rng.random(2 * d) < 0.5, -1, 1)
+    keys *= 2.0 ** -5
+    keys[place], values[place] = 0.5 * sign, 0
+    held = O.four_bits(keys[place].reshape(G, d), a.cfg["key_scale"])
+    for h in range(4):                                           # queries along that key
+        c = np.float16(gap / np.abs(held[h // 2]).sum())
+        proj[:, h * d:(h + 1) * d] = c * sign[h // 2 * d:(h // 2 + 1) * d]
+    before, rows = proj[:T], proj[T:]
+    a.forward(SIMT, [1], before)
+    a.oracle([1], before)
+    want, got = a.oracle([1], rows), a.forward(route, [1], rows)
+    own_rows_close(got.reshape(-1, d), want.reshape(-1, d), 2.0 ** -7 if precision else 2e-5, "heads")
