@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(kThreads) quantized_rows_kernel(const Quantize
         for (int r = 0; r < R; ++r) {
             const int last = min(pos0 + min(first + r, total - 1) / p.group, t1 - 1);
             const float x = token <= last ? s[r] * p.scale_log2 : -INFINITY, mn = fmaxf(m[r], warp_max(x));
-            // a row that has seen nothing yet keeps its maximum at -infinity and its weights at zero
-            const float f = m[r] == -INFINITY ? 0.0f : exp2f(m[r] - mn), w = mn == -INFINITY ? 0.0f : exp2f(x - mn);
+            // a row that has seen nothing yet keeps its maximum at -infinity and its weights at zero (a score that is NaN has no maximum, but its weight)
+            const float f = m[r] == -INFINITY ? 0.0f : exp2f(m[r] - mn), w = x == -INFINITY ? 0.0f : exp2f(x - mn);
             m[r] = mn;
             l[r] = fmaf(l[r], f, w);
             w_s[warp][r][lane] = w;

@@ -183,3 +183,22 @@ def test_quantized_weights_beside_one_that_takes_nearly_everything(cuda, stack_l
     a.oracle([1], before)
     want, got = a.oracle([1], rows), a.forward(route, [1], rows)
     own_rows_close(got.reshape(-1, d), want.reshape(-1, d), 2.0 ** -7 if precision else 2e-5, "heads")
+
+
+@pytest.mark.parametrize("precision,route", [(0, SIMT), (0, 0), (1, SIMT), (1, STREAM), (1, FLASH), (1, 0)])
+@pytest.mark.parametrize("before", [0, 32, 63, 128, 224, 300])
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_quantized_numbers_that_are_not_finite_reach_the_rows_behind(cuda, stack_lib, precision, route, before, what):
+    """A NaN in a key or value is seen in every head that reads it, also where it is the only token of a tile that a row sees, and in no other."""
+    a = Quantized(cuda, stack_lib, cfg4(4, 2, 64, 32, 0.2, gated=False), precision)
+    rng = np.random.default_rng(before)
+    if before:
+        a.forward(SIMT, [1], rng.standard_normal((before, a.cols)).astype(np.float32))
+    d = 64
+    proj = rng.standard_normal((1, a.cols)).astype(np.float32)
+    proj[0, (5 if what == "key" else 7) * d + 3] = np.nan       # of key/value head 1
+    for _ in range(3):                                           # the token itself, and two behind it
+        got = a.forward(route, [1], proj).reshape(4, d)
+        assert np.isfinite(got[:2]).all()
+        assert np.isnan(got[2:]).all() if what == "key" else np.isnan(got[2:, :16]).all() and np.isfinite(got[2:, 16:]).all()
+        proj = rng.standard_normal((1, a.cols)).astype(np.float32)
