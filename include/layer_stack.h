@@ -256,7 +256,7 @@ int tbl_attention_forward(const tbl_attention_mixer* mixer, int precision, int r
 /* Norm and rotation of stacked projections proj fp32 [n_seq*n_tok, ld]: q_heads heads of `dim` from column 0 on, then k_heads.  q_dev
  * [rows, q_heads, dim] and k_dev [rows, k_heads, dim] have the precision's type; either count may be 0 (its pointer is not used then).  Row
  * sequence*n_tok + t stands at positions_dev[slots_dev[sequence]] + t; a position outside the tables sets TBL_DEV_CACHE_FULL, and its
- * rows stay as they were.  dim <= TBL_MAX_ROTATED_DIM.  The tables and norms are in place before the call. */
+ * rows stay as they were.  dim <= TBL_MAX_ROTATED_DIM. */
 int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int precision, float eps, const float* proj_dev, int ld, int q_heads,
                               int k_heads, int dim, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok,
                               void* q_dev, void* k_dev, void* stream);

@@ -35,6 +35,8 @@ __global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_ke
     int at[kRuns];
 #pragma unroll
     for (int u = 0; u < U; ++u) Units::runs(p.r, gl + LPH * u, at[2 * u], at[2 * u + 1]);
+    pdl_launch_dependents();
+    pdl_wait();
     float bound = 1.0f;
     if (HALVES && p.q_norm) {                                    // sqrt(dim) times the largest weight bounds a normed head
         float most = 0.0f, w[kNumbers];
@@ -46,8 +48,6 @@ __global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_ke
         for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         bound = power_below(sqrtf(static_cast<float>(dim)) * most);
     }
-    pdl_launch_dependents();
-    pdl_wait();
     const int row = blockIdx.x;
     const int pos = p.positions[p.slots[row / p.n_tok]] + row % p.n_tok;
     const bool outside = p.r.half > 0 && (pos < 0 || pos >= p.r.positions);

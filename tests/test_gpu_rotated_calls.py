@@ -215,3 +215,29 @@ def test_quantized_cache_past_32_bits(cuda, stack_lib, precision, route, n):
         assert np.abs(got[:, h] - want).max() <= (2.0 ** -7 if precision else 2e-5) * np.abs(want).max()
     far = a.cache[1, :, cap - n:]
     assert not bool(far.any()) and bool((a.cache[0] == 255).all())               # the new tokens' keys and values are zero too
+
+
+@pytest.mark.parametrize("precision,route,n", [(0, SIMT, 3), (1, STREAM, 1), (1, STREAM, 3), (1, FLASH, 64)])
+def test_quantized_norms_written_by_the_call_ahead(cuda, stack_lib, precision, route, n):
+    """Norms are operands like any other: the call before may have written them.  (Here a rotation without angles, which copies fp32 heads.)"""
+    from reimagined_b200 import capi
+    torch = cuda
+    a = Quantized(cuda, stack_lib, cfg4(4, 2, 64, 32, 0.2), precision)
+    rng = np.random.default_rng(4)
+    proj = rng.standard_normal((n, a.cols)).astype(np.float32)
+    pd, out = a.device(proj), torch.zeros((n, a.H * a.d), device="cuda", dtype=a.dtype)
+    norms, big = torch.zeros((2, 64), device="cuda"), torch.zeros((4096, 4096), device="cuda")
+    for m in (a.rotation, a.m.rotation):
+        m.q_norm, m.k_norm = norms[0].data_ptr(), norms[1].data_ptr()
+    size = stack_lib.tbl_quantized_workspace_bytes(C.byref(a.m), precision, route, 1, n, n)
+    ws, zero, plain = a.space(size), a.b.i32([0]), capi.HeadRotation()
+    for _ in range(20):
+        a.q_norm, a.k_norm = (1 + 0.2 * rng.standard_normal(64).astype(np.float32) for _ in range(2))
+        source = a.device([a.q_norm, a.k_norm])
+        a.memory.clear()
+        want = a.oracle([0], proj)
+        big.fill_(1.0)                                           # keeps the stream busy until everything is enqueued
+        assert stack_lib.tbl_head_rotation_forward(C.byref(plain), 0, a.eps, source.data_ptr(), 64, 1, 0, 64, zero, zero, 1, 2, norms.data_ptr(), None, stream(torch)) == 0
+        assert stack_lib.tbl_quantized_forward(C.byref(a.m), precision, route, a.eps, pd.data_ptr(), a.cache.data_ptr(), 3, a.capacity, zero, a.positions.data_ptr(), 1, n, n,
+                                               out.data_ptr(), ws.data_ptr(), size, stream(torch)) == 0
+        rows_close(f64(out), want, 2.0 ** -7 if precision else 2e-5, "rows")
