@@ -117,11 +117,6 @@ __device__ __forceinline__ float lanes_max(float v) {
     for (int o = LPH / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-// The power of two at or below a head's largest number, 2^-113 at least (also for a head of zeros, which so counts less than any other); times kUp its inverse
-// is a number.
-__device__ __forceinline__ float power_of(float most) { return power_below(fmaxf(most, 0x1p-113f)); }
-// one over a power of two
-__device__ __forceinline__ float inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ float largest(const float (&x)[8]) {
     float m = fabsf(x[0]);
 #pragma unroll
@@ -197,7 +192,6 @@ __device__ __forceinline__ int table_row(const DecayParams& p, int pos) { return
 // go to decay_chunk_kernel on the way, as the tiles that it multiplies.  The second tile's rows are asked for as soon as the first one's registers are free.  Bound by the
 // way of the rows to the registers (35 % of the issue slots, 40 % of the stalls wait for loads); registers and tensor memory leave two CTAs to an SM.  64 chunks of 32 heads:
 // 149 us for 537 MB in and out, 3.6 TB/s.
-constexpr float kUp = 8192.0f, kUpBits = 13.0f;          // numbers below 2 end below 2^14
 constexpr float kHighest = 60.0f;                        // (a score of two such heads ends below 2^35)
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkParams c) {

@@ -37,17 +37,6 @@ __global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_ke
     for (int u = 0; u < U; ++u) Units::runs(p.r, gl + LPH * u, at[2 * u], at[2 * u + 1]);
     pdl_launch_dependents();
     pdl_wait();
-    float bound = 1.0f;
-    if (HALVES && p.q_norm) {                                    // sqrt(dim) times the largest weight bounds a normed head
-        float most = 0.0f, w[kNumbers];
-#pragma unroll
-        for (int u = 0; u < kRuns; ++u) Units::load_run(p.q_norm, at[u], limit, w + V * u);
-#pragma unroll
-        for (int e = 0; e < kNumbers; ++e) most = fmaxf(most, fabsf(w[e]));
-#pragma unroll
-        for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        bound = power_below(sqrtf(static_cast<float>(dim)) * most);
-    }
     const int row = blockIdx.x;
     const int pos = p.positions[p.slots[row / p.n_tok]] + row % p.n_tok;
     const bool outside = p.r.half > 0 && (pos < 0 || pos >= p.r.positions);
@@ -102,17 +91,14 @@ __global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_ke
             }
         float back = 1.0f;
         if (HALVES) {
-            float power = bound;
-            if (!p.q_norm) {
-                float most = 0.0f;
+            float most = 0.0f;
 #pragma unroll
-                for (int e = 0; e < kNumbers; ++e) most = fmaxf(most, fabsf(x[e]));
+            for (int e = 0; e < kNumbers; ++e) most = fmaxf(most, fabsf(x[e]));
 #pragma unroll
-                for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                power = power_below(most);
-            }
-            back = __uint_as_float((254u << 23) - __float_as_uint(power));
-            if (gl == 0 && h < p.heads) p.q_factor[static_cast<size_t>(row) * p.heads + h] = power;
+            for (int o = LPH / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float power = power_of(most);
+            back = inverse_power(power) * kUp;
+            if (gl == 0 && h < p.heads) p.q_factor[static_cast<size_t>(row) * p.heads + h] = power * (1.0f / kUp);
         }
         if (h >= p.heads) continue;
         T* dst = HALVES ? static_cast<T*>(p.q) + (static_cast<size_t>(row) * p.heads + h) * p.ldq

@@ -166,9 +166,16 @@ __device__ __forceinline__ float power_below(float v) {
     const uint32_t power = min(__float_as_uint(v) >> 23, 253u);
     return power ? __uint_as_float(power << 23) : 1.0f;
 }
+// Numbers as fp16: under the power of two at or below the largest of them (2^-113 at least, also for zeros, which so count less than anything else), and
+// brought up by kUp to below 2^14, so that those 2^-28 below the largest keep their bits.  The largest itself, not what a norm allows: weights may be uneven, the norm's
+// epsilon may rule, tables may scale.
+constexpr float kUp = 8192.0f, kUpBits = 13.0f;
+__device__ __forceinline__ float power_of(float most) { return power_below(fmaxf(most, 0x1p-113f)); }
+// one over a power of two
+__device__ __forceinline__ float inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 
 // head_rotation.cu: q_heads, then k_heads heads of `dim` from column 0 of proj on -> q, k [rows][heads][dim].  With q_factor (k_heads 0): q is fp16
-// [rows][heads][ldq], zeros behind a head, each head divided by a power of two, q_factor [rows][heads], that leaves its numbers below 2.
+// [rows][heads][ldq], zeros behind a head, each head divided by a power of two, q_factor [rows][heads], that leaves its numbers below 2^14.
 struct RotationCall {
     const float* proj;
     int ld, q_heads, k_heads, dim;

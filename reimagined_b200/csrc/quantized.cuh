@@ -102,7 +102,7 @@ __device__ __forceinline__ void put_row(const QuantizedParams& p, uint8_t* dst, 
     const int used = p.width + p.width / 8;
     if (!is_k && used + lane < p.row) dst[used + lane] = 0;
 }
-// fp16 queries: the power of two a head is divided by, so that its largest number lies in [1, 2), and the factor that does it
+// fp16 queries: the power of two a head is divided by, and the factor that does it
 template <int V>
 __device__ __forceinline__ float query_power(const HeadUnits<V, 32>& x, float& factor) {
     float most = 0.0f;
@@ -110,9 +110,9 @@ __device__ __forceinline__ float query_power(const HeadUnits<V, 32>& x, float& f
     for (int i = 0; i < HeadUnits<V, 32>::kUnits; ++i)
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) most = fmaxf(most, fabsf(x.x[i][e]));
-    const uint32_t power = min(__float_as_uint(warp_max(most)) >> 23, 253u);
-    factor = power ? __uint_as_float((254u - power) << 23) : 1.0f;
-    return power ? __uint_as_float(power << 23) : 1.0f;
+    const float power = power_of(warp_max(most));
+    factor = inverse_power(power) * kUp;
+    return power * (1.0f / kUp);
 }
 
 // quantized_decode.cu: streams the 4-bit rows for a few query rows

@@ -202,3 +202,31 @@ def test_quantized_numbers_that_are_not_finite_reach_the_rows_behind(cuda, stack
         assert np.isfinite(got[:2]).all()
         assert np.isnan(got[2:]).all() if what == "key" else np.isnan(got[2:, :16]).all() and np.isfinite(got[2:, 16:]).all()
         proj = rng.standard_normal((1, a.cols)).astype(np.float32)
+
+
+Q_CALLS = [(0, SIMT, 3), (1, SIMT, 3), (1, STREAM, 1), (1, STREAM, 3), (1, FLASH, 80)]
+
+
+@pytest.mark.parametrize("precision,route,n", Q_CALLS)
+@pytest.mark.parametrize("case", ["uneven", "uneven the other way", "far below epsilon", "tables that scale"])
+def test_quantized_queries_of_very_different_sizes(cuda, stack_lib, precision, route, n, case):
+    """No number of a query is lost beside a larger one, or under what its norm would allow.  Scores have a standard deviation s of some units; fp16 queries move
+    one by 2^-12 / sqrt(3) s, and an output by about as much of itself: with s below 4, 2^-11, beside the result's 2^-8."""
+    uneven_by = {"uneven": 18, "uneven the other way": -18}.get(case, 0)
+    scale = {"far below epsilon": 6e4, "tables that scale": 0.2 / 256}.get(case, 0.3)
+    units = (2.0 ** 9 if uneven_by > 0 else 0.5 if case == "tables that scale" else 0.05, 0.07)
+    a = Quantized(cuda, stack_lib, cfg4(4, 2, 64, 64, scale, gated=False, units=units), precision, capacity=500)
+    if uneven_by:
+        uneven(a, "k_norm", uneven_by)
+        uneven(a, "q_norm", -uneven_by)
+    if case == "tables that scale":
+        scale_tables(a, 16)
+    rng = np.random.default_rng(len(case))
+    proj = rng.standard_normal((400 + n, a.cols)).astype(np.float32)
+    if case == "far below epsilon":
+        proj[:, :4 * 64] *= np.float32(1e-7)
+    before, rows = proj[:400], proj[400:]
+    a.forward(SIMT, [1], before)
+    a.oracle([1], before)
+    want, got = a.oracle([1], rows), a.forward(route, [1], rows)
+    own_rows_close(got.reshape(-1, 64), want.reshape(-1, 64), 2.0 ** -7 if precision else 2e-5, "heads")
