@@ -170,12 +170,17 @@ tbl_attention_mixer as_attention(const tbl_quantized_mixer& m) {
     return a;
 }
 
+// what the flash kernel's grid and the 32-bit rows of its tensor maps hold (expanded keys and values of every sequence and head, whole blocks of 128)
+bool flash_fits(const tbl_quantized_mixer& m, int n_seq, int context) {
+    return attention_flash_supported(as_attention(m)) && static_cast<long long>(n_seq) * m.kv_heads * round_up(context, 128) <= 2147483647LL;
+}
+
 // bf16: the flash kernel where its time, worked out from what it took, is shorter than the streaming kernel's (32 query and 8 key/value heads of 128, in us, streaming and
 // flash kernel: one sequence of 64 tokens over 1024 20 and 43, over 16384 97 and 287; 256 over 4096 115 and 109; 512 over 512 58 and 45; eight sequences of 64 over
 // 4096 193 and 233, of 128 over 128 86 and 64, over 4096 372 and 244).  Both read or walk the context: the one for every block of 8 or 16 query rows, the other a wave of CTAs at a time.
 int pick_route(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context) {
     if (precision != TBL_BF16) return kSimt;
-    if (!attention_flash_supported(as_attention(m))) return kStream;
+    if (!flash_fits(m, n_seq, context)) return kStream;
     const double rows = static_cast<double>(n_seq) * n_tok, caches = static_cast<double>(n_seq) * m.kv_heads * quantized_width(m.dim) / 128;
     const double seen = context - 0.5 * n_tok, group = m.heads / m.kv_heads;
     const double blocks = ceil(n_tok * group / quantized_stream_rows(m, n_tok)), waves = ceil(n_seq * static_cast<double>(m.heads) * ceil_div(n_tok, 256) / kNumSm);
@@ -317,7 +322,9 @@ int launch_quantized(const tbl_quantized_mixer& m, int precision, int route, flo
     if (rows > 2147483647LL || static_cast<long long>(n_seq) * m.kv_heads > 65535 || ceil_div(m.heads + 2 * m.kv_heads, kPrepWarps) > 65535 || w.splits > 65535) return TBL_ERR_SHAPE;
     // blocks of query rows are one side of a grid
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads), stream_rows = quantized_stream_rows(m, n_tok);
-    if ((w.route == kStream && (total + stream_rows - 1) / stream_rows > 65535) || (w.route == kSimt && quantized_rows_blocks(m, n_seq, n_tok, context) > 65535)) return TBL_ERR_SHAPE;
+    if ((w.route == kStream && (total + stream_rows - 1) / stream_rows > 65535) || (w.route == kSimt && quantized_rows_blocks(m, n_seq, n_tok, context) > 65535) ||
+        (w.route == kFlash && !flash_fits(m, n_seq, context)))
+        return TBL_ERR_SHAPE;
     QuantizedParams p = basic_params(m, capacity, slots, positions, n_tok);
     if (!p.status) return TBL_ERR_CUDA;
     uint8_t* base = static_cast<uint8_t*>(ws);

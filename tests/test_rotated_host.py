@@ -188,3 +188,11 @@ def test_more_query_rows_than_a_grid_has(stack_lib):
     for precision, route in ((0, 0), (0, 1), (1, 1), (1, 2)):
         assert stack_lib.tbl_quantized_forward(C.byref(m), precision, route, 1e-5, 4096, 4096, 2, n, 4096, 4096, 1, n, n, 4096, 4096, 1 << 60, None) == -2
     assert stack_lib.tbl_launch_count() == before
+
+
+def test_more_than_the_prompt_kernel_holds(stack_lib):
+    """Heads in two parts that pass a grid's side, and expanded rows that pass 32 bits: refused before anything is appended."""
+    before = stack_lib.tbl_launch_count()
+    for m, n_seq, context in ((quantized(heads=32768, kv_heads=1, dim=136, gated=0), 1, 64), (quantized(heads=8, kv_heads=8), 64, 4194304), (quantized(heads=8, kv_heads=8), 64, 4194304 - 100)):
+        assert stack_lib.tbl_quantized_forward(C.byref(m), 1, 3, 1e-5, 4096, 4096, 64, 4194304, 4096, 4096, n_seq, 64, context, 4096, 4096, (1 << 63) - 1, None) == -2
+    assert stack_lib.tbl_launch_count() == before
