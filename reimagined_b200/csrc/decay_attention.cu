@@ -206,12 +206,13 @@ __device__ __forceinline__ void finish_head(const DecayParams& p, const float* s
 // Up to four tokens of a head in one launch (32 heads of 128, four tokens 9.2 us, eight 14.1, the scan of nine 11.0; 16 sequences 21.8, 34.7 and 31.7).  A CTA has the whole head: its state comes into shared memory by one bulk copy and goes back by another, so that registers
 // hold a few rows at a time and three CTAs of heads of 128 share an SM; while it comes, a warp each norms and turns the tokens' queries and keys.  Bound by the
 // state's bytes: the projections are asked for first, or they would queue behind the states of the whole batch (64 sequences of 32 heads of 128: 49.7 us, 5.5 TB/s; with
-// the state in registers 65 to 79).
+// the state in registers 65 to 79).  The bound on registers is what three CTAs have (left to itself the compiler takes 47 instead of 60, with fewer loads on
+// their way: 51).
 constexpr size_t kStepRoom = 200 * 1024;
 size_t step_smem(int keys, int d, int n_tok) { return sizeof(float) * (static_cast<size_t>(d) * d + static_cast<size_t>(n_tok) * (2 * keys + 3 * d)); }
 
 template <typename T, int V, int LK, int C>
-__global__ void __launch_bounds__(kThreads) decay_step_kernel(const DecayParams p) {
+__global__ void __launch_bounds__(kThreads, 3) decay_step_kernel(const DecayParams p) {
     using S = State<LK, C, 4>;
     extern __shared__ __align__(128) float room[];
     __shared__ __align__(8) uint64_t full;
@@ -231,8 +232,10 @@ __global__ void __launch_bounds__(kThreads) decay_step_kernel(const DecayParams 
     const int slot = p.slots[seq];
     const size_t row0 = static_cast<size_t>(seq) * p.n_tok;
     const float* proj = p.proj + row0 * p.ld + head * p.d;
-    HeadUnits<V, 32> x;                                          // of this warp's first vector
-    if (warp < 2 * p.n_tok) x.load(p.r, proj + static_cast<size_t>(warp >> 1) * p.ld + (warp & 1) * p.H * p.d, p.d, lane);
+    static_assert(2 * kStepTokens <= kThreads / 32, "a warp for every vector");
+    const int vec = warp >> 1, is_k = warp & 1;                  // a warp's: the query or key of a token
+    HeadUnits<V, 32> x;
+    if (vec < p.n_tok) x.load(p.r, proj + static_cast<size_t>(vec) * p.ld + is_k * p.H * p.d, p.d, lane);
     for (int i = tid; i < 2 * p.n_tok * p.d; i += kThreads) {
         const int is_g = i >= p.n_tok * p.d, e = i - is_g * p.n_tok * p.d;
         if (!is_g || p.g_off >= 0) v_s[i] = proj[static_cast<size_t>(e / p.d) * p.ld + (is_g ? p.g_off : p.v_off) + e % p.d];
@@ -245,11 +248,9 @@ __global__ void __launch_bounds__(kThreads) decay_step_kernel(const DecayParams 
         if (p.r.half > 0 && head == 0 && (pos < 0 || pos + p.n_tok > p.r.positions)) atomicOr(p.status, TBL_DEV_CACHE_FULL);
     }
     __syncthreads();
-    for (int i = warp; i < 2 * p.n_tok; i += kThreads / 32) {
-        const int t = i >> 1, is_k = i & 1;
-        if (i != warp) x.load(p.r, proj + static_cast<size_t>(t) * p.ld + is_k * p.H * p.d, p.d, lane);
-        x.template turn<float>(p.r, is_k ? p.k_norm : p.q_norm, p.eps, p.r.half > 0 ? min(max(pos + t, 0), p.r.positions - 1) : 0, p.d, lane);
-        x.store(p.r, (is_k ? k_s : q_s) + t * S::kKeys, p.d, lane);
+    if (vec < p.n_tok) {
+        x.template turn<float>(p.r, is_k ? p.k_norm : p.q_norm, p.eps, p.r.half > 0 ? min(max(pos + vec, 0), p.r.positions - 1) : 0, p.d, lane);
+        x.store(p.r, (is_k ? k_s : q_s) + vec * S::kKeys, p.d, lane);
     }
     const float l = expm1f(p.log_decay[head]);
     const uint64_t less = pair_of(l, l);

@@ -86,22 +86,9 @@ struct HeadLane {
             }
         }
     }
-    __device__ __forceinline__ void turn(bool pairs, const float (&c)[4], const float (&s)[4], float (&x)[8]) const {
+    __device__ __forceinline__ void turn(int interleaved, const float (&c)[4], const float (&s)[4], float (&x)[8]) const {
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float *y = x + 2 * V * u, cj = c[V * u + j], sj = s[V * u + j];
-                if (pairs) {
-                    const float a = y[2 * j], b = y[2 * j + 1];
-                    y[2 * j] = a * cj - b * sj;
-                    y[2 * j + 1] = b * cj + a * sj;
-                } else {
-                    const float a = y[j], b = y[V + j];
-                    y[j] = a * cj - b * sj;
-                    y[V + j] = b * cj + a * sj;
-                }
-            }
+        for (int u = 0; u < kUnits; ++u) turn_unit<V>(interleaved, c + V * u, s + V * u, x + 2 * V * u);
     }
 };
 
@@ -257,7 +244,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
 #pragma unroll
                 for (int e = 0; e < 8; ++e) k[i][e] *= w[e] * f;
             }
-            kl.turn(p.r.interleaved != 0, cs, sn, k[i]);
+            kl.turn(p.r.interleaved, cs, sn, k[i]);
             power[i] = power_of(lanes_max<Lane::kLph>(largest(k[i])));
             const float v_most = lanes_max<Lane::kLph>(largest(v[i])), v_power = power_of(v_most);
             most = fmaxf(most, v_most * (weight_s[j] * power[i]));
@@ -477,7 +464,7 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[i][e] *= w[e] * inv;
                 }
-                ql.turn(p.r.interleaved != 0, cs, sn, x[i]);
+                ql.turn(p.r.interleaved, cs, sn, x[i]);
                 const float power = power_of(lanes_max<Lane::kLph>(largest(x[i]))), f = inverse_power(power) * kUp;
 #pragma unroll
                 for (int u = 0; u < Lane::kRuns; ++u) {

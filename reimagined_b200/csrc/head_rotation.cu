@@ -75,20 +75,7 @@ __global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_ke
             for (int e = 0; e < kNumbers; ++e) x[e] *= w[e] * f;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float *y = x + 2 * V * u, cj = c[V * u + j], sj = sn[V * u + j];
-                if (p.r.interleaved) {
-                    const float a = y[2 * j], b = y[2 * j + 1];
-                    y[2 * j] = a * cj - b * sj;
-                    y[2 * j + 1] = b * cj + a * sj;
-                } else {
-                    const float a = y[j], b = y[V + j];
-                    y[j] = a * cj - b * sj;
-                    y[V + j] = b * cj + a * sj;
-                }
-            }
+        for (int u = 0; u < U; ++u) turn_unit<V>(p.r.interleaved, c + V * u, sn + V * u, x + 2 * V * u);
         float back = 1.0f;
         if (HALVES) {
             float most = 0.0f;

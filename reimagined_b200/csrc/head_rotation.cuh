@@ -21,11 +21,29 @@ inline Rotation rotation_of(const tbl_head_rotation& r) { return Rotation{r.rope
 __device__ __forceinline__ float reciprocal_root(float v) { return rsqrtf(v); }          // 2 units in the last place
 __device__ __forceinline__ double reciprocal_root(double v) { return 1.0 / sqrt(v); }
 
+// The V pairs of a unit y [2 V] turn by their cosines and sines: the two runs of V, or neighbours.
+template <int V, typename A>
+__device__ __forceinline__ void turn_unit(int interleaved, const float* c, const float* s, A* y) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (interleaved) {
+            const A p = y[2 * j], q = y[2 * j + 1];
+            y[2 * j] = p * A(c[j]) - q * A(s[j]);
+            y[2 * j + 1] = q * A(c[j]) + p * A(s[j]);
+        } else {
+            const A p = y[j], q = y[V + j];
+            y[j] = p * A(c[j]) - q * A(s[j]);
+            y[V + j] = q * A(c[j]) + p * A(s[j]);
+        }
+    }
+}
+
 // A head spread over LPH lanes, in units of 2 V numbers: V pairs (a, b) that turn together, or numbers that do not turn.  Without `interleaved` a unit that
-// turns is two runs of V neighbours half a rotated part apart, otherwise it is 2 V neighbours.  V = 4: 16-byte accesses (vector_heads below), V = 1: any size.
+// turns is two runs of V neighbours half a rotated part apart, otherwise it is 2 V neighbours.  V = 4: 16-byte accesses (vector_heads below), V = 2: 8-byte ones
+// (paired_heads), V = 1: any size.
 template <int V, int LPH>
 struct HeadUnits {
-    static constexpr int kUnits = V == 4 ? 1 : TBL_MAX_ROTATED_DIM / 2 / LPH;      // vectors: callers choose LPH >= dim / 8
+    static constexpr int kUnits = V == 4 ? 1 : TBL_MAX_ROTATED_DIM / (2 * V) / LPH;      // vectors: callers choose LPH >= dim / 8
     float x[kUnits][2 * V];
 
     // where unit u begins, and its second run of V numbers
@@ -87,18 +105,7 @@ struct HeadUnits {
                 float c[V], s[V];
                 load_run(r.cos + static_cast<size_t>(pos) * r.half, V * u, r.half, c);
                 load_run(r.sin + static_cast<size_t>(pos) * r.half, V * u, r.half, s);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (r.interleaved) {
-                        const A p = y[2 * j], q = y[2 * j + 1];
-                        y[2 * j] = p * A(c[j]) - q * A(s[j]);
-                        y[2 * j + 1] = q * A(c[j]) + p * A(s[j]);
-                    } else {
-                        const A p = y[j], q = y[V + j];
-                        y[j] = p * A(c[j]) - q * A(s[j]);
-                        y[V + j] = q * A(c[j]) + p * A(s[j]);
-                    }
-                }
+                turn_unit<V>(r.interleaved, c, s, y);
             }
 #pragma unroll
             for (int e = 0; e < 2 * V; ++e) x[i][e] = static_cast<float>(y[e]);

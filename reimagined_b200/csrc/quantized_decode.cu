@@ -8,7 +8,7 @@
 //
 // The order of the dimensions inside an MMA is free as long as both operands agree, so a lane takes 16 neighbouring dimensions of a token's key -- one scale -- for four steps, and
 // eight of a value.  For the values two tokens' codes are brought side by side while they are still 4 bits wide (two logic operations for sixteen numbers).
-// A warp works alone on every fourth tile of 32 tokens of the CTA's split: a ring of bulk copies of its own, its own maxima, sums and outputs; the warps meet in
+// A warp of W works alone on every W-th tile of 32 tokens of the CTA's split: a ring of bulk copies of its own, its own maxima, sums and outputs; the warps meet in
 // shared memory at the end, splits of the context in quantized_merge_kernel.
 //
 // Bound: turning 4 bits into halves.  A tile of 16 tokens of a head of 128 (2304 bytes, 100 cycles of an SM's share of the memory) costs 64 conversions and some 40 logic
