@@ -262,11 +262,17 @@ int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int precision, 
                               void* q_dev, void* k_dev, void* stream);
 /* Attention over the 4-bit cache on stacked projections proj fp32 [rows, in.outputs]: norm, rotation, rounding and append at
  * positions_dev[slot] .., attention, output gate -> out (precision's type) [rows, heads*dim].  cache_dev [slots][kv_heads][capacity]
- * [row bytes], 16-byte aligned; slots_dev names distinct slots, context covers every sequence's tokens; rows behind a sequence's last token are neither used nor written, whatever they hold.  A token past the capacity or the
- * rotary tables sets TBL_DEV_CACHE_FULL; the rows of its sequence are undefined, the cache holds what has room.  positions_dev is not
- * advanced, so that a repeated call writes the same rows again.  route: 0 as the step, 1 fp32 arithmetic on the 4-bit rows, 2 the
- * cache-streaming kernel (warp-level MMAs on the 4-bit rows), 3 the flash kernel (tcgen05) over expanded keys and values, as far as its
- * tiles have room (dim <= 192); 2 and 3 take bf16 only.  With route 0 the workspace of a context serves every shorter one.  A number that is not finite reaches the rows that see its token, and may reach those of the same call and sequence before it. */
+ * [row bytes], 16-byte aligned; slots_dev names distinct slots, context covers every sequence's tokens; rows behind a sequence's last
+ * token are neither used nor written, whatever they hold.  A token past the capacity or the rotary tables sets TBL_DEV_CACHE_FULL; the
+ * rows of its sequence are undefined, the cache holds what has room.  positions_dev is not advanced, so that a repeated call writes the
+ * same rows again.  A number that is not finite reaches the rows that see its token, and may reach those of the same call and sequence
+ * before it.
+ * route: 0 as the step, 1 fp32 arithmetic on the 4-bit rows, 2 the cache-streaming kernel (warp-level MMAs on the 4-bit rows), 3 the flash
+ * kernel (tcgen05) over expanded keys and values, as far as its tiles have room (dim <= 192).  2 and 3 take bf16 only, and round queries
+ * and softmax weights to fp16: 2^-12 of a number; weights below 2^-25 of a row's largest lose bits, below 2^-35 they are left out.
+ * With route 0 the workspace of a context serves every shorter one.  Route 3 (and 0, where it takes it: portions of a prompt) holds
+ * every key and value up to the context as fp16 in the workspace, 4 bytes * dim for each token, key/value head and sequence: three and a
+ * half times what the cache takes for them. */
 int tbl_quantized_row_bytes(const tbl_quantized_mixer* mixer);
 size_t tbl_quantized_workspace_bytes(const tbl_quantized_mixer* mixer, int precision, int route, int n_seq, int n_tok, int context);
 int tbl_quantized_forward(const tbl_quantized_mixer* mixer, int precision, int route, float eps, const float* proj_dev, void* cache_dev,
@@ -279,9 +285,13 @@ int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const vo
                        void* stream);
 /* Linear attention with decay on stacked projections proj fp32 [rows, in.outputs]: norm, rotation, recurrence, head norm, output gate -> out
  * (precision's type) [rows, heads*dim].  states_dev fp32 [slots][heads][dim][dim] are read, next_states_dev (the same array, or another of
- * its shape) receives those after the last token; slots_dev names distinct slots, the others are not touched.  A token past the rotary tables sets TBL_DEV_CACHE_FULL; the rows and
- * states of its sequence are undefined.  Projections are finite: a prompt is worked out in blocks, in which one that is not spoils other rows.  route: 0 as the step, 1 the scan kernel (any size, fp32
- * arithmetic), 2 the chunk kernels (tcgen05; bf16, dim <= 128).  With route 0 the workspace of a number of tokens serves every smaller one. */
+ * its shape) receives those after the last token; slots_dev names distinct slots, the others are not touched.  A token past the rotary
+ * tables sets TBL_DEV_CACHE_FULL; the rows and states of its sequence are undefined.  Projections are finite: a prompt is worked out in
+ * blocks, in which one that is not spoils other rows.
+ * route: 0 as the step, 1 the scan kernel (any size, fp32 arithmetic; up to four tokens in one launch where the head size is a multiple of
+ * four and the state fits shared memory: below 224, four tokens 216), 2 the chunk kernels (tcgen05; bf16, dim <= 128): states from products
+ * of 22 bits, outputs from operands rounded to fp16 (2^-12 of a number, down to 2^-28 of the largest of its token, state row or row of
+ * weights).  With route 0 the workspace of a number of tokens serves every smaller one. */
 size_t tbl_decay_workspace_bytes(const tbl_decay_mixer* mixer, int precision, int route, int n_seq, int n_tok);
 int tbl_decay_forward(const tbl_decay_mixer* mixer, int precision, int route, float eps, const float* proj_dev, const float* states_dev,
                       float* next_states_dev, const int32_t* slots_dev, const int32_t* positions_dev, int n_seq, int n_tok, void* out_dev,

@@ -6,8 +6,8 @@
 //   decay_starts_kernel      long scans of few heads: the states before segments of the tokens, which are then scanned side by side
 // Prompts in bf16 go by chunks (decay_chunk.cu).
 //
-// The decay enters as S + (exp(log_decay) - 1) S: 1 - exp(log_decay) has 24 bits however slow the decay is, whereas a decay rounded to fp32 would be off by 2^-25
-// every token, all in one direction.
+// The decay enters as S + (exp(log_decay) - 1) S: 1 - exp(log_decay) has 24 bits however slow the decay is, whereas a decay rounded to fp32 would be
+// off by 2^-25 every token, all in one direction.
 #include <float.h>
 
 #include "decay.cuh"
@@ -23,9 +23,9 @@ using flash::unpair;
 
 constexpr int kThreads = 256, kTile = 8, kStepTokens = 4, kMostSegments = 8;
 
-// LK lanes share a value row's keys: lane a holds 4 a + 4 LK j + e for j < C, in pairs of fp32.  A lane holds R rows, a warp 32 / LK times as many.  Lanes along
-// the keys, so that what all rows multiply with comes out of shared memory in whole lines (eight lanes a row: 328 lines a token for 32 rows of 90, and
-// they were the bound).
+// LK lanes share a value row's keys: lane a holds 4 a + 4 LK j + e for j < C, in pairs of fp32.  A lane holds R rows, a warp 32 / LK times as many.
+// Lanes along the keys, so that what all rows multiply with comes out of shared memory in whole lines (eight lanes a row: 328 lines a token for 32
+// rows of 90, and they were the bound).
 template <int LK, int C, int R>
 struct State {
     static constexpr int kKeys = 4 * LK * C, kRows = 32 / LK * R;
@@ -203,11 +203,12 @@ __device__ __forceinline__ void finish_head(const DecayParams& p, const float* s
     }
 }
 
-// Up to four tokens of a head in one launch (32 heads of 128, four tokens 9.2 us, eight 14.1, the scan of nine 11.0; 16 sequences 21.8, 34.7 and 31.7).  A CTA has the whole head: its state comes into shared memory by one bulk copy and goes back by another, so that registers
-// hold a few rows at a time and three CTAs of heads of 128 share an SM; while it comes, a warp each norms and turns the tokens' queries and keys.  Bound by the
-// state's bytes: the projections are asked for first, or they would queue behind the states of the whole batch (64 sequences of 32 heads of 128: 49.7 us, 5.5 TB/s; with
-// the state in registers 65 to 79).  The bound on registers is what three CTAs have (left to itself the compiler takes 47 instead of 60, with fewer loads on
-// their way: 51).
+// Up to four tokens of a head in one launch (32 heads of 128, four tokens 9.2 us, eight 14.1, the scan of nine 11.0; 16 sequences 21.8, 34.7 and
+// 31.7).  A CTA has the whole head: its state comes into shared memory by one bulk copy and goes back by another, so that registers hold a few rows
+// at a time and three CTAs of heads of 128 share an SM; while it comes, a warp each norms and turns the tokens' queries and keys.  Bound by the
+// state's bytes: the projections are asked for first, or they would queue behind the states of the whole batch (64 sequences of 32 heads of 128: 49.7
+// us, 5.5 TB/s; with the state in registers 65 to 79).  The bound on registers is what three CTAs have (left to itself the compiler takes 47 instead
+// of 60, with fewer loads on their way: 51).
 constexpr size_t kStepRoom = 200 * 1024;
 size_t step_smem(int keys, int d, int n_tok) { return sizeof(float) * (static_cast<size_t>(d) * d + static_cast<size_t>(n_tok) * (2 * keys + 3 * d)); }
 
@@ -300,15 +301,16 @@ __device__ __forceinline__ void copy4(float* dst, const float* src, bool ok) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
 
-// Any number of tokens: a CTA of four warps has 4 State::kRows rows of a head, and a segment of the tokens.  Their vectors come by tiles of kTile ahead of their
-// use, a thread the same columns of every token; two tokens' instructions mix.  Bound by a token's chain (0.2 us) where a block has an SM to itself, by fp32 operations and
-// shared memory where several share one (62 % of the issue slots).  SUMS: from an empty state, and only the state after the segment, which is the start of
-// the next (decay_starts_kernel adds what came before).
+// Any number of tokens: a CTA of four warps has 4 State::kRows rows of a head, and a segment of the tokens.  Their vectors come by tiles of kTile
+// ahead of their use, a thread the same columns of every token; two tokens' instructions mix.  Bound by a token's chain (0.2 us) where a block has an
+// SM to itself, by fp32 operations and shared memory where several share one (62 % of the issue slots).  SUMS: from an empty state, and only the
+// state after the segment, which is the start of the next (decay_starts_kernel adds what came before).
 constexpr int kScanThreads = 128;
 template <int LK, int C, int R, bool SUMS>
 __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayParams p) {
     using S = State<LK, C, R>;
-    constexpr int kRows = kScanThreads / 32 * S::kRows, kFirst = SUMS ? S::kKeys : 0, kCols = 2 * S::kKeys + kRows, kPer = (kCols - kFirst + kScanThreads - 1) / kScanThreads;
+    constexpr int kRows = kScanThreads / 32 * S::kRows, kFirst = SUMS ? S::kKeys : 0, kCols = 2 * S::kKeys + kRows;
+    constexpr int kPer = (kCols - kFirst + kScanThreads - 1) / kScanThreads;
     __shared__ __align__(16) float vec_s[2][kTile][kCols];       // queries, keys, values
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = lane % LK, first = warp * S::kRows + lane / LK * R;
     const int head = blockIdx.x % p.H, seq = blockIdx.x / p.H, row0 = blockIdx.y * kRows, part = blockIdx.z;
@@ -360,8 +362,10 @@ __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayPar
         const int n = min(kTile, tokens - t0);
         if constexpr (SUMS) {
 #pragma unroll 2
-            for (int t = 0; t < n; ++t)
-                s.add(expf(t0 + t == tokens - 1 ? 0.0f : rate * static_cast<float>(tokens - 1 - t0 - t)), vec_s[buf][t] + S::kKeys, vec_s[buf][t] + 2 * S::kKeys + first, share);
+            for (int t = 0; t < n; ++t) {
+                const float kept = expf(t0 + t == tokens - 1 ? 0.0f : rate * static_cast<float>(tokens - 1 - t0 - t));       // (a branch: 60 us instead of 58)
+                s.add(kept, vec_s[buf][t] + S::kKeys, vec_s[buf][t] + 2 * S::kKeys + first, share);
+            }
             continue;
         }
         auto token = [&](int t, float (&a)[R]) {
@@ -453,12 +457,13 @@ template <int LK, int C, int R>
 cudaError_t launch_scan_r(const DecayParams& p, cudaStream_t st) {
     const unsigned units = p.n_seq * p.H, rows = ceil_div(p.d, kScanThreads / 32 * State<LK, C, R>::kRows);
     if (p.n_tok <= kTile) return launch_dependent(decay_scan_kernel<LK, C, R, false>, dim3(units, rows), dim3(kScanThreads), 0, st, p);
-    // Behind a kernel of many rows an early launch finds room on few SMs and stays there, several blocks to one (2000 tokens of 8 heads of 128: 263 and 119 us, three
-    // prompts of 301 tokens, 10 heads of 90, 59 and 54).
+    // Behind a kernel of many rows an early launch finds room on few SMs and stays there, several blocks to one (2000 tokens of 8 heads of 128: 263
+    // and 119 us, three prompts of 301 tokens, 10 heads of 90, 59 and 54).
     if (p.segments > 1) {
         decay_scan_kernel<LK, C, R, true><<<dim3(units, rows, p.segments - 1), kScanThreads, 0, st>>>(p);
         note_launch();
-        const cudaError_t e = launch_dependent(decay_starts_kernel, dim3(ceil_div(p.d * State<LK, C, R>::kKeys, 256), units), dim3(256), 0, st, p, State<LK, C, R>::kKeys);
+        constexpr int keys = State<LK, C, R>::kKeys;
+        const cudaError_t e = launch_dependent(decay_starts_kernel, dim3(ceil_div(p.d * keys, 256), units), dim3(256), 0, st, p, keys);
         if (e != cudaSuccess) return e;
     }
     decay_scan_kernel<LK, C, R, false><<<dim3(units, rows, p.segments), kScanThreads, 0, st>>>(p);
@@ -475,9 +480,10 @@ cudaError_t launch_scan(const DecayParams& p, cudaStream_t st) {
         default: return launch_scan_r<32, 2, 8>(p, st);
     }
 }
-// Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; with segments the tokens are read twice, by more blocks.  Times in us: a
-// token 0.2 where a block has an SM to itself, 0.1 for each block where they share one, sums alone half of that; the other two launches 9.5.  Fewest of that wins (fp32,
-// without and with: three prompts of 301 tokens, 10 heads of 90, 75 and 54; 32 heads of 128, 64 tokens 22 and 28, 300 tokens 72 and 64; 8 heads, 2000 tokens 405 and 119).
+// Segments of a scan: a block takes its tokens one after the other, so few heads leave the GPU empty; with segments the tokens are read twice, by
+// more blocks.  Times in us: a token 0.2 where a block has an SM to itself, 0.1 for each block where they share one, sums alone half of that; the
+// other two launches 9.5.  Fewest of that wins (fp32, without and with: three prompts of 301 tokens, 10 heads of 90, 75 and 54; 32 heads of 128, 64
+// tokens 22 and 28, 300 tokens 72 and 64; 8 heads, 2000 tokens 405 and 119).
 int scan_segments(int heads, int d, int n_seq, int n_tok) {
     const long long units = static_cast<long long>(n_seq) * heads;
     const int keys = keys_of(d), lanes = keys <= 32 ? 8 : keys <= 64 ? 16 : 32;
@@ -490,8 +496,8 @@ int scan_segments(int heads, int d, int n_seq, int n_tok) {
 }
 
 enum Route { kAuto = 0, kScan = 1, kChunk = 2 };
-// Tokens from which the chunks are faster than the scan: few heads leave both waiting for one chain (32 heads of 128, scan and chunks: 48 tokens 19 and 23 us, 64 27 and
-// 24; 256 heads: 48 tokens 55 and 50).
+// Tokens from which the chunks are faster than the scan: few heads leave both waiting for one chain (32 heads of 128, scan and chunks: 48 tokens 19
+// and 23 us, 64 27 and 24; 256 heads: 48 tokens 55 and 50).
 int chunk_min_tokens(long long units) { return units >= kNumSm ? 48 : 64; }
 
 struct Plan {

@@ -9,10 +9,11 @@
 // Queries and keys are normed and turned where they are read, from the fp32 projections, which pass through memory once.  A long prompt goes by pieces whose
 // operands and sums stay in the second-level cache between the three kernels.
 //
-// Precision.  The states are sums over the whole sequence and stay fp32: their products take both operands as two fp16 terms each (22 bits, three products; numbers
-// 2^-14 below a tile's largest keep fewer).  Outputs are rounded to bf16, so their operands are single fp16 terms under a power of two for every token, and for every
-// row of a state: errors of 2^-12.  They are brought up to 2^14, so that numbers down to 2^-28 of the largest beside them keep their bits.  A weight y^(i-j) (q_i . k_j) carries the factors of its key and value, and is an fp16 beside the largest weight of its row: a
-// token that a row does not see, or has forgotten, takes no bits from it.
+// Precision.  The states are sums over the whole sequence and stay fp32: their products take both operands as two fp16 terms each (22 bits, three
+// products; numbers 2^-14 below a tile's largest keep fewer).  Outputs are rounded to bf16, so their operands are single fp16 terms under a power of
+// two for every token, and for every row of a state: errors of 2^-12.  They are brought up to 2^14, so that numbers down to 2^-28 of the largest
+// beside them keep their bits.  A weight y^(i-j) (q_i . k_j) carries the factors of its key and value, and is an fp16 beside the largest weight of
+// its row: a token that a row does not see, or has forgotten, takes no bits from it.
 #include <cuda_fp16.h>
 
 #include "decay.cuh"
@@ -50,8 +51,9 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t addr, int box) {
 // place of column c of row r in tiles of 64 columns, `tile` bytes each
 __device__ __forceinline__ uint32_t swizzled(int r, int c, int tile) { return (c >> 6) * tile + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2; }
 
-// A head's numbers over the lanes of a warp: LPH lanes for a token, 32 / LPH tokens side by side, eight numbers a lane in units of 2 V (head_rotation.cuh).  What
-// does not change from token to token stays in registers: a run's columns, and its place in a row of operands.  EXACT: the head is DP wide.
+// A head's numbers over the lanes of a warp: LPH lanes for a token, 32 / LPH tokens side by side, eight numbers a lane in units of 2 V
+// (head_rotation.cuh).  What does not change from token to token stays in registers: a run's columns, and its place in a row of operands.  EXACT: the
+// head is DP wide.
 template <int DP, int V, bool EXACT>
 struct HeadLane {
     static constexpr int kLph = V == 4 ? DP / 8 : 32, kSide = 32 / kLph, kUnits = 4 / V, kRuns = 2 * kUnits;
@@ -173,17 +175,18 @@ __device__ __forceinline__ void fetch_ahead(const ChunkParams& c, int column0, i
 __device__ __forceinline__ int table_row(const DecayParams& p, int pos) { return p.r.half > 0 ? min(max(pos, 0), p.r.positions - 1) : 0; }
 
 // ---- sums of the chunks -----------------------------------------------------------------------------------------------------------------
-// One CTA per (unit, chunk), two tiles of 64 tokens: D[value][key] = sum over a tile's tokens, M = 128 values (of which DP count), N = DP keys; both operands lie as they
-// come, a row per token.  Keys are divided by their power of two, values (times the decay to the chunk's end) by the tile's largest, both then brought up to 2^14, where
-// fp16 has room below: two terms hold 22 bits, three products 22 bits of the sums, which a tile has in columns of its own.  The keys' first terms and the values
-// go to decay_chunk_kernel on the way, as the tiles that it multiplies.  The second tile's rows are asked for as soon as the first one's registers are free.  Bound by the
-// way of the rows to the registers (35 % of the issue slots, 40 % of the stalls wait for loads); registers and tensor memory leave two CTAs to an SM.  64 chunks of 32 heads:
-// 149 us for 537 MB in and out, 3.6 TB/s.
+// One CTA per (unit, chunk), two tiles of 64 tokens: D[value][key] = sum over a tile's tokens, M = 128 values (of which DP count), N = DP keys; both
+// operands lie as they come, a row per token.  Keys are divided by their power of two, values (times the decay to the chunk's end) by the tile's
+// largest, both then brought up to 2^14, where fp16 has room below: two terms hold 22 bits, three products 22 bits of the sums, which a tile has in
+// columns of its own.  The keys' first terms and the values go to decay_chunk_kernel on the way, as the tiles that it multiplies.  The second tile's
+// rows are asked for as soon as the first one's registers are free.  Bound by the way of the rows to the registers (35 % of the issue slots, 40 % of
+// the stalls wait for loads); registers and tensor memory leave two CTAs to an SM.  64 chunks of 32 heads: 150 us for 537 MB in and out, 3.6 TB/s.
 constexpr float kHighest = 60.0f;                        // (a score of two such heads ends below 2^35)
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
-    constexpr int kSumWarps = kSumThreads / 32, kPiece = DP / 64 * kBox, kTile = DP / 64 * kSub, kPerWarp = 64 / kSumWarps, kRounds = kPerWarp / Lane::kSide, kRuns = Lane::kRuns;
+    constexpr int kSumWarps = kSumThreads / 32, kPiece = DP / 64 * kBox, kTile = DP / 64 * kSub, kPerWarp = 64 / kSumWarps;
+    constexpr int kRounds = kPerWarp / Lane::kSide, kRuns = Lane::kRuns;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ __align__(8) uint64_t done;
@@ -338,7 +341,8 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
 }
 
 // ---- states before the chunks -----------------------------------------------------------------------------------------------------------
-// DP / 8 lanes share a row (a value's keys), eight neighbouring keys each; the next eight chunks' sums are on their way.  64 chunks of 32 heads: 53 us for 201 MB.
+// DP / 8 lanes share a row (a value's keys), eight neighbouring keys each; the next eight chunks' sums are on their way.  64 chunks of 32 heads: 53
+// us for 201 MB.
 template <int DP>
 __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
     constexpr int kLph = DP / 8, kSide = 32 / kLph;
@@ -395,10 +399,11 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 }
 
 // ---- outputs of the chunks ----------------------------------------------------------------------------------------------------------------
-// One CTA per (unit, chunk).  Scores Q K^T in the first 128 columns of its tensor memory, weights in their place (fp16, the A operand of the second product), the
-// tokens' part of the outputs behind them, then the state's part over the weights.  Keys and values come by bulk copies while the queries are normed, the state's operand
-// by another into the keys' room.  Outputs are collected in shared memory, so that gates are read and rows are written whole.  512 threads, since it is their loads and
-// barriers that take the time (43 % of the issue slots; with 256 threads 174 instead of 163 us): 64 chunks of 32 heads 156 us for 537 MB, 3.4 TB/s.
+// One CTA per (unit, chunk).  Scores Q K^T in the first 128 columns of its tensor memory, weights in their place (fp16, the A operand of the second
+// product), the tokens' part of the outputs behind them, then the state's part over the weights.  Keys and values come by bulk copies while the
+// queries are normed, the state's operand by another into the keys' room.  Outputs are collected in shared memory, so that gates are read and rows
+// are written whole.  512 threads, since it is their loads and barriers that take the time (44 % of the issue slots; with 256 threads 174 instead of
+// 163 us): 64 chunks of 32 heads 160 us for 537 MB, 3.4 TB/s.
 template <int DP, int V, bool EXACT>
 __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const ChunkParams c) {
     using Lane = HeadLane<DP, V, EXACT>;
@@ -541,7 +546,8 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
         const float f = inverse_power(row_power) * kUp;
         uint32_t y[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = ch <= (warp & 3) ? bits_of(__floats2half2_rn(__uint_as_float(x[2 * e]) * f, __uint_as_float(x[2 * e + 1]) * f)) : 0u;
+        for (int e = 0; e < 16; ++e)
+            y[e] = ch <= (warp & 3) ? bits_of(__floats2half2_rn(__uint_as_float(x[2 * e]) * f, __uint_as_float(x[2 * e + 1]) * f)) : 0u;
         tmem_st16(tmem + lanes + ch * 32, y);
     }
     tmem_st_wait();
@@ -637,8 +643,9 @@ __global__ void __launch_bounds__(kOutThreads, 2) decay_chunk_kernel(const Chunk
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
 int width_of(int dim) { return dim <= 64 ? 64 : 128; }
 
-// Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes, and the two large kernels' last CTAs fill the GPU (8192
-// tokens of 32 heads: pieces of 9, 18, 37 and 64 chunks take 433, 414, 404 and 411 us, 39 chunks 418).
+// Chunks of a piece for each sequence: keys, values and what is made of them stay within this many bytes, and the two large kernels' last CTAs fill
+// the GPU (8192 tokens of 32 heads, before weights had their row's maximum, which costs 2 us: pieces of 9, 18, 37 and 64 chunks take 433, 414, 404 and 411 us,
+// 39 chunks 418).
 constexpr size_t kPieceBytes = 352u << 20;
 int most_chunks(const tbl_decay_mixer& m, int n_seq, int n_tok) {
     const size_t w = width_of(m.dim), chunk = static_cast<size_t>(n_seq) * m.heads * (kTokens * (m.dim * 8 + w * 4) + w * w * 6), most = kPieceBytes / chunk;
@@ -705,7 +712,8 @@ int launch_decay_chunks(const tbl_decay_mixer& m, const DecayParams& p, void* ws
     ChunkParams c{};
     c.d = p;
     c.per_dim = 1.0f / static_cast<float>(p.d);
-    c.sums = reinterpret_cast<float*>(base + r.sums); c.tokens = base + r.tokens; c.powers = reinterpret_cast<float*>(base + r.powers); c.images = base + r.images; c.scales = reinterpret_cast<float*>(base + r.scales);
+    c.sums = reinterpret_cast<float*>(base + r.sums); c.tokens = base + r.tokens; c.powers = reinterpret_cast<float*>(base + r.powers);
+    c.images = base + r.images; c.scales = reinterpret_cast<float*>(base + r.scales);
     const int per = chunks_of(m, p.n_seq, p.n_tok);
     const cudaError_t e = width_of(m.dim) == 64 ? run_width<64>(c, per, st) : run_width<128>(c, per, st);
     return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;

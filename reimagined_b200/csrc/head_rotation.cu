@@ -22,8 +22,8 @@ struct RotationParams {
 
 constexpr int kMostThreads = 256;
 
-// LPH lanes a head, U units a lane.  A thread has the same columns of every head it takes: their places and weights stay in registers, a row's angles for all its
-// heads.  HALVES: queries as fp16 under a power of two (RotationCall).
+// LPH lanes a head, U units a lane.  A thread has the same columns of every head it takes: their places and weights stay in registers, a row's angles
+// for all its heads.  HALVES: queries as fp16 under a power of two (RotationCall).
 template <typename T, int V, int LPH, int U, bool HALVES, bool EXACT>
 __global__ void __launch_bounds__(kMostThreads, V == 4 ? 6 : 4) head_rotation_kernel(const RotationParams p) {
     using Units = HeadUnits<V, LPH>;
@@ -124,7 +124,8 @@ int launch_head_rotation(const tbl_head_rotation& r, int precision, const Rotati
     p.rows = c.n_seq * c.n_tok; p.ldq = c.ldq; p.per_dim = 1.0f / static_cast<float>(c.dim);
     // runs of four or two numbers where everything lies on their bytes
     const int run = vector_heads(r, c.dim, c.proj, c.ld) && aligned16(c.q) && aligned16(c.k) ? 4 : paired_heads(r, c.dim, c.proj, c.ld, c.q, c.k) ? 2 : 1;
-    const cudaError_t e = c.q_factor ? launch_type<__half, true>(p, run, st) : precision == TBL_BF16 ? launch_type<bf16, false>(p, run, st) : launch_type<float, false>(p, run, st);
+    const cudaError_t e = c.q_factor ? launch_type<__half, true>(p, run, st) : precision == TBL_BF16 ? launch_type<bf16, false>(p, run, st)
+                                                                                                     : launch_type<float, false>(p, run, st);
     return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
 
@@ -149,6 +150,7 @@ extern "C" int tbl_head_rotation_forward(const tbl_head_rotation* rotation, int 
     if ((reinterpret_cast<uintptr_t>(proj_dev) & 3) || (q_heads > 0 && (reinterpret_cast<uintptr_t>(q_dev) & own)) ||
         (k_heads > 0 && (reinterpret_cast<uintptr_t>(k_dev) & own)))
         return TBL_ERR_ALIGNMENT;
-    const RotationCall c{proj_dev, ld, q_heads, k_heads, dim, slots_dev, positions_dev, n_seq, n_tok, eps, q_heads > 0 ? q_dev : nullptr, k_heads > 0 ? k_dev : nullptr, nullptr, 0};
+    const RotationCall c{proj_dev, ld, q_heads, k_heads, dim, slots_dev, positions_dev, n_seq, n_tok, eps,
+                         q_heads > 0 ? q_dev : nullptr, k_heads > 0 ? k_dev : nullptr, nullptr, 0};
     return launch_head_rotation(*rotation, precision, c, static_cast<cudaStream_t>(stream));
 }

@@ -38,9 +38,9 @@ __device__ __forceinline__ void turn_unit(int interleaved, const float* c, const
     }
 }
 
-// A head spread over LPH lanes, in units of 2 V numbers: V pairs (a, b) that turn together, or numbers that do not turn.  Without `interleaved` a unit that
-// turns is two runs of V neighbours half a rotated part apart, otherwise it is 2 V neighbours.  V = 4: 16-byte accesses (vector_heads below), V = 2: 8-byte ones
-// (paired_heads), V = 1: any size.
+// A head spread over LPH lanes, in units of 2 V numbers: V pairs (a, b) that turn together, or numbers that do not turn.  Without `interleaved` a
+// unit that turns is two runs of V neighbours half a rotated part apart, otherwise it is 2 V neighbours.  V = 4: 16-byte accesses (vector_heads
+// below), V = 2: 8-byte ones (paired_heads), V = 1: any size.
 template <int V, int LPH>
 struct HeadUnits {
     static constexpr int kUnits = V == 4 ? 1 : TBL_MAX_ROTATED_DIM / (2 * V) / LPH;      // vectors: callers choose LPH >= dim / 8
@@ -173,9 +173,9 @@ __device__ __forceinline__ float power_below(float v) {
     const uint32_t power = min(__float_as_uint(v) >> 23, 253u);
     return power ? __uint_as_float(power << 23) : 1.0f;
 }
-// Numbers as fp16: under the power of two at or below the largest of them (2^-113 at least, also for zeros, which so count less than anything else), and
-// brought up by kUp to below 2^14, so that those 2^-28 below the largest keep their bits.  The largest itself, not what a norm allows: weights may be uneven, the norm's
-// epsilon may rule, tables may scale.
+// Numbers as fp16: under the power of two at or below the largest of them (2^-113 at least, also for zeros, which so count less than anything else),
+// and brought up by kUp to below 2^14, so that those 2^-28 below the largest keep their bits.  The largest itself, not what a norm allows: weights
+// may be uneven, the norm's epsilon may rule, tables may scale.
 constexpr float kUp = 8192.0f, kUpBits = 13.0f;
 __device__ __forceinline__ float power_of(float most) { return power_below(fmaxf(most, 0x1p-113f)); }
 // one over a power of two

@@ -1,7 +1,8 @@
 // Shared by the translation units of the attention over a 4-bit cache (quantized_attention.cu, quantized_decode.cu, quantized_rows.cu).
 //
-// Cache of a layer: [slot][kv head][token][row], a row being, with n = the head size rounded up to 64, n/2 bytes of key codes, n/2 of value codes, n/16
-// scale bytes of the key, n/16 of the value, and zeros to a multiple of 16.  One token of a head is one contiguous row, so that a tile of tokens is one bulk copy.
+// Cache of a layer: [slot][kv head][token][row], a row being, with n = the head size rounded up to 64, n/2 bytes of key codes, n/2 of value codes,
+// n/16 scale bytes of the key, n/16 of the value, and zeros to a multiple of 16.  One token of a head is one contiguous row, so that a tile of tokens
+// is one bulk copy.
 #pragma once
 
 #include <cuda_fp4.h>
@@ -72,8 +73,9 @@ __device__ __forceinline__ uint32_t quantize8(const float (&x)[8], float unit, u
     return codes;
 }
 
-// A head of a row: for a key (turned = its rotation) normed and turned in 64 bits, so that the code of a number does not depend on how a sum of squares is rounded;
-// then rounded to 4 bits.  A warp; `mine`: its room for the head's numbers; lane i has the codes of numbers 8 i .. 8 i + 7, even lanes the scale of 16.
+// A head of a row: for a key (turned = its rotation) normed and turned in 64 bits, so that the code of a number does not depend on how a sum of
+// squares is rounded; then rounded to 4 bits.  A warp; `mine`: its room for the head's numbers; lane i has the codes of numbers 8 i .. 8 i + 7, even
+// lanes the scale of 16.
 template <int V>
 __device__ __forceinline__ uint32_t quantize_head(const QuantizedParams& p, const float* src, bool is_k, int at, float* mine, int lane, uint8_t& scale) {
     for (int c = p.d + lane; c < p.width; c += 32) mine[c] = 0.0f;

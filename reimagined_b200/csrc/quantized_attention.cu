@@ -3,8 +3,9 @@
 //   quantized_prep_kernel    norm and rotation of queries and keys, rounding of keys and values to 4 bits, append
 //   quantized_expand_kernel  the visible cache as numbers: code x scale has six bits between 2^-10 and 2688, which fp16 holds
 //   quantized_read_kernel    the same for single tokens, in the layer's units
-// Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, and weights need one term instead of two), a few query rows
-// over the 4-bit rows themselves (quantized_decode.cu), fp32 and what else there is in fp32 arithmetic (quantized_rows.cu).  The layer's units enter as factors of the scores and of the output.
+// Prompts go over expanded keys and values through the flash kernel of attention_prefill.cu (in fp16: queries and weights err by 2^-12, down to 2^-25
+// of the largest weight, and weights need one term instead of two), a few query rows over the 4-bit rows themselves (quantized_decode.cu), fp32 and
+// what else there is in fp32 arithmetic (quantized_rows.cu).  The layer's units enter as factors of the scores and of the output.
 #include <math.h>
 
 #include "attention.cuh"
@@ -175,15 +176,17 @@ bool flash_fits(const tbl_quantized_mixer& m, int n_seq, int context) {
     return attention_flash_supported(as_attention(m)) && static_cast<long long>(n_seq) * m.kv_heads * round_up(context, 128) <= 2147483647LL;
 }
 
-// bf16: the flash kernel where its time, worked out from what it took, is shorter than the streaming kernel's (32 query and 8 key/value heads of 128, in us, streaming and
-// flash kernel: one sequence of 64 tokens over 1024 20 and 43, over 16384 97 and 287; 256 over 4096 115 and 109; 512 over 512 58 and 45; eight sequences of 64 over
-// 4096 193 and 233, of 128 over 128 86 and 64, over 4096 372 and 244).  Both read or walk the context: the one for every block of 8 or 16 query rows, the other a wave of CTAs at a time.
+// bf16: the flash kernel where its time, worked out from what it took, is shorter than the streaming kernel's (32 query and 8 key/value heads of 128,
+// in us, streaming and flash kernel: one sequence of 64 tokens over 1024 20 and 43, over 16384 97 and 287; 256 over 4096 115 and 109; 512 over 512 58
+// and 45; eight sequences of 64 over 4096 193 and 233, of 128 over 128 86 and 64, over 4096 372 and 244).  Both read or walk the context: the one for
+// every block of 8 or 16 query rows, the other a wave of CTAs at a time.
 int pick_route(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context) {
     if (precision != TBL_BF16) return kSimt;
     if (!flash_fits(m, n_seq, context)) return kStream;
     const double rows = static_cast<double>(n_seq) * n_tok, caches = static_cast<double>(n_seq) * m.kv_heads * quantized_width(m.dim) / 128;
     const double seen = context - 0.5 * n_tok, group = m.heads / m.kv_heads;
-    const double blocks = ceil(n_tok * group / quantized_stream_rows(m, n_tok)), waves = ceil(n_seq * static_cast<double>(m.heads) * ceil_div(n_tok, 256) / kNumSm);
+    const double blocks = ceil(n_tok * group / quantized_stream_rows(m, n_tok));
+    const double waves = ceil(n_seq * static_cast<double>(m.heads) * ceil_div(n_tok, 256) / kNumSm);
     const double stream = 11 + 1.8e-3 * rows * m.heads + 42e-6 * caches * blocks * seen * (m.dim > 128 ? 0.7 : 1.0);
     const double flash = 23 + 0.57e-3 * rows * (m.heads + 2 * m.kv_heads) + 250e-6 * caches * context + 0.014 * waves * seen;
     return flash < stream ? kFlash : kStream;
@@ -225,8 +228,8 @@ Plan make_plan(const tbl_quantized_mixer& m, int precision, int route, int n_seq
     return w;
 }
 
-// Bytes of a route.  Without one (0), room for whatever a context no longer than this one takes: a host may ask once for the longest.  (Both times in pick_route are
-// straight lines over the context, so the flash kernel is taken somewhere below only if it is at one end.)
+// Bytes of a route.  Without one (0), room for whatever a context no longer than this one takes: a host may ask once for the longest.  (Both times in
+// pick_route are straight lines over the context, so the flash kernel is taken somewhere below only if it is at one end.)
 size_t bytes_of(const tbl_quantized_mixer& m, int precision, int route, int n_seq, int n_tok, int context) {
     if (route != kAuto || precision != TBL_BF16) return make_plan(m, precision, route, n_seq, n_tok, context).bytes;
     const size_t bytes = make_plan(m, precision, kStream, n_seq, n_tok, context).bytes;
@@ -298,7 +301,8 @@ int check_quantized(const tbl_quantized_mixer& m, int width) {
     if (m.heads <= 0 || m.kv_heads <= 0 || m.heads > 65535 || m.heads % m.kv_heads) return TBL_ERR_SHAPE;
     const int rc = check_rotation(m.rotation, m.dim);
     if (rc != TBL_OK) return rc;
-    if (!(m.key_scale > 0.0f) || !(m.value_scale > 0.0f) || m.key_scale > 1e30f || m.value_scale > 1e30f || m.key_scale < 1e-30f || m.value_scale < 1e-30f) return TBL_ERR_SCALE;
+    auto unit = [](float s) { return s >= 1e-30f && s <= 1e30f; };
+    if (!unit(m.key_scale) || !unit(m.value_scale)) return TBL_ERR_SCALE;
     const double factor = static_cast<double>(m.scale) * m.key_scale;       // of the scores: the flash kernel takes their largest before it
     if (!(factor >= 1e-30 && factor <= 1e30)) return TBL_ERR_SCALE;
     if (m.gated != 0 && m.gated != 1) return TBL_ERR_INVALID_ARG;
@@ -319,18 +323,21 @@ int launch_quantized(const tbl_quantized_mixer& m, int precision, int route, flo
                      const int32_t* positions, int n_seq, int n_tok, int context, void* out, void* ws, cudaStream_t st) {
     const Plan w = make_plan(m, precision, route, n_seq, n_tok, context);
     const long long rows = static_cast<long long>(n_seq) * n_tok;
-    if (rows > 2147483647LL || static_cast<long long>(n_seq) * m.kv_heads > 65535 || ceil_div(m.heads + 2 * m.kv_heads, kPrepWarps) > 65535 || w.splits > 65535) return TBL_ERR_SHAPE;
+    if (rows > 2147483647LL || static_cast<long long>(n_seq) * m.kv_heads > 65535 || ceil_div(m.heads + 2 * m.kv_heads, kPrepWarps) > 65535 ||
+        w.splits > 65535)
+        return TBL_ERR_SHAPE;
     // blocks of query rows are one side of a grid
     const long long total = static_cast<long long>(n_tok) * (m.heads / m.kv_heads), stream_rows = quantized_stream_rows(m, n_tok);
-    if ((w.route == kStream && (total + stream_rows - 1) / stream_rows > 65535) || (w.route == kSimt && quantized_rows_blocks(m, n_seq, n_tok, context) > 65535) ||
-        (w.route == kFlash && !flash_fits(m, n_seq, context)))
+    if ((w.route == kStream && (total + stream_rows - 1) / stream_rows > 65535) ||
+        (w.route == kSimt && quantized_rows_blocks(m, n_seq, n_tok, context) > 65535) || (w.route == kFlash && !flash_fits(m, n_seq, context)))
         return TBL_ERR_SHAPE;
     QuantizedParams p = basic_params(m, capacity, slots, positions, n_tok);
     if (!p.status) return TBL_ERR_CUDA;
     uint8_t* base = static_cast<uint8_t*>(ws);
     p.proj = proj; p.q_norm = m.rotation.q_norm; p.k_norm = m.rotation.k_norm; p.cache = static_cast<uint8_t*>(cache); p.out = out; p.eps = eps;
-    p.q = base + w.q; p.expanded = base + w.expanded; p.q_factor = w.route != kSimt ? reinterpret_cast<float*>(base + w.factor) : nullptr; p.ldo = padded16(p.d); p.part_m = reinterpret_cast<float*>(base + w.pm); p.part_l = reinterpret_cast<float*>(base + w.pl);
-    p.part_o = reinterpret_cast<float*>(base + w.po); p.splits = w.splits; p.ctx = w.ctx;
+    p.q = base + w.q; p.expanded = base + w.expanded; p.q_factor = w.route != kSimt ? reinterpret_cast<float*>(base + w.factor) : nullptr;
+    p.part_m = reinterpret_cast<float*>(base + w.pm); p.part_l = reinterpret_cast<float*>(base + w.pl); p.part_o = reinterpret_cast<float*>(base + w.po);
+    p.ldo = padded16(p.d); p.splits = w.splits; p.ctx = w.ctx;
     p.ldq = w.route == kStream ? p.width : w.route == kFlash ? padded16(p.d) : p.d;
     p.scale_log2 = static_cast<float>(static_cast<double>(m.scale) * m.key_scale * 1.4426950408889634);
     return run(m, precision, p, w, n_seq, st);
@@ -389,9 +396,9 @@ int tbl_quantized_read(const tbl_quantized_mixer* mixer, int precision, const vo
     const int most = ceil_div(static_cast<long long>(p.G) * p.width / 4, 256);
     const dim3 grid(static_cast<unsigned>(rows), most < 64 ? most : 64);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = precision == TBL_BF16
-                              ? launch_dependent(quantized_read_kernel<bf16>, grid, dim3(256), 0, st, p, static_cast<bf16*>(keys_dev), static_cast<bf16*>(values_dev))
-                              : launch_dependent(quantized_read_kernel<float>, grid, dim3(256), 0, st, p, static_cast<float*>(keys_dev), static_cast<float*>(values_dev));
+    auto launch = [&](auto kernel, auto* keys, auto* values) { return launch_dependent(kernel, grid, dim3(256), 0, st, p, keys, values); };
+    const cudaError_t e = precision == TBL_BF16 ? launch(quantized_read_kernel<bf16>, static_cast<bf16*>(keys_dev), static_cast<bf16*>(values_dev))
+                                                : launch(quantized_read_kernel<float>, static_cast<float*>(keys_dev), static_cast<float*>(values_dev));
     return e == cudaSuccess ? TBL_OK : TBL_ERR_CUDA;
 }
 

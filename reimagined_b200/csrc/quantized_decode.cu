@@ -1,19 +1,22 @@
-// Attention of a few query rows over a long 4-bit cache (decode, short portions): the rows of 4-bit numbers stream through shared memory once per block of 8 or 16
-// query rows that share a key/value head, and become matrix operands in registers.
+// Attention of a few query rows over a long 4-bit cache (decode, short portions): the rows of 4-bit numbers stream through shared memory once per
+// block of 8 or 16 query rows that share a key/value head, and become matrix operands in registers.
 //
 // Code x scale (e2m1 x e4m3: six bits between 2^-10 and 2688) is exact in fp16, so the products are warp-level MMAs (16 x 8 x 16, fp16 operands, fp32
-// sums) of exact keys and values; queries are rounded to fp16 under a power of two per head, softmax weights to fp16 (2^-12 each, where the bf16 result is rounded by
-// 2^-9): the largest weight stands at 2^11, so that one down to 2^-25 of it keeps its bits, 2^-35 is left out.  Scores are made as S^T = K Q^T and outputs as O^T = V^T P^T: cached numbers are the A operand, whose 16 x 16 numbers a step cost the fewest MMAs, and the
-// fragments of S^T turn into those of P^T by one transposed 8 x 8 move each.
+// sums) of exact keys and values; queries are rounded to fp16 under a power of two per head, softmax weights to fp16 (2^-12 each, where the bf16
+// result is rounded by 2^-9): the largest weight stands at 2^11, so that one down to 2^-25 of it keeps its bits, 2^-35 is left out.  Scores are made
+// as S^T = K Q^T and outputs as O^T = V^T P^T: cached numbers are the A operand, whose 16 x 16 numbers a step cost the fewest MMAs, and the fragments
+// of S^T turn into those of P^T by one transposed 8 x 8 move each.
 //
-// The order of the dimensions inside an MMA is free as long as both operands agree, so a lane takes 16 neighbouring dimensions of a token's key -- one scale -- for four steps, and
-// eight of a value.  For the values two tokens' codes are brought side by side while they are still 4 bits wide (two logic operations for sixteen numbers).
-// A warp of W works alone on every W-th tile of 32 tokens of the CTA's split: a ring of bulk copies of its own, its own maxima, sums and outputs; the warps meet in
-// shared memory at the end, splits of the context in quantized_merge_kernel.
+// The order of the dimensions inside an MMA is free as long as both operands agree, so a lane takes 16 neighbouring dimensions of a token's key --
+// one scale -- for four steps, and eight of a value.  For the values two tokens' codes are brought side by side while they are still 4 bits wide (two
+// logic operations for sixteen numbers).  A warp of W works alone on every W-th tile of 32 tokens of the CTA's split: a ring of bulk copies of its
+// own, its own maxima, sums and outputs; the warps meet in shared memory at the end, splits of the context in quantized_merge_kernel.
 //
-// Bound: turning 4 bits into halves.  A tile of 16 tokens of a head of 128 (2304 bytes, 100 cycles of an SM's share of the memory) costs 64 conversions and some 40 logic
-// operations on one pipe (two warps a cycle), 64 multiplications on another, 16 MMAs: some 300 instructions.  One token of 64 sequences of 8 heads over 4096: 74 us with the
-// kernel ahead, 4.2 TB/s of 302 MB; of one sequence over 131001 46 us (58 % of the issue slots, the conversions' pipe 50 %).
+// No single pipe bounds it.  A tile of 16 tokens of a head of 128 (2304 bytes, 100 cycles of an SM's share of the memory) costs 64 conversions and
+// some 40 logic operations on one pipe (two warps a cycle), 64 multiplications on another, 16 MMAs: some 300 instructions.  One token of 64 sequences
+// of 8 heads over 4096: 74 us with the kernel ahead, 4.2 TB/s of 302 MB; of one sequence over 131001 46 us, of which this kernel has 37: 58 % of the
+// issue slots, the conversions' pipe 51 %, MMAs 25 %, memory 0.63 of a copy's rate, and warps (sixteen to an SM) that wait as long for their turn as
+// for results and for the pipe.
 #include <float.h>
 
 #include "attention.cuh"
@@ -36,7 +39,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// the eight codes of a word as four pairs of halves, times a pair of scales (as one piece of assembly the conversions take their byte of the word by themselves)
+// the eight codes of a word as four pairs of halves, times a pair of scales (as one piece of assembly the conversions take their byte of the word by
+// themselves)
 __device__ __forceinline__ void widen(uint32_t codes, __half2 scale, uint32_t (&out)[4]) {
     asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %4;\ncvt.rn.f16x2.e2m1x2 %0, a;\ncvt.rn.f16x2.e2m1x2 %1, b;\ncvt.rn.f16x2.e2m1x2 %2, c;\ncvt.rn.f16x2.e2m1x2 %3, d;\n}"
         : "=r"(out[0]), "=r"(out[1]), "=r"(out[2]), "=r"(out[3]) : "r"(codes));
@@ -65,8 +69,8 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) { uint2 v; asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a)); return v; }
 
-// The token (of 16) that stands in row i of an MMA: with rows of 144 bytes the 16 or 32 lanes that a shared-memory access serves together then hit every bank once,
-// for the keys (rows 0 .. 3 and 4 .. 7 of the MMA) as for the values (rows 0, 2, 4, 6 and so on).
+// The token (of 16) that stands in row i of an MMA: with rows of 144 bytes the 16 or 32 lanes that a shared-memory access serves together then hit
+// every bank once, for the keys (rows 0 .. 3 and 4 .. 7 of the MMA) as for the values (rows 0, 2, 4, 6 and so on).
 __device__ __forceinline__ int token_of(int i) {
     const int r = i & 7;
     return ((r & 1) ? 8 + (((r & 6) + 4) & 7) : r) + (i >> 3);
@@ -78,9 +82,9 @@ struct Layout {
     static constexpr size_t kMerge = sizeof(float) * W * 8 * NT * kLdo, kBytes = kRing > kMerge ? kRing : kMerge;
 };
 
-// The bound on registers is what shared memory leaves blocks for (left to itself the compiler saves some that bring no further block: 64 sequences over 4096 tokens 77
-// instead of 74 us; five blocks with two stages each 74, six 81).
-// DP: the head size rounded up to 64; NT: blocks of eight query rows; W: warps; V: 0, or how the vectors of a whole call (StreamPlan) are read (HeadUnits).
+// The bound on registers is what shared memory leaves blocks for (left to itself the compiler saves some that bring no further block: 64 sequences
+// over 4096 tokens 77 instead of 74 us; five blocks with two stages each 74, six 81). DP: the head size rounded up to 64; NT: blocks of eight query
+// rows; W: warps; V: 0, or how the vectors of a whole call (StreamPlan) are read (HeadUnits).
 template <int DP, int NT, int W, int V>
 __global__ void __launch_bounds__(32 * W, W == 16 || DP > 128 ? 1 : NT == 1 ? 4 : 3) quantized_stream_kernel(const QuantizedParams p) {
     using L = Layout<DP, NT, W>;
@@ -283,7 +287,8 @@ __global__ void __launch_bounds__(32 * W, W == 16 || DP > 128 ? 1 : NT == 1 ? 4 
                     pt[h][u][r] = transposed(*reinterpret_cast<const uint32_t*>(&w));
                 }
         }
-        // rows nobody has written may hold anything: a weight of zero needs a finite value beside it (the split's last tile: nothing is loaded over it any more)
+        // rows nobody has written may hold anything: a weight of zero needs a finite value beside it (the split's last tile: nothing is loaded over
+        // it any more)
         if (t + kTile > t1) {
             if (t + lane >= t1)
 #pragma unroll
@@ -339,7 +344,8 @@ __global__ void __launch_bounds__(32 * W, W == 16 || DP > 128 ? 1 : NT == 1 ? 4 
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2)
-                    *reinterpret_cast<float4*>(dst + 64 * b + 2 * i) = make_float4(o[4 * b + i][u][e], o[4 * b + i][u][2 + e], o[4 * b + i + 1][u][e], o[4 * b + i + 1][u][2 + e]);
+                    *reinterpret_cast<float4*>(dst + 64 * b + 2 * i) =
+                        make_float4(o[4 * b + i][u][e], o[4 * b + i][u][2 + e], o[4 * b + i + 1][u][e], o[4 * b + i + 1][u][2 + e]);
         }
     __syncthreads();
     // the warps come together: sums of this split, over the first warp's
@@ -417,17 +423,17 @@ StreamPlan quantized_stream_plan(const tbl_quantized_mixer& m, int n_seq, int n_
     if (s > tokens) s = tokens;
     if (s > 1024) s = 1024;
     w.splits = w.most = s < 1 ? 1 : static_cast<int>(s);
-    // Instead of splits, whose sums another kernel joins: one CTA of sixteen warps an SM.  In the time of a tile (1.7 us with sixteen warps to an SM): what a warp takes
-    // one after the other, and 1.4 tiles for the other kernel, more with its blocks (a 64th for a unit up to 80) and splits (a 20th each).  One token of 32 and 8 heads,
-    // sixteen warps and splits: one sequence over 900 9.7 and 9.8 us, 2000 13.2 and 10.6, 8192 33.5 and 14.7; 8 over 2048 13.9 and 15.0, 4096 20.7 and 18.7;
-    // 18 over 4096 22 and 27; 30 over 4096 43 and 45.
+    // Instead of splits, whose sums another kernel joins: one CTA of sixteen warps an SM.  In the time of a tile (1.7 us with sixteen warps to an
+    // SM): what a warp takes one after the other, and 1.4 tiles for the other kernel, more with its blocks (a 64th for a unit up to 80) and splits (a
+    // 20th each).  One token of 32 and 8 heads, sixteen warps and splits: one sequence over 900 9.7 and 9.8 us, 2000 13.2 and 10.6, 8192 33.5 and
+    // 14.7; 8 over 2048 13.9 and 15.0, 4096 20.7 and 18.7; 18 over 4096 22 and 27; 30 over 4096 43 and 45.
     if (w.splits > 1 && m.dim <= 128) {
         const double wide = ceil_div(context, 16 * kTile) * static_cast<double>(ceil_div(units, kNumSm));
         const double split = ceil_div(context, 4LL * kTile * w.splits) + 1.4 + (units < 80 ? units : 80) / 64.0 + w.splits / 20.0;
         if (wide <= split) { w.warps = 16; w.splits = 1; }
     }
-    // As a whole one launch less, but fewer CTAs to an SM, whose own chains before the first tile show once they take turns (64 sequences of 8 heads over 4096 tokens
-    // 82 and 72 us, over 600 26 and 20, 37 over 4096 46 and 44)
+    // As a whole one launch less, but fewer CTAs to an SM, whose own chains before the first tile show once they take turns (64 sequences of 8 heads
+    // over 4096 tokens 82 and 72 us, over 600 26 and 20, 37 over 4096 46 and 44)
     w.whole = n_tok == 1 && w.splits == 1 && total <= rows && units <= (w.warps == 16 ? 1 : 2) * kNumSm;
     return w;
 }

@@ -1,9 +1,11 @@
 // Attention over a 4-bit cache in fp32 arithmetic: any head size, any number of query rows.
 //
-// A CTA has up to 16 query rows that share a key/value head and a split of the context; each of its four warps takes tiles of 32 tokens by itself, with its own maxima,
-// sums and outputs.  For the scores a lane has a token and turns its codes into numbers sixteen at a time (one scale), for all rows at once; for the outputs a lane
-// has neighbouring dimensions, and the tokens' weights come from shared memory.  Cached numbers so are read as they lie, 4 bits each, once per 16 rows.
-// Bound by its multiplications, one for a number and row, and for few tokens by latency (five sequences of three tokens over 777: 22 us of the chain of one tile a warp).
+// A CTA has up to 16 query rows that share a key/value head and a split of the context; each of its four warps takes tiles of 32 tokens by itself,
+// with its own maxima, sums and outputs.  For the scores a lane has a token and turns its codes into numbers sixteen at a time (one scale), for all
+// rows at once; for the outputs a lane has neighbouring dimensions, and the tokens' weights come from shared memory.  Cached numbers so are read as
+// they lie, 4 bits each, once per 16 rows.  Bound by latency: eight warps to an SM at sixteen rows (254 registers) leave 56 % of the issue slots and
+// 71 % of the multiplications' pipe unused while rows come (200 tokens behind 500, 32 and 8 heads of 128: 182 us), and few tokens take the chain of one
+// tile a warp (five sequences of three tokens over 777: 27 us, this kernel 15).
 #include "quantized.cuh"
 
 namespace tbl {
@@ -139,9 +141,9 @@ __global__ void __launch_bounds__(kThreads) quantized_rows_kernel(const Quantize
     }
 }
 
-// Query rows of a CTA.  Many of them share what a cached number costs; few of them are done sooner, where the CTAs at hand (`tiles`: splits at most, times sequences and
-// key/value heads) leave SMs empty (fp32, sixteen rows and as here: five sequences of three tokens over 777, 10 and 2 heads of 90, 28 and 22 us; four tokens over 300, 32 and 8
-// heads of 128, 27 and 17; 16 over 4000, 8 and 2 heads, 34 with sixteen rows, 36 with eight).
+// Query rows of a CTA.  Many of them share what a cached number costs; few of them are done sooner, where the CTAs at hand (`tiles`: splits at most,
+// times sequences and key/value heads) leave SMs empty (fp32, sixteen rows and as here: five sequences of three tokens over 777, 10 and 2 heads of
+// 90, 28 and 22 us; four tokens over 300, 32 and 8 heads of 128, 27 and 17; 16 over 4000, 8 and 2 heads, 34 with sixteen rows, 36 with eight).
 int rows_of(int width, long long total, long long tiles) {
     int r = total <= 4 ? 4 : total <= 8 || width > 128 ? 8 : 16;
     while (r > 4 && tiles * ceil_div(total, r) < 3 * kNumSm / 2) r /= 2;
