@@ -23,6 +23,17 @@ struct DecayParams {
     float scale, eps;
 };
 
+// What exp(log_decay) -- or several tokens' together, exp(log) -- leaves of a state s: m s + (slow ? s : 0).  A slow decay enters as 1 - exp(log),
+// which has 24 bits however slow it is, whereas a decay rounded to fp32 would be off by 2^-25 every token, all in one direction; a fast one as
+// itself, which has 24 bits however little it leaves, whereas 1 - exp(log) would be off by 2^-25 of the state before (as much
+// as is left of it after 17 in the exponent).  Where it is a token's the loops are there twice: a scan of 3 x 301 tokens 58.4 -> 59.4 us.
+struct Decay {
+    float m;
+    bool slow;
+    __device__ __forceinline__ explicit Decay(float log) : slow(log > -0.5f) { m = slow ? expm1f(log) : expf(log); }
+    __device__ __forceinline__ float of(float s) const { return fmaf(m, s, slow ? s : 0.0f); }
+};
+
 // decay_chunk.cu: prompts by chunks on the tensor cores
 bool decay_chunk_supported(const tbl_decay_mixer& m);
 size_t decay_chunk_workspace(const tbl_decay_mixer& m, int n_seq, int n_tok);

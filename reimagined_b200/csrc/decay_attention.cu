@@ -6,9 +6,10 @@
 //   decay_starts_kernel      long scans of few heads: the states before segments of the tokens, which are then scanned side by side
 // Prompts in bf16 go by chunks (decay_chunk.cu).
 //
-// The decay enters as S + (exp(log_decay) - 1) S: 1 - exp(log_decay) has 24 bits however slow the decay is, whereas a decay rounded to fp32 would be
-// off by 2^-25 every token, all in one direction.
+// A slow decay enters as S + (exp(log_decay) - 1) S, a fast one as exp(log_decay) S (Decay in decay.cuh).
 #include <float.h>
+
+#include <type_traits>
 
 #include "decay.cuh"
 #include "flash.cuh"
@@ -106,8 +107,9 @@ struct State {
             for (int j = 0; j < C; ++j)
                 if (row + r < d) *reinterpret_cast<ulonglong2*>(head + (row + r) * kKeys + 4 * share + 4 * LK * j) = make_ulonglong2(s[r][2 * j], s[r][2 * j + 1]);
     }
-    // one token: the state, and this lane's share of its rows' outputs; v: the rows' values (R floats, R a multiple of 4 on 16 bytes)
-    __device__ __forceinline__ void step(uint64_t less, const float* q, const float* k, const float* v, int share, float (&a)[R]) {
+    // one token: the state, and this lane's share of its rows' outputs; v: the rows' values (R floats, R a multiple of 4 on 16 bytes); m: of Decay, twice
+    template <bool SLOW>
+    __device__ __forceinline__ void step(uint64_t m, const float* q, const float* k, const float* v, int share, float (&a)[R]) {
         ulonglong2 qq[C], kk[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -125,8 +127,8 @@ struct State {
 #pragma unroll
                 for (int j = 0; j < C; ++j) {
                     uint64_t &x = s[r + e][2 * j], &y = s[r + e][2 * j + 1];
-                    x = fma2(kk[j].x, vv, fma2(less, x, x));
-                    y = fma2(kk[j].y, vv, fma2(less, y, y));
+                    x = fma2(kk[j].x, vv, fma2(m, x, SLOW ? x : 0));
+                    y = fma2(kk[j].y, vv, fma2(m, y, SLOW ? y : 0));
                     acc = fma2(qq[j].x, x, acc);
                     acc = fma2(qq[j].y, y, acc);
                 }
@@ -253,12 +255,12 @@ __global__ void __launch_bounds__(kThreads, 3) decay_step_kernel(const DecayPara
         x.template turn<float>(p.r, is_k ? p.k_norm : p.q_norm, p.eps, p.r.half > 0 ? min(max(pos + vec, 0), p.r.positions - 1) : 0, p.d, lane);
         x.store(p.r, (is_k ? k_s : q_s) + vec * S::kKeys, p.d, lane);
     }
-    const float l = expm1f(p.log_decay[head]);
-    const uint64_t less = pair_of(l, l);
+    const Decay decay(p.log_decay[head]);
+    const uint64_t m = pair_of(decay.m, decay.m);
     const bool alive = mbar_wait_bounded(&full, 0, p.status);
     __syncthreads();
     // four rows a lane at a time (d is a multiple of four: all there or none)
-    for (int r0 = warp * S::kRows; r0 < p.d; r0 += kThreads / 32 * S::kRows) {
+    auto rows = [&](auto slow, int r0) {
         const int r = r0 + lane / LK * 4;
         const bool in = r < p.d;
         S s;
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 3) decay_step_kernel(const DecayPara
             }
         for (int n = 0; n < p.n_tok; ++n) {
             float a[4];
-            s.step(less, q_s + n * S::kKeys, k_s + n * S::kKeys, v_s + n * p.d + (in ? r : 0), share, a);
+            s.template step<decltype(slow)::value>(m, q_s + n * S::kKeys, k_s + n * S::kKeys, v_s + n * p.d + (in ? r : 0), share, a);
             const float o = S::sums(a, share);
             if (in && S::writes(share)) o_s[n * p.d + r + S::row_at(share)] = o * p.scale;
         }
@@ -286,6 +288,10 @@ __global__ void __launch_bounds__(kThreads, 3) decay_step_kernel(const DecayPara
                 const int c = 4 * share + 4 * LK * j;
                 if (in && c < p.d) *reinterpret_cast<ulonglong2*>(mine + i * p.d + c) = make_ulonglong2(s.s[i][2 * j], s.s[i][2 * j + 1]);
             }
+    };
+    for (int r0 = warp * S::kRows; r0 < p.d; r0 += kThreads / 32 * S::kRows) {
+        if (decay.slow) rows(std::true_type{}, r0);
+        else rows(std::false_type{}, r0);
     }
     fence_proxy_async();
     __syncthreads();
@@ -350,48 +356,53 @@ __global__ void __launch_bounds__(kScanThreads) decay_scan_kernel(const DecayPar
     if constexpr (SUMS) s.clear();
     else if (p.segments > 1) s.load_padded(p.d, starts, row0 + first, share);
     else s.load(p, p.states + state, row0 + first, share);
-    const float rate = p.log_decay[head], l = expm1f(rate);
-    const uint64_t less = pair_of(l, l);
+    const float rate = p.log_decay[head];
+    const Decay decay(rate);
+    const uint64_t m = pair_of(decay.m, decay.m);
     const int row = row0 + first + S::row_at(share);
     const bool writes = S::writes(share) && row < p.d;
     float* raw = p.raw + (token0 * p.H + head) * p.d + row;
-    for (int t0 = 0, buf = 0; t0 < tokens; t0 += kTile, buf ^= 1) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();                                         // this tile is there, the one before it is no longer read
-        if (t0 + kTile < tokens) fetch(t0 + kTile, buf ^ 1);
-        const int n = min(kTile, tokens - t0);
-        if constexpr (SUMS) {
+    auto scan = [&](auto slow) {
+        for (int t0 = 0, buf = 0; t0 < tokens; t0 += kTile, buf ^= 1) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();                                         // this tile is there, the one before it is no longer read
+            if (t0 + kTile < tokens) fetch(t0 + kTile, buf ^ 1);
+            const int n = min(kTile, tokens - t0);
+            if constexpr (SUMS) {
 #pragma unroll 2
-            for (int t = 0; t < n; ++t) {
-                const float kept = expf(t0 + t == tokens - 1 ? 0.0f : rate * static_cast<float>(tokens - 1 - t0 - t));       // (a branch: 60 us instead of 58)
-                s.add(kept, vec_s[buf][t] + S::kKeys, vec_s[buf][t] + 2 * S::kKeys + first, share);
+                for (int t = 0; t < n; ++t) {
+                    const float kept = expf(t0 + t == tokens - 1 ? 0.0f : rate * static_cast<float>(tokens - 1 - t0 - t));       // (a branch: 60 us instead of 58)
+                    s.add(kept, vec_s[buf][t] + S::kKeys, vec_s[buf][t] + 2 * S::kKeys + first, share);
+                }
+                continue;
             }
-            continue;
-        }
-        auto token = [&](int t, float (&a)[R]) {
-            const float* v = vec_s[buf][t];
-            s.step(less, v, v + S::kKeys, v + 2 * S::kKeys + first, share, a);
-        };
-        int t = 0;
-        for (; t + 2 <= n; t += 2) {
-            float a[R], b[R];
-            token(t, a);
-            token(t + 1, b);
-            const float x = S::sums(a, share), y = S::sums(b, share);
-            if (writes) {
-                raw[0] = x * p.scale;
-                raw[static_cast<size_t>(p.H) * p.d] = y * p.scale;
+            auto token = [&](int t, float (&a)[R]) {
+                const float* v = vec_s[buf][t];
+                s.template step<decltype(slow)::value>(m, v, v + S::kKeys, v + 2 * S::kKeys + first, share, a);
+            };
+            int t = 0;
+            for (; t + 2 <= n; t += 2) {
+                float a[R], b[R];
+                token(t, a);
+                token(t + 1, b);
+                const float x = S::sums(a, share), y = S::sums(b, share);
+                if (writes) {
+                    raw[0] = x * p.scale;
+                    raw[static_cast<size_t>(p.H) * p.d] = y * p.scale;
+                }
+                raw += 2 * static_cast<size_t>(p.H) * p.d;
             }
-            raw += 2 * static_cast<size_t>(p.H) * p.d;
+            if (t < n) {
+                float a[R];
+                token(t, a);
+                const float x = S::sums(a, share);
+                if (writes) raw[0] = x * p.scale;
+                raw += static_cast<size_t>(p.H) * p.d;
+            }
         }
-        if (t < n) {
-            float a[R];
-            token(t, a);
-            const float x = S::sums(a, share);
-            if (writes) raw[0] = x * p.scale;
-            raw += static_cast<size_t>(p.H) * p.d;
-        }
-    }
+    };
+    if (SUMS || decay.slow) scan(std::true_type{});
+    else scan(std::false_type{});
     pdl_launch_dependents();
     if constexpr (SUMS) s.store_padded(p.d, starts + p.d * S::kKeys, row0 + first, share);
     else if (part == p.segments - 1) s.store(p, p.next + state, row0 + first, share);
@@ -405,7 +416,7 @@ __global__ void __launch_bounds__(256) decay_starts_kernel(const DecayParams p, 
     if (i >= numbers) return;
     const int head = unit % p.H, slot = p.slots[unit / p.H];
     float* at = p.starts + static_cast<size_t>(unit) * p.segments * numbers + i;
-    const float less = expm1f(p.log_decay[head] * static_cast<float>(p.segment));
+    const Decay decay(p.log_decay[head] * static_cast<float>(p.segment));
     float s = col < p.d ? p.states[((static_cast<size_t>(slot) * p.H + head) * p.d + row) * p.d + col] : 0.0f;
     float x[kMostSegments];
 #pragma unroll
@@ -414,7 +425,7 @@ __global__ void __launch_bounds__(256) decay_starts_kernel(const DecayParams p, 
 #pragma unroll
     for (int k = 1; k < kMostSegments; ++k)
         if (k < p.segments) {
-            s = fmaf(less, s, s) + x[k];
+            s = decay.of(s) + x[k];
             at[static_cast<size_t>(k) * numbers] = s;
         }
 }

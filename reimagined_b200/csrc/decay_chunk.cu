@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
         if (i < c.chunks) { x[i][0] = src[static_cast<size_t>(i) * DP * DP / 4]; x[i][1] = src[static_cast<size_t>(i) * DP * DP / 4 + DP]; }
-    const float less = expm1f(rate * static_cast<float>(kTokens));
+    const Decay whole(rate * static_cast<float>(kTokens));
     for (int i0 = 0; i0 < c.chunks; i0 += kAhead) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
@@ -383,10 +383,10 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
             *reinterpret_cast<uint4*>(c.images + at * DP * DP * 2 + swizzled(row, 8 * gl, DP * 128)) = make_uint4(h[0], h[1], h[2], h[3]);
             if (gl == 0) c.scales[at * DP + row] = power;
             const int n = min(kTokens, p.n_tok - c.first - i * kTokens);
-            const float l = n == kTokens ? less : expm1f(rate * static_cast<float>(n));
+            const Decay l = n == kTokens ? whole : Decay(rate * static_cast<float>(n));
             const float4 u = x[k][0], v = x[k][1];
-            s[0] = fmaf(l, s[0], s[0]) + u.x; s[1] = fmaf(l, s[1], s[1]) + u.y; s[2] = fmaf(l, s[2], s[2]) + u.z; s[3] = fmaf(l, s[3], s[3]) + u.w;
-            s[4] = fmaf(l, s[4], s[4]) + v.x; s[5] = fmaf(l, s[5], s[5]) + v.y; s[6] = fmaf(l, s[6], s[6]) + v.z; s[7] = fmaf(l, s[7], s[7]) + v.w;
+            s[0] = l.of(s[0]) + u.x; s[1] = l.of(s[1]) + u.y; s[2] = l.of(s[2]) + u.z; s[3] = l.of(s[3]) + u.w;
+            s[4] = l.of(s[4]) + v.x; s[5] = l.of(s[5]) + v.y; s[6] = l.of(s[6]) + v.z; s[7] = l.of(s[7]) + v.w;
             if (i + kAhead < c.chunks) {
                 x[k][0] = src[static_cast<size_t>(i + kAhead) * DP * DP / 4];
                 x[k][1] = src[static_cast<size_t>(i + kAhead) * DP * DP / 4 + DP];

@@ -6,7 +6,7 @@ import pytest
 
 from oracle import layer_stack as O
 from rotated_helpers import Decay, Quantized, f64, stream, tables
-from test_gpu_rotated_mixers import CHUNK, FLASH, SIMT, STREAM, cfg4, cfgd
+from test_gpu_rotated_mixers import CHUNK, FLASH, SCAN, SIMT, STREAM, cfg4, cfgd
 
 pytestmark = pytest.mark.gpu
 
@@ -230,3 +230,52 @@ def test_quantized_queries_of_very_different_sizes(cuda, stack_lib, precision, r
     a.oracle([1], before)
     want, got = a.oracle([1], rows), a.forward(route, [1], rows)
     own_rows_close(got.reshape(-1, 64), want.reshape(-1, 64), 2.0 ** -7 if precision else 2e-5, "heads")
+
+
+@pytest.mark.parametrize("precision,route,n,dim", [(0, 0, 1, 64), (0, 0, 4, 128), (0, SCAN, 9, 64), (0, SCAN, 9, 90), (0, SCAN, 9, 256), (1, 0, 2, 128), (1, SCAN, 9, 128), (1, CHUNK, 9, 128),
+                                                   (1, CHUNK, 2, 64)])
+def test_decay_fast_decays_of_what_is_left(cuda, stack_lib, precision, route, n, dim):
+    """After a token come ones without key or value (padding, say), which only read: what fast decays leave of the state keeps its bits, as little as it is.
+    Six tokens' decays are off by three half steps each (two units in the last place of exp, a rounding), all of them together as one exponential by 48 x 2^-24 of its
+    argument and two units: 4e-6."""
+    rates = [-0.3, -0.49, -0.51, -0.7, -2.0, -5.0, -8.0]
+    a = Decay(cuda, stack_lib, cfgd(len(rates), dim, 0, 0.1, gated=False, norm=False), precision, norm=False, rates=rates)
+    rng = np.random.default_rng(n)
+    proj = rng.standard_normal((n, a.cols)).astype(np.float32)
+    a.forward(route, [1], proj)
+    a.oracle([1], proj)
+    left = 6
+    while left:
+        take = min(left, n)
+        proj = rng.standard_normal((take, a.cols)).astype(np.float32)
+        for p in parts(a, proj):
+            p[:] = 0
+        queries = a.heads(proj, a.memory[1]["at"])[0]
+        want, got = a.oracle([1], proj), a.forward(route, [1], proj)
+        # S q: four standard deviations of the operands' roundings (chunks: fp16) or of some ten fp32 ones, where its terms cancel as they do
+        S = a.memory[1]["S"]
+        o, size = (np.sqrt((np.einsum("hvk,thk->thv", x, y) ** p).mean(axis=2)) for x, y, p in ((S, queries, 2), (S ** 2, queries ** 2, 1)))
+        step = (2.0 ** -12 * np.sqrt(2 / 3) if route == CHUNK else 2.0 ** -24 * np.sqrt(10)) * size / o
+        own_rows_close(got.reshape(-1, dim), want.reshape(-1, dim), (4 * step + (2.0 ** -8 if precision else 0) + 4e-6).ravel(), "rows")
+        left -= take
+    got, want = f64(a.states[1]), a.memory[1]["S"]
+    for h in range(a.H):
+        assert np.abs(got[h] - want[h]).max() <= 4e-6 * np.abs(want[h]).max() + (5 * np.sqrt(2 * n / 12) * 2.0 ** -23) * np.abs(want[h]).max(), a.rates[h]
+
+
+@pytest.mark.parametrize("precision,route,dim", [(0, SCAN, 64), (0, SCAN, 90), (1, SCAN, 128), (1, CHUNK, 128), (1, CHUNK, 90)])
+@pytest.mark.parametrize("zeros", [40, 128, 200])
+def test_decay_of_a_state_over_padding(cuda, stack_lib, precision, route, dim, zeros):
+    """A prompt behind which as many tokens of zeros follow as leave e^-45 of its state, in one call (segments, chunks): the argument's rounding 45 x 2^-24, two units of
+    exp for each of its up to three factors, a rounding each token (scan: the decay's own, at most 2^-23, too): 200 x 2^-23 at most."""
+    rates = [-45.0 / zeros, -20.0 / zeros, -2.0 / zeros]
+    a = Decay(cuda, stack_lib, cfgd(3, dim, 0, 0.1, gated=False, norm=False), precision, norm=False, rates=rates)
+    rng = np.random.default_rng(zeros)
+    proj = rng.standard_normal((100 + zeros, a.cols)).astype(np.float32)
+    for p in parts(a, proj):
+        p[100:] = 0
+    a.oracle([1], proj)
+    a.forward(route, [1], proj)
+    got, want = f64(a.states[1]), a.memory[1]["S"]
+    for h in range(a.H):
+        assert np.abs(got[h] - want[h]).max() <= 200 * 2.0 ** -23 * np.abs(want[h]).max(), a.rates[h]
