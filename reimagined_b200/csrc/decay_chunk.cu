@@ -346,7 +346,6 @@ __global__ void __launch_bounds__(kSumThreads, 2) decay_sums_kernel(const ChunkP
 template <int DP>
 __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
     constexpr int kLph = DP / 8, kSide = 32 / kLph;
-    pdl_launch_dependents();
     pdl_wait();
     const DecayParams& p = c.d;
     const int lane = threadIdx.x & 31, gl = lane % kLph, row = (blockIdx.x * 4 + (threadIdx.x >> 5)) * kSide + lane / kLph, unit = blockIdx.y;
@@ -393,6 +392,9 @@ __global__ void __launch_bounds__(128) decay_join_kernel(const ChunkParams c) {
             }
         }
     }
+    // (only now: CTAs of the next kernel that come early find room on few SMs, two to one, and stay there; 32 heads, 128 tokens 26 to 31 us as it
+    // fell out and 26 so, 512 tokens 38 and 30)
+    pdl_launch_dependents();
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (row < p.d && 8 * gl + e < p.d) p.next[state + 8 * gl + e] = s[e];

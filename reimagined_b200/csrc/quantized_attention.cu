@@ -177,7 +177,7 @@ bool flash_fits(const tbl_quantized_mixer& m, int n_seq, int context) {
 }
 
 // bf16: the flash kernel where its time, worked out from what it took, is shorter than the streaming kernel's (32 query and 8 key/value heads of 128,
-// in us, streaming and flash kernel: one sequence of 64 tokens over 1024 20 and 43, over 16384 97 and 287; 256 over 4096 115 and 109; 512 over 512 58
+// in us, streaming and flash kernel: one sequence of 64 tokens over 1024 20 and 43, over 16384 102 and 287; 256 over 4096 115 and 109; 512 over 512 58
 // and 45; eight sequences of 64 over 4096 193 and 233, of 128 over 128 86 and 64, over 4096 372 and 244).  Both read or walk the context: the one for
 // every block of 8 or 16 query rows, the other a wave of CTAs at a time.
 int pick_route(const tbl_quantized_mixer& m, int precision, int n_seq, int n_tok, int context) {
